@@ -99,6 +99,43 @@ NVFP4_MLA_API int nvfp4_mla_decode_multi(const void* q_nope, const void* q_pe, c
                      float ckv_scale, float kpe_scale, int max_kv_len, int num_splits, int precision, void* out,
                      float* out_f32, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* nvfp4_mla_decode (16-bit mode, num_splits 0) over a sliding window: the query token of a request, its last one, attends to
+ * the last `window` tokens of its cache, itself among them, and to the first `sink_tokens` tokens. Arguments as there, and
+ *
+ *   page_table_width  columns of page_table that hold page ids. Pages that hold no visible token are not looked up: their entries
+ *                     may hold anything (a serving engine has returned them to its pool)
+ *   status            optional device int: receives the codes of nvfp4_mla_workspace_status (the caller zeroes it); NULL: the
+ *                     workspace's first word receives them
+ *   workspace         at least nvfp4_mla_decode_window_workspace_bytes() bytes, 256-byte aligned; nothing in it is kept between calls
+ *
+ * What is read and multiplied is the visible tokens, in whole pages. Kernels launched: one more than nvfp4_mla_decode's. (No
+ * counterpart in the reference.) */
+NVFP4_MLA_API int64_t nvfp4_mla_decode_window_workspace_bytes(int batch, int heads, int page_size, int page_table_width, int window,
+                                                              int sink_tokens);
+NVFP4_MLA_API int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
+                     const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table,
+                     int64_t page_table_stride, int page_table_width, const int32_t* kv_lens, int batch, int heads, float sm_scale,
+                     float ckv_scale, float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, float* out_f32, float* lse,
+                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* Attention of a chunk of new tokens per request (chunked prefill): the query tokens qo_indptr[b] .. qo_indptr[b + 1] are the last
+ * ones of request b's kv_lens[b] cached tokens (their rows are in the cache), and each attends to the tokens up to its own
+ * position; with window > 0 to the last `window` of these, itself among them, and to the first `sink_tokens`.
+ *
+ *   q_nope, q_pe  [total_q, heads, 512] and [total_q, heads, 64] bfloat16;  out [total_q, heads, 512] bfloat16
+ *   qo_indptr     [batch + 1] int32, non-decreasing, read on the device. Query tokens of no request (before qo_indptr[0], at or
+ *                 behind qo_indptr[batch]) and tokens in front of a request's first (more new tokens than kv_lens) give zeros
+ *   window        0: none
+ *   others        as in nvfp4_mla_decode_window; 16-bit arithmetic
+ * (No counterpart in the reference, which decodes one query token per request.) */
+NVFP4_MLA_API int64_t nvfp4_mla_extend_workspace_bytes(int batch, int total_q, int heads, int page_size, int page_table_width, int max_kv_len,
+                                                       int window, int sink_tokens);
+NVFP4_MLA_API int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
+                     const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table, int64_t page_table_stride,
+                     int page_table_width, const int32_t* kv_lens, const int32_t* qo_indptr, int batch, int total_q, int heads, float sm_scale,
+                     float ckv_scale, float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, void* workspace,
+                     int64_t workspace_bytes, int32_t* status, void* stream);
+
 /* nvfp4_mla_decode for callers that have no way to hand over scratch memory. (No counterpart in the reference, whose
  * launcher always allocates its partial buffers through torch.)
  *
@@ -177,6 +214,42 @@ NVFP4_MLA_API int nvfp4_mla_quantize_append(const void* ckv, const void* kpe, co
                               uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* kv_indices,
                               const int32_t* kv_indptr, int batch, float ckv_scale, float kpe_scale, int32_t* status,
                               void* stream);
+
+/* The cache writer behind the latent projection, in one pass: row i's latent part is normalised, its rope part rotated, and both
+ * are quantised and appended as by nvfp4_mla_quantize_append (same tables, same status).
+ *
+ *   ckv          row i at ckv + i * ckv_stride (bfloat16 elements; a multiple of 8, 16-byte aligned): 512 raw latent channels
+ *   kpe          row i at kpe + i * kpe_stride (a multiple of 2, 4-byte aligned): 64 raw rope channels; both may be columns of
+ *                one [nnz, 576] projection
+ *   norm_weight  [512] bfloat16
+ *   cos_sin      [max_position, 64] float: the cosines of the 32 angles of a position, then their sines
+ *   interleaved  1: the rotated pairs are channels (2k, 2k + 1); 0: (k, k + 32)
+ *
+ * y = norm_weight * x / sqrt(mean(x^2) + eps) and the rotated pair (a cos - b sin, b cos + a sin) are fp32 numbers rounded from
+ * 64-bit arithmetic, then rounded to bfloat16; the cache's bytes are those the writer makes of these bfloat16 rows. The row of cos_sin
+ * is positions[i]; a token with positions[i] >= max_position is skipped like one outside the tables. (No counterpart in the
+ * reference, whose writer takes normalised and rotated rows.) */
+NVFP4_MLA_API int nvfp4_mla_norm_rope_append(const void* ckv, int64_t ckv_stride, const void* kpe, int64_t kpe_stride,
+                                             const void* norm_weight, const float* cos_sin, int max_position, double eps, int interleaved,
+                                             const int32_t* batch_indices, const int32_t* positions, int64_t nnz, uint8_t* ckv_cache,
+                                             uint8_t* ckv_sf_cache, uint8_t* kpe_cache, int64_t num_pages, int page_size,
+                                             const int32_t* kv_indices, const int32_t* kv_indptr, int batch, float ckv_scale,
+                                             float kpe_scale, int32_t* status, void* stream);
+
+/* Ranges of tokens out of the pages, dequantised into contiguous rows: output row i, indptr[b] <= i < indptr[b + 1], is token
+ * starts[b] + i - indptr[b] of request b (starts NULL: 0), in the arithmetic of nvfp4_mla_dequantize.
+ *
+ *   page_table   [batch, page_table_stride] int32, of which page_table_width columns are page ids
+ *   indptr       [batch + 1] int32, non-decreasing, read on the device; rows before indptr[0], at or behind indptr[batch] and at or
+ *                behind `total` are left as they are
+ *   ckv_out      [total, 512] float (out_bf16 = 0) or bfloat16 (1), 16-byte aligned;  kpe_out [total, 64] likewise, 8-byte aligned
+ *   status       optional device word, set to 1 if a token lies outside the page table or on a page outside the cache: its row is 0
+ *
+ * (The reference reads whole caches only: nvfp4_mla/csrc/mla_decode.cu:1113-1132.) */
+NVFP4_MLA_API int nvfp4_mla_gather(const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, const uint8_t* kpe_cache, int64_t num_pages,
+                                   int page_size, const int32_t* page_table, int64_t page_table_stride, int page_table_width,
+                                   const int32_t* indptr, const int32_t* starts, int batch, int64_t total, float ckv_scale,
+                                   float kpe_scale, int out_bf16, void* ckv_out, void* kpe_out, int32_t* status, void* stream);
 
 /* Log-sum-exp merge of `parts` partial results: o_part [parts, rows, 512] float (each normalised by its own
  * softmax sum), lse_part [parts, rows] float in log2 units (-inf = empty partial, weight 0); parts <= 512. Any of out

@@ -5,13 +5,14 @@ Drop-in for the reference project's ``nvfp4_mla`` package (nvfp4_mla/__init__.py
 ``libnvfp4_mla_b200.so`` behind a C ABI (``include/nvfp4_mla_b200.h``); torch only owns the memory and the stream.
 """
 import functools
+import operator
 
 import torch
 
 from . import _lib
 
-__all__ = ["decode", "dequantize", "decode_partial", "combine", "combine_packed", "combine_records", "combine_records_signalled", "workspace_status", "quantize_append_paged_mla_kv_cache",
-           "get_batch_indices_positions"]
+__all__ = ["decode", "decode_window", "extend", "dequantize", "decode_partial", "combine", "combine_packed", "combine_records", "combine_records_signalled", "workspace_status", "quantize_append_paged_mla_kv_cache",
+           "norm_rope_append_paged_mla_kv_cache", "gather_paged_mla_kv_cache", "get_batch_indices_positions"]
 __version__ = "0.1.0"
 
 CKV, KPE = 512, 64
@@ -158,6 +159,138 @@ def decode(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens
         raise ValueError(f"precision must be one of {list(_PRECISIONS)}, got {precision!r}")
     return _decode(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens, sm_scale, ckv_scale,
                    kpe_scale, max_kv_len, num_splits, _PRECISIONS[precision], True, False)[0]
+
+
+_statuses = {}  # device index -> int32 word that the kernels of the calls below report to, sticky
+
+
+def _status(dev):
+    """The device's status word; None while a graph is captured before any call has made it."""
+    word = _statuses.get(dev.index)
+    if word is None and not torch.cuda.is_current_stream_capturing():
+        word = _statuses[dev.index] = torch.zeros(1, dtype=torch.int32, device=dev)
+    return word
+
+
+@functools.lru_cache(maxsize=4096)
+def _window_bytes(device_index, batch, heads, page_size, width, window, sink_tokens):
+    nbytes = _lib.load().nvfp4_mla_decode_window_workspace_bytes(batch, heads, page_size, width, window, sink_tokens)
+    if nbytes < 0:
+        raise RuntimeError(_lib.load().nvfp4_mla_last_error().decode())
+    return nbytes
+
+
+def _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale):
+    """What the calls below refuse of queries and tables; ``(query tokens, heads, requests)``."""
+    if q_nope.dim() != 3 or q_nope.shape[2] != CKV or q_pe.dim() != 3 or tuple(q_pe.shape) != (*q_nope.shape[:2], KPE):
+        raise RuntimeError("q_nope must be [tokens, heads, 512] and q_pe [tokens, heads, 64]")
+    if q_nope.dtype != torch.bfloat16 or q_pe.dtype != torch.bfloat16:
+        raise RuntimeError("q must be bfloat16")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise RuntimeError("page_table must be int32 [batch, max_pages] with contiguous rows")
+    B = page_table.shape[0]
+    if kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (B,):
+        raise RuntimeError("kv_lens must be int32 [batch]")
+    for t in (q_nope, q_pe, page_table, kv_lens):
+        if t.device != ckv_cache.device or (t is not page_table and not t.is_contiguous()):
+            raise RuntimeError("inputs must be contiguous and on the cache device")
+    if not (ckv_scale > 0 and kpe_scale > 0):
+        raise RuntimeError("ckv_scale and kpe_scale must be positive")
+    if ckv_cache.shape[1] & (ckv_cache.shape[1] - 1):
+        raise RuntimeError("page_size must be a power of two")
+    return (*q_nope.shape[:2], B)
+
+
+def _check_window(window, sink_tokens):
+    window, sink_tokens = operator.index(window), operator.index(sink_tokens)
+    if not (0 < window < 2 ** 31 and 0 <= sink_tokens < 2 ** 31):
+        raise ValueError("window must be positive and sink_tokens not negative, both below 2^31")
+    return window, sink_tokens
+
+
+def decode_window(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens, sm_scale, window, sink_tokens=0,
+                  ckv_scale=1.0, kpe_scale=1.0, max_kv_len=None):
+    """``decode`` over a sliding window: the query token of a request, its last one, attends to the last ``window`` tokens of its
+    cache (itself among them) and to the first ``sink_tokens`` tokens.
+
+    Arguments as for ``decode``, 16-bit arithmetic. Pages without a visible token are not looked up, so that they can go back to the
+    pool and their page-table entries may hold anything; the rows of ``page_table`` may be a slice of a wider one. What the call
+    reads grows with ``window + sink_tokens``, not with the length. ``max_kv_len`` bounds ``kv_lens`` as in ``decode``; without it the
+    page table's width does, and nothing synchronises either way. Returns ``[batch, heads, 512]`` bfloat16; ``workspace_status``
+    reports bad pages."""
+    window, sink_tokens = _check_window(window, sink_tokens)
+    _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
+    N, H, B = _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale)
+    if N != B:
+        raise RuntimeError("q_nope must be [batch, heads, 512]")
+    if H == 0 or H % 16 != 0:
+        raise RuntimeError("heads must be a multiple of 16")
+    dev, ps, width = ckv_cache.device, ckv_cache.shape[1], page_table.shape[1]
+    bound = min(width * ps, 2 ** 31 - 1)
+    max_kv_len = bound if max_kv_len is None else min(int(max_kv_len), bound)
+
+    def launch():
+        out = torch.empty(B, H, CKV, dtype=torch.bfloat16, device=dev)
+        ws = torch.empty(_window_bytes(dev.index, B, H, ps, width, window, sink_tokens), dtype=torch.uint8, device=dev)
+        _lib.check(_lib.load().nvfp4_mla_decode_window(
+            q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), ckv_cache.shape[0], ps,
+            page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), B, H, float(sm_scale), float(ckv_scale), float(kpe_scale),
+            max_kv_len, window, sink_tokens, out.data_ptr(), None, None, ws.data_ptr(), ws.numel(), _ptr(_status(dev)),
+            torch.cuda.current_stream(dev).cuda_stream))
+        return out
+
+    return _on_device(dev, launch)
+
+
+@functools.lru_cache(maxsize=4096)
+def _extend_bytes(device_index, *sizes):
+    nbytes = _lib.load().nvfp4_mla_extend_workspace_bytes(*sizes)
+    if nbytes < 0:
+        raise RuntimeError(_lib.load().nvfp4_mla_last_error().decode())
+    return nbytes
+
+
+def extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens, qo_indptr, sm_scale, ckv_scale=1.0, kpe_scale=1.0,
+           max_kv_len=None, window=0, sink_tokens=0):
+    """Attention of a chunk of new tokens per request over the paged cache (chunked prefill), causal, ragged.
+
+    Args:
+        q_nope: ``[total_q, heads, 512]`` bfloat16, the absorbed queries of all requests' new tokens, request by request.
+        q_pe: ``[total_q, heads, 64]`` bfloat16.
+        page_table: ``[batch, max_pages]`` int32; its rows may be a slice of a wider table.
+        kv_lens: ``[batch]`` int32, tokens per request WITH the new ones, which are the last and whose rows are in the cache.
+        qo_indptr: ``[batch + 1]`` int32, non-decreasing: request ``b`` has the query tokens ``qo_indptr[b] .. qo_indptr[b + 1]``.
+        max_kv_len: an upper bound of ``kv_lens``, which with the shapes fixes the launch shape and the workspace. Without it the page
+            table's width is the bound; nothing synchronises either way, and the call can be captured in a CUDA graph.
+        window, sink_tokens: with ``window > 0`` a token attends to the last ``window`` tokens up to its own position and to the first
+            ``sink_tokens``; pages that no query of the call sees are not looked up.
+
+    The caches, scales and ``sm_scale`` are those of ``decode``; 16-bit arithmetic. Returns ``[total_q, heads, 512]`` bfloat16. Query tokens of
+    no request (at or behind ``qo_indptr[-1]``: a padded batch) and tokens that see nothing give zeros. ``workspace_status`` reports
+    bad pages.
+    """
+    window, sink_tokens = _check_window(window, sink_tokens) if window else (0, _check_window(1, sink_tokens)[1])
+    _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
+    N, H, B = _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale)
+    if qo_indptr.dtype != torch.int32 or tuple(qo_indptr.shape) != (B + 1,) or not qo_indptr.is_contiguous() or qo_indptr.device != ckv_cache.device:
+        raise RuntimeError("qo_indptr must be a contiguous int32 [batch + 1] tensor on the cache device")
+    if H == 0:
+        raise RuntimeError("heads must be positive")
+    dev, ps, width = ckv_cache.device, ckv_cache.shape[1], page_table.shape[1]
+    bound = min(width * ps, 2 ** 31 - 1)
+    max_kv_len = bound if max_kv_len is None else min(int(max_kv_len), bound)
+
+    def launch():
+        out = torch.empty(N, H, CKV, dtype=torch.bfloat16, device=dev)
+        ws = torch.empty(_extend_bytes(dev.index, B, N, H, ps, width, max_kv_len, window, sink_tokens), dtype=torch.uint8, device=dev)
+        _lib.check(_lib.load().nvfp4_mla_extend(
+            q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), ckv_cache.shape[0], ps,
+            page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), qo_indptr.data_ptr(), B, N, H, float(sm_scale),
+            float(ckv_scale), float(kpe_scale), max_kv_len, window, sink_tokens, out.data_ptr(), ws.data_ptr(), ws.numel(),
+            _ptr(_status(dev)), torch.cuda.current_stream(dev).cuda_stream))
+        return out
+
+    return _on_device(dev, launch)
 
 
 def decode_partial(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens, sm_scale,
@@ -342,6 +475,90 @@ def _append(nnz, ckv, kpe, batch_indices, positions, ckv_cache, ckv_sf_cache, kp
         float(kpe_scale), _ptr(status), torch.cuda.current_stream(dev).cuda_stream)))
 
 
+def norm_rope_append_paged_mla_kv_cache(ckv, kpe, norm_weight, cos_sin, batch_indices, positions, ckv_cache, ckv_sf_cache, kpe_cache,
+                                        kv_indices, kv_indptr, eps=1e-6, ckv_scale=1.0, kpe_scale=1.0, interleaved=True, check=False):
+    """RMS-normalises, rotates, quantises and writes the latent projection's raw rows into the paged cache, in place and in one pass.
+
+    ``ckv [nnz, 512]`` and ``kpe [nnz, 64]`` are bfloat16 with contiguous rows; the row strides are free (multiples of 8 and 2
+    elements), so both may be columns of one ``[nnz, 576]`` projection. ``norm_weight [512]`` bfloat16, ``cos_sin [positions, 64]``
+    float32 (the 32 cosines of a position, then its sines); a token is rotated by the angles of its ``positions`` entry, in pairs
+    ``(2k, 2k + 1)`` (``interleaved``) or ``(k, k + 32)``. The normalised and the rotated row are rounded to bfloat16 once, from
+    64-bit arithmetic by way of fp32, and the cache receives the bytes that ``quantize_append_paged_mla_kv_cache`` makes of them;
+    the tables and ``check`` are that call's. A token past the end of ``cos_sin`` counts as outside the tables."""
+    _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
+    if ckv.dtype != torch.bfloat16 or kpe.dtype != torch.bfloat16 or norm_weight.dtype != torch.bfloat16 or cos_sin.dtype != torch.float32:
+        raise RuntimeError("ckv, kpe and norm_weight must be bfloat16 and cos_sin float32")
+    nnz = ckv.shape[0]
+    if tuple(ckv.shape) != (nnz, CKV) or tuple(kpe.shape) != (nnz, KPE):
+        raise RuntimeError("ckv must be [nnz, 512] and kpe [nnz, 64]")
+    strides = tuple(t.stride(0) if nnz > 1 else t.shape[1] for t in (ckv, kpe))  # (a single row has no stride to speak of)
+    if ckv.stride(1) != 1 or kpe.stride(1) != 1 or strides[0] < CKV or strides[0] % 8 or strides[1] < KPE or strides[1] % 2:
+        raise RuntimeError("rows of ckv and kpe must be contiguous, their strides multiples of 8 and 2 elements")
+    if tuple(norm_weight.shape) != (CKV,) or cos_sin.dim() != 2 or cos_sin.shape[1] != KPE or not (norm_weight.is_contiguous() and cos_sin.is_contiguous()):
+        raise RuntimeError("norm_weight must be a contiguous [512] and cos_sin a contiguous [positions, 64] tensor")
+    for name, t, n in (("batch_indices", batch_indices, nnz), ("positions", positions, nnz), ("kv_indices", kv_indices, None),
+                       ("kv_indptr", kv_indptr, None)):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
+            raise RuntimeError(f"{name} must be a contiguous 1-D int32 tensor" + (f" of {n} elements" if n is not None else ""))
+    dev = ckv_cache.device
+    if any(t.device != dev for t in (ckv, kpe, norm_weight, cos_sin, batch_indices, positions, kv_indices, kv_indptr)):
+        raise RuntimeError("inputs must be on the cache device")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    _on_device(dev, lambda: _lib.check(_lib.load().nvfp4_mla_norm_rope_append(
+        _ptr(ckv), strides[0], _ptr(kpe), strides[1], _ptr(norm_weight), _ptr(cos_sin), cos_sin.shape[0], float(eps), int(bool(interleaved)),
+        _ptr(batch_indices), _ptr(positions), nnz, _ptr(ckv_cache), _ptr(ckv_sf_cache), _ptr(kpe_cache), *ckv_cache.shape[:2],
+        _ptr(kv_indices), _ptr(kv_indptr), kv_indptr.numel() - 1, float(ckv_scale), float(kpe_scale), _ptr(status),
+        torch.cuda.current_stream(dev).cuda_stream)))
+    if check and int(status.item()) != 0:
+        raise RuntimeError("norm_rope_append: a token named a request, position or page outside the tables")
+
+
+def gather_paged_mla_kv_cache(ckv_cache, ckv_sf_cache, kpe_cache, page_table, indptr, total, starts=None, ckv_scale=1.0, kpe_scale=1.0,
+                              dtype=torch.bfloat16, out=None, check=False):
+    """Reads ranges of tokens out of the pages: ``(ckv [total, 512], kpe [total, 64])`` in ``dtype`` (bfloat16 or float32), the
+    arithmetic that of ``dequantize``.
+
+    Rows ``indptr[b] .. indptr[b + 1]`` are the tokens of request ``b`` from ``starts[b]`` on (default 0). ``page_table
+    [batch, max_pages]``, ``indptr [batch + 1]`` (non-decreasing) and ``starts [batch]`` are int32 and stay on the device; ``total`` is the
+    number of output rows, ``indptr[-1]`` or more. With ``out=(ckv, kpe)`` the rows go into those tensors, and rows that belong to no
+    request are left as they are (without, they are undefined). ``check=True`` synchronises and raises if a token lay outside the
+    page table or the cache (its row is 0)."""
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"dtype must be bfloat16 or float32, got {dtype}")
+    _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
+    dev = ckv_cache.device
+    total = operator.index(total)
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise RuntimeError("page_table must be int32 [batch, max_pages] with contiguous rows")
+    B = page_table.shape[0]
+    if indptr.dtype != torch.int32 or tuple(indptr.shape) != (B + 1,) or not indptr.is_contiguous():
+        raise RuntimeError("indptr must be a contiguous int32 [batch + 1] tensor")
+    if starts is not None and (starts.dtype != torch.int32 or tuple(starts.shape) != (B,) or not starts.is_contiguous()):
+        raise RuntimeError("starts must be a contiguous int32 [batch] tensor")
+    if any(t is not None and t.device != dev for t in (page_table, indptr, starts)):
+        raise RuntimeError("inputs must be on the cache device")
+    if total < 0:
+        raise ValueError("total must not be negative")
+    if not (ckv_scale > 0 and kpe_scale > 0):
+        raise RuntimeError("ckv_scale and kpe_scale must be positive")
+    if out is None:
+        out = torch.empty(total, CKV, dtype=dtype, device=dev), torch.empty(total, KPE, dtype=dtype, device=dev)
+    ckv, kpe = out
+    if not (ckv.dtype == kpe.dtype == dtype and tuple(ckv.shape) == (total, CKV) and tuple(kpe.shape) == (total, KPE)
+            and ckv.is_contiguous() and kpe.is_contiguous() and ckv.device == dev and kpe.device == dev):
+        raise RuntimeError("out must be contiguous ([total, 512], [total, 64]) tensors of dtype on the cache device")
+    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    _on_device(dev, lambda: _lib.check(_lib.load().nvfp4_mla_gather(
+        _ptr(ckv_cache), _ptr(ckv_sf_cache), _ptr(kpe_cache), *ckv_cache.shape[:2], _ptr(page_table), page_table.stride(0),
+        page_table.shape[1], _ptr(indptr), _ptr(starts), B, total, float(ckv_scale), float(kpe_scale), int(dtype == torch.bfloat16),
+        _ptr(ckv), _ptr(kpe), _ptr(status), torch.cuda.current_stream(dev).cuda_stream)))
+    if check and int(status.item()) != 0:
+        raise RuntimeError("gather: a token lies outside the page table or on a page outside the cache")
+    return ckv, kpe
+
+
 def workspace_status(device=None, clear=False):
     """Synchronises and returns the worst device-side status of the decode workspaces of ``device`` (0 = fine,
     1 = a bounded wait inside the decode kernel gave up, 2 = schedule capacity exceeded, 3 = a page id inside a request's
@@ -361,4 +578,13 @@ def workspace_status(device=None, clear=False):
                 ws[:4].zero_()
                 torch.cuda.synchronize(idx)
             worst = max(worst, st)
+    for idx, word in _statuses.items():
+        if device is not None and torch.device(device).index not in (None, idx):
+            continue
+        with torch.cuda.device(idx):
+            torch.cuda.synchronize(idx)
+            worst = max(worst, int(word.item()))
+            if clear:
+                word.zero_()
+                torch.cuda.synchronize(idx)
     return worst

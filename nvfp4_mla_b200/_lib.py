@@ -8,7 +8,7 @@ import pathlib
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libnvfp4_mla_b200.so"
 
-_vp, _i32, _i64, _f32, _u32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_uint32
+_vp, _i32, _i64, _f32, _f64, _u32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_uint32
 
 # name -> (restype, argtypes); mirrors include/nvfp4_mla_b200.h
 SIGNATURES = {
@@ -23,6 +23,12 @@ SIGNATURES = {
     "nvfp4_mla_decode_multi_folds": (_i32, [_i32, _i32, _i32, _i32, _i32]),
     "nvfp4_mla_decode_multi": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _i32, _f32, _f32, _f32,
                                       _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "nvfp4_mla_decode_window_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "nvfp4_mla_decode_window": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i32, _f32, _f32, _f32, _i32, _i32, _i32,
+                                       _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "nvfp4_mla_extend_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "nvfp4_mla_extend": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _f32, _f32, _i32, _i32,
+                                _i32, _vp, _vp, _i64, _vp, _vp]),
     "nvfp4_mla_decode_static": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _f32, _f32, _f32,
                                        _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "nvfp4_mla_decode_static_capacity": (_i64, []),
@@ -37,6 +43,9 @@ SIGNATURES = {
     "nvfp4_mla_combine_records_signalled": (_i32, [_vp, _vp, _i32, _u32, _i64, _i32, _i64, _vp, _vp, _vp, _vp, _vp]),
     "nvfp4_mla_quantize_append": (_i32, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _f32, _f32,
                                          _vp, _vp]),
+    "nvfp4_mla_norm_rope_append": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _f64, _i32, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _vp,
+                                          _vp, _i32, _f32, _f32, _vp, _vp]),
+    "nvfp4_mla_gather": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _i64, _f32, _f32, _i32, _vp, _vp, _vp, _vp]),
 }
 
 

@@ -16,8 +16,10 @@
 #include "mla_decode_hm_sm100.cuh"
 #include "mla_decode_hm16_sm100.cuh"
 #include "mla_dequant.cuh"
+#include "mla_gather.cuh"
 #include "mla_quantize.cuh"
 #include "mla_schedule.cuh"
+#include "mla_window.cuh"
 
 namespace {
 
@@ -102,13 +104,14 @@ int schedule_units(const DeviceInfo& d, int precision, int hpc) {
 }
 int ctas_per_unit(int hpc) { return runs_on_pairs(hpc) ? 2 : 1; }
 // the kernels that take tensor maps (all but the 16-bit heads-as-M kernel)
-DecodeKernel decode_kernel(int precision, int hpc) {
+DecodeKernel decode_kernel(int precision, int hpc, bool window = false) {
   if (precision == NVFP4_MLA_PRECISION_FP8)
     return hpc == 128  ? mla::mla_decode_hm_kernel<kRawSlotsHm>
            : hpc == 32 ? mla::mla_decode_kernel<32, kRawSlots8, true>
                        : mla::mla_decode_kernel<16, kRawSlots8, true>;
-  return mla::mla_decode_vt_kernel;
+  return window ? mla::mla_decode_vt_kernel<true> : mla::mla_decode_vt_kernel<false>;
 }
+auto hm16_kernel(bool window) { return window ? mla::mla_decode_hm16_kernel<true> : mla::mla_decode_hm16_kernel<false>; }
 unsigned decode_threads(int precision, int hpc) {
   if (precision == NVFP4_MLA_PRECISION_FP8) return hpc == 128 ? mla::kHmThreads : mla::kDecodeThreads;
   return hpc > 16 ? mla::kH16Threads : mla::kVtThreads;
@@ -120,9 +123,9 @@ size_t decode_smem(int precision, int hpc) {
                        : mla::decode_smem_bytes<16, kRawSlots8, true>();
   return hpc > 16 ? mla::h16_smem_bytes() : mla::vt_smem_bytes();
 }
-const void* decode_entry(int precision, int hpc) {
-  if (precision != NVFP4_MLA_PRECISION_FP8 && hpc > 16) return reinterpret_cast<const void*>(mla::mla_decode_hm16_kernel);
-  return reinterpret_cast<const void*>(decode_kernel(precision, hpc));
+const void* decode_entry(int precision, int hpc, bool window = false) {
+  if (precision != NVFP4_MLA_PRECISION_FP8 && hpc > 16) return reinterpret_cast<const void*>(hm16_kernel(window));
+  return reinterpret_cast<const void*>(decode_kernel(precision, hpc, window));
 }
 static_assert(mla::h16_smem_bytes() <= 232448, "16-bit heads-as-M kernel exceeds the shared memory a CTA can opt in to");
 static_assert(mla::hm_smem_bytes<kRawSlotsHm>() <= 232448, "heads-as-M kernel exceeds the shared memory a CTA can opt in to");
@@ -146,6 +149,9 @@ int device_info(DeviceInfo** out) {
       for (int hpc : {16, 32, 128})
         MLA_CUDA(cudaFuncSetAttribute(decode_entry(prec, hpc), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       int(decode_smem(prec, hpc))));
+    for (int hpc : {16, 128})
+      MLA_CUDA(cudaFuncSetAttribute(decode_entry(NVFP4_MLA_PRECISION_BF16, hpc, true), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    int(decode_smem(NVFP4_MLA_PRECISION_BF16, hpc))));
     {  // clusters of two need both SMs in one GPC: ask how many can be resident rather than assuming sm_count / 2
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(unsigned(d.sm_count / 2 * 2)), cfg.blockDim = dim3(mla::kHmThreads);
@@ -309,12 +315,15 @@ int64_t nvfp4_mla_decode_workspace_bytes(int batch, int heads, int num_splits) {
 }
 
 // The decode call proper; `heads` counts the rows of all q_len query tokens of a request, `hpc_limit` caps the heads per CTA
-// (see heads_per_cta), which are chosen for requests of `expected_kv_len` tokens (0: of the bound max_kv_len).
+// (see heads_per_cta), which are chosen for requests of `expected_kv_len` tokens (0: of the bound max_kv_len). `dead`: the tokens of
+// each request that are not seen (windowed decode, 16-bit mode), or null; `status`: where the kernels report, or null for the
+// workspace's first word.
 static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
                        const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table,
                        int64_t page_table_stride, const int32_t* kv_lens, int batch, int heads, float sm_scale, float ckv_scale,
                        float kpe_scale, int max_kv_len, int num_splits, int precision, void* out, float* out_f32, float* lse,
-                       void* workspace, int64_t workspace_bytes, void* stream, int hpc_limit, int q_len = 1, int expected_kv_len = 0) {
+                       void* workspace, int64_t workspace_bytes, void* stream, int hpc_limit, int q_len = 1, int expected_kv_len = 0,
+                       const int2* dead = nullptr, int* status = nullptr) {
   g_error[0] = 0;
   MLA_CHECK(precision == NVFP4_MLA_PRECISION_BF16 || precision == NVFP4_MLA_PRECISION_FP8,
             "precision must be 0 (bf16) or 1 (fp8), got %d", precision);
@@ -371,14 +380,15 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   P.sm_scale_log2 = sm_scale * 1.4426950408889634f, P.ckv_scale = ckv_scale, P.kpe_scale = kpe_scale;
   P.cta_range = cta_range, P.segs = segs, P.lse_part = lse_part, P.o_part = o_part, P.header = header;
   P.kv_lens = kv_lens, P.pb = pb, P.inline_sched = inline_sched ? 1 : 0, P.item_range = item_range;
-  P.cta_range_out = cta_range, P.segs_out = segs;
+  P.cta_range_out = cta_range, P.segs_out = segs, P.dead = dead;
+  if (status) P.header = status;
   Profile* prof = g_profile && g_profile->used < int(g_profile->start.size()) ? g_profile : nullptr;
   if (prof) MLA_CUDA(cudaEventRecord(prof->start[prof->used], st));
   const dim3 grid(pb.n_cta * ctas_per_unit(hpc)), block(decode_threads(precision, hpc));
   if (hm16)
-    MLA_CUDA(launch_dependent(mla::mla_decode_hm16_kernel, grid, block, decode_smem(precision, hpc), st, P));
+    MLA_CUDA(launch_dependent(hm16_kernel(dead != nullptr), grid, block, decode_smem(precision, hpc), st, P));
   else
-    MLA_CUDA(launch_dependent_cluster(decode_kernel(precision, hpc), grid, block, decode_smem(precision, hpc), st,
+    MLA_CUDA(launch_dependent_cluster(decode_kernel(precision, hpc, dead != nullptr), grid, block, decode_smem(precision, hpc), st,
                                       unsigned(ctas_per_unit(hpc)), ckv_map, sf_map, kpe_map, P));
   if (prof) MLA_CUDA(cudaEventRecord(prof->stop[prof->used++], st));
 
@@ -436,6 +446,124 @@ int nvfp4_mla_decode_multi(const void* q_nope, const void* q_pe, const uint8_t* 
   return decode_impl(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, page_table, page_table_stride, kv_lens,
                      batch, q_len * heads, sm_scale, ckv_scale, kpe_scale, max_kv_len, num_splits, precision, out, out_f32, lse,
                      workspace, workspace_bytes, stream, 128, q_len);
+}
+
+// ---- windowed decode ------------------------------------------------------------------------------------------------
+// Workspace: the decode call's | page table of the visible pages | lengths | gaps
+namespace {
+struct WindowLayout {
+  size_t decode, table, lens, dead, total;
+  int width;     // pages of a request that can be visible
+  int max_len;   // bound of the lengths in them
+};
+int window_layout(int batch, int heads, int page_size, int page_table_width, int max_kv_len, int window, int sinks, WindowLayout* l) {
+  MLA_CHECK(batch >= 0, "batch must be non-negative");
+  MLA_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0, "page_size must be a power of two, got %d", page_size);
+  MLA_CHECK(window >= 0 && sinks >= 0, "window and sink_tokens must be non-negative, got %d and %d", window, sinks);
+  MLA_CHECK(page_table_width >= 0 && max_kv_len >= 0, "page_table_width and max_kv_len must be non-negative");
+  const int64_t bytes = workspace_bytes_of(batch, heads, 0, NVFP4_MLA_PRECISION_BF16);
+  if (bytes < 0) return 1;
+  // the first tokens' pages, the window's (one more than its tokens fill: it need not start on a page), and the one between
+  // where the two meet
+  const int64_t pages = window == 0 ? page_table_width : (int64_t(sinks) + page_size - 1) / page_size + (int64_t(window) + page_size - 1) / page_size + 2;
+  l->width = int(pages < page_table_width ? pages : page_table_width);
+  const int64_t len = int64_t(l->width) * page_size;
+  l->max_len = int(len < max_kv_len ? len : max_kv_len);
+  l->decode = 0;
+  l->table = mla::align_up(size_t(bytes), 256);
+  l->lens = mla::align_up(l->table + size_t(batch) * l->width * 4, 256);
+  l->dead = mla::align_up(l->lens + size_t(batch) * 4, 256);
+  l->total = mla::align_up(l->dead + size_t(batch) * 8, 256);
+  return 0;
+}
+}  // namespace
+
+int64_t nvfp4_mla_decode_window_workspace_bytes(int batch, int heads, int page_size, int page_table_width, int window, int sink_tokens) {
+  g_error[0] = 0;
+  WindowLayout l;
+  if (window <= 0) return fail("window must be positive, got %d", window), -1;
+  return window_layout(batch, heads, page_size, page_table_width, 0, window, sink_tokens, &l) ? -1 : int64_t(l.total);
+}
+
+int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
+                            const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table,
+                            int64_t page_table_stride, int page_table_width, const int32_t* kv_lens, int batch, int heads, float sm_scale,
+                            float ckv_scale, float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, float* out_f32,
+                            float* lse, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  g_error[0] = 0;
+  WindowLayout l;
+  MLA_CHECK(window > 0, "window must be positive, got %d", window);
+  if (window_layout(batch, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)) return 1;
+  if (batch == 0) return 0;
+  MLA_CHECK((page_table || page_table_width == 0) && kv_lens && workspace, "null pointer argument");
+  MLA_CHECK(page_table_stride >= 0, "page_table_stride must be non-negative");
+  MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes,
+            (long long)l.total);
+  MLA_CHECK(aligned(workspace, 256), "workspace must be 256-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  int* table = reinterpret_cast<int*>(ws + l.table);
+  int* lens = reinterpret_cast<int*>(ws + l.lens);
+  int2* dead = reinterpret_cast<int2*>(ws + l.dead);
+  constexpr int per_block = mla::kWindowThreads / 32;
+  mla::mla_window_plan_kernel<<<unsigned((batch + per_block - 1) / per_block), mla::kWindowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      page_table, page_table_stride, page_table_width, kv_lens, mla::ChunkTokens{nullptr, batch, 0}, batch, __builtin_ctz(unsigned(page_size)),
+      window, sink_tokens, l.width, table, lens, dead);
+  MLA_CUDA(cudaGetLastError());
+  return decode_impl(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, table, l.width, lens, batch, heads, sm_scale,
+                     ckv_scale, kpe_scale, l.max_len, 0, NVFP4_MLA_PRECISION_BF16, out, out_f32, lse, workspace, int64_t(l.table), stream, 128,
+                     1, 0, dead, status);
+}
+
+// ---- chunks of new tokens ------------------------------------------------------------------------------------------
+namespace {
+// Every query token as a request of its own, this many at a time (the partial results of a slice take 2 KB per head and token)
+constexpr int kExtendSlice = 512;
+}  // namespace
+
+int64_t nvfp4_mla_extend_workspace_bytes(int batch, int total_q, int heads, int page_size, int page_table_width, int max_kv_len, int window,
+                                         int sink_tokens) {
+  g_error[0] = 0;
+  WindowLayout l;
+  return window_layout(total_q < kExtendSlice ? total_q : kExtendSlice, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)
+             ? -1
+             : int64_t(l.total);
+}
+
+int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, const uint8_t* kpe_cache,
+                     int64_t num_pages, int page_size, const int32_t* page_table, int64_t page_table_stride, int page_table_width,
+                     const int32_t* kv_lens, const int32_t* qo_indptr, int batch, int total_q, int heads, float sm_scale, float ckv_scale,
+                     float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, void* workspace, int64_t workspace_bytes,
+                     int32_t* status, void* stream) {
+  g_error[0] = 0;
+  MLA_CHECK(batch >= 0 && total_q >= 0, "batch and total_q must be non-negative");
+  WindowLayout l;
+  if (window_layout(total_q < kExtendSlice ? total_q : kExtendSlice, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)) return 1;
+  if (total_q == 0) return 0;
+  MLA_CHECK(batch > 0, "query tokens without requests");
+  MLA_CHECK((page_table || page_table_width == 0) && kv_lens && qo_indptr && workspace, "null pointer argument");
+  MLA_CHECK(page_table_stride >= 0, "page_table_stride must be non-negative");
+  MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes,
+            (long long)l.total);
+  MLA_CHECK(aligned(workspace, 256), "workspace must be 256-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  int* table = reinterpret_cast<int*>(ws + l.table);
+  int* lens = reinterpret_cast<int*>(ws + l.lens);
+  int2* dead = reinterpret_cast<int2*>(ws + l.dead);
+  constexpr int per_block = mla::kWindowThreads / 32;
+  for (int i = 0; i < total_q; i += kExtendSlice) {
+    const int n = total_q - i < kExtendSlice ? total_q - i : kExtendSlice;
+    mla::mla_window_plan_kernel<<<unsigned((n + per_block - 1) / per_block), mla::kWindowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+        page_table, page_table_stride, page_table_width, kv_lens, mla::ChunkTokens{qo_indptr, batch, i}, n, __builtin_ctz(unsigned(page_size)),
+        window, sink_tokens, l.width, table, lens, dead);
+    MLA_CUDA(cudaGetLastError());
+    const size_t row = size_t(i) * heads;
+    if (decode_impl(static_cast<const uint16_t*>(q_nope) + row * mla::CKV, static_cast<const uint16_t*>(q_pe) + row * mla::KPE, ckv_cache,
+                    ckv_sf_cache, kpe_cache, num_pages, page_size, table, l.width, lens, n, heads, sm_scale, ckv_scale, kpe_scale, l.max_len, 0,
+                    NVFP4_MLA_PRECISION_BF16, static_cast<uint16_t*>(out) + row * mla::CKV, nullptr, nullptr, workspace, int64_t(l.table), stream,
+                    128, 1, 0, dead, status))
+      return 1;
+  }
+  return 0;
 }
 
 // ---- decode without caller-provided scratch -----------------------------------------------------------------------
@@ -600,6 +728,74 @@ int nvfp4_mla_quantize_append(const void* ckv, const void* kpe, const int32_t* b
       static_cast<const __nv_bfloat16*>(ckv), static_cast<const __nv_bfloat16*>(kpe), batch_indices, positions, nnz, ckv_cache,
       ckv_sf_cache, kpe_cache, num_pages, __builtin_ctz(unsigned(page_size)), kv_indices, kv_indptr, batch, ckv_scale, kpe_scale,
       status);
+  MLA_CUDA(cudaGetLastError());
+  return 0;
+}
+
+int nvfp4_mla_norm_rope_append(const void* ckv, int64_t ckv_stride, const void* kpe, int64_t kpe_stride, const void* norm_weight,
+                               const float* cos_sin, int max_position, double eps, int interleaved, const int32_t* batch_indices,
+                               const int32_t* positions, int64_t nnz, uint8_t* ckv_cache, uint8_t* ckv_sf_cache, uint8_t* kpe_cache,
+                               int64_t num_pages, int page_size, const int32_t* kv_indices, const int32_t* kv_indptr, int batch,
+                               float ckv_scale, float kpe_scale, int32_t* status, void* stream) {
+  g_error[0] = 0;
+  MLA_CHECK(nnz >= 0 && batch >= 0, "nnz and batch must be non-negative");
+  MLA_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0, "page_size must be a power of two, got %d", page_size);
+  MLA_CHECK(num_pages > 0 && num_pages * page_size < (int64_t(1) << 31), "num_pages * page_size must be in [1, 2^31)");
+  MLA_CHECK(ckv_scale > 0.f && kpe_scale > 0.f, "ckv_scale and kpe_scale must be positive");
+  MLA_CHECK(eps >= 0., "eps must not be negative");
+  MLA_CHECK(ckv_stride >= mla::CKV && ckv_stride % 8 == 0 && kpe_stride >= mla::KPE && kpe_stride % 2 == 0,
+            "the row strides must cover a row, ckv's a multiple of 8 and kpe's of 2 elements");
+  MLA_CHECK(max_position >= 0, "max_position must be non-negative");
+  if (nnz == 0) return 0;
+  MLA_CHECK(ckv && kpe && norm_weight && cos_sin && batch_indices && positions && ckv_cache && ckv_sf_cache && kpe_cache && kv_indices && kv_indptr,
+            "null pointer argument");
+  MLA_CHECK(aligned(ckv, 16) && aligned(kpe, 4) && aligned(norm_weight, 16) && aligned(cos_sin, 4) && aligned(ckv_cache, 8) && aligned(kpe_cache, 2),
+            "ckv and norm_weight must be 16-byte, kpe and cos_sin 4-byte, ckv_cache 8-byte and kpe_cache 2-byte aligned");
+  DeviceInfo* d;
+  if (device_info(&d)) return 1;
+  const long long warps_per_block = mla::kQuantThreads / 32;
+  long long blocks = (nnz + warps_per_block - 1) / warps_per_block;
+  const long long cap = (long long)d->sm_count * 32;  // grid-stride beyond 32 CTAs per SM
+  if (blocks > cap) blocks = cap;
+  const auto kernel = interleaved ? mla::mla_norm_rope_append_kernel<true> : mla::mla_norm_rope_append_kernel<false>;
+  kernel<<<unsigned(blocks), mla::kQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const __nv_bfloat16*>(ckv), ckv_stride, static_cast<const __nv_bfloat16*>(kpe), kpe_stride,
+      static_cast<const __nv_bfloat16*>(norm_weight), cos_sin, max_position, eps, batch_indices, positions, nnz, ckv_cache, ckv_sf_cache,
+      kpe_cache, num_pages, __builtin_ctz(unsigned(page_size)), kv_indices, kv_indptr, batch, ckv_scale, kpe_scale, status);
+  MLA_CUDA(cudaGetLastError());
+  return 0;
+}
+
+int nvfp4_mla_gather(const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, const uint8_t* kpe_cache, int64_t num_pages, int page_size,
+                     const int32_t* page_table, int64_t page_table_stride, int page_table_width, const int32_t* indptr,
+                     const int32_t* starts, int batch, int64_t total, float ckv_scale, float kpe_scale, int out_bf16, void* ckv_out,
+                     void* kpe_out, int32_t* status, void* stream) {
+  g_error[0] = 0;
+  MLA_CHECK(total >= 0 && total < (int64_t(1) << 31) - 64 && batch >= 0, "total must be in [0, 2^31 - 64) and batch non-negative");
+  MLA_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0, "page_size must be a power of two, got %d", page_size);
+  MLA_CHECK(num_pages > 0 && num_pages * page_size < (int64_t(1) << 31), "num_pages * page_size must be in [1, 2^31)");
+  MLA_CHECK(page_table_stride >= 0 && page_table_width >= 0, "page_table_stride and page_table_width must be non-negative");
+  if (total == 0 || batch == 0) return 0;
+  MLA_CHECK(ckv_cache && ckv_sf_cache && kpe_cache && page_table && indptr && ckv_out && kpe_out, "null pointer argument");
+  MLA_CHECK(aligned(ckv_cache, 4) && aligned(kpe_cache, 2) && aligned(ckv_out, 16) && aligned(kpe_out, 8),
+            "ckv_cache must be 4-byte and kpe_cache 2-byte aligned, ckv_out 16-byte and kpe_out 8-byte aligned");
+  DeviceInfo* d;
+  if (device_info(&d)) return 1;
+  // rows per warp: as many as leave every SM its warps
+  int rows = 32;
+  while (rows > mla::kDequantTokens && total < (long long)rows * d->sm_count * 32) rows /= 2;
+  const long long per_block = (long long)rows * (mla::kGatherThreads / 32);
+  const unsigned blocks = unsigned((total + per_block - 1) / per_block);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int shift = __builtin_ctz(unsigned(page_size));
+  if (out_bf16)
+    mla::mla_gather_kernel<__nv_bfloat16><<<blocks, mla::kGatherThreads, 0, st>>>(
+        ckv_cache, ckv_sf_cache, kpe_cache, num_pages, shift, page_table, page_table_stride, page_table_width, indptr, starts, batch,
+        int(total), rows, ckv_scale, kpe_scale, static_cast<__nv_bfloat16*>(ckv_out), static_cast<__nv_bfloat16*>(kpe_out), status);
+  else
+    mla::mla_gather_kernel<float><<<blocks, mla::kGatherThreads, 0, st>>>(
+        ckv_cache, ckv_sf_cache, kpe_cache, num_pages, shift, page_table, page_table_stride, page_table_width, indptr, starts, batch,
+        int(total), rows, ckv_scale, kpe_scale, static_cast<float*>(ckv_out), static_cast<float*>(kpe_out), status);
   MLA_CUDA(cudaGetLastError());
   return 0;
 }

@@ -138,7 +138,7 @@ __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams
 // there the block becomes 0, and the token's rope part, which only enters scores, NaN. The loads of tile t + 1 are issued as soon as tile t's bytes have
 // been converted, the page ids of tile t + 2 behind them.
 // ---------------------------------------------------------------------------------------------------------------
-template <bool part_a>  // whether the warp's panel belongs to part A
+template <bool part_a, bool WINDOW>  // whether the warp's panel belongs to part A
 __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams& P, int n_segs, uint32_t& it) {
   const int lane = ptx::lane_id();
   const int cw = (threadIdx.x >> 5) - 8, w = cw & 7, v = cw >> 3, hh = lane & 1;
@@ -159,6 +159,7 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
     const int nt = h16_tiles(seg);
     if (nt <= 0) continue;
     const int* pt = P.page_table + (long long)seg.b * P.pt_stride;
+    const int2 dead = WINDOW ? P.dead[seg.b] : make_int2(0, 0);  // tokens that no row sees: they read as zeros
     const int first_masked = P.q_len > 1 ? P.kv_lens[seg.b] - (P.q_len - 1) : INT_MAX;  // first token that some row does not see
     uint4 rw[2];
     uint32_t rs[2];
@@ -173,7 +174,8 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
       const bool live = tok < seg.tok_end, good = uint32_t(page) < uint32_t(P.num_pages);
       // a stale or corrupt id is never dereferenced: the row reads as zeros and the call is flagged
       if (live && !good) atomicExch(P.header, int(kBadPage));
-      const int row = live && good ? (page << P.page_shift) + (tok & ((1 << P.page_shift) - 1)) : -1;
+      const bool seen = live && (!WINDOW || tok < dead.x || tok >= dead.y);
+      const int row = seen && good ? (page << P.page_shift) + (tok & ((1 << P.page_shift) - 1)) : -1;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         ru[u] = __shfl_sync(~0u, row, 16 * u + (lane >> 1));
@@ -252,9 +254,10 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
   }
 }
 
+template <bool WINDOW>
 __device__ __forceinline__ void h16_convert_role(H16Smem& s, const DecodeParams& P, int n_segs, uint32_t& it, int cg) {
-  if (int(((threadIdx.x >> 5) - 8) >> 2 & 1) != cg) h16_convert_warps<true>(s, P, n_segs, it);
-  else h16_convert_warps<false>(s, P, n_segs, it);
+  if (int(((threadIdx.x >> 5) - 8) >> 2 & 1) != cg) h16_convert_warps<true, WINDOW>(s, P, n_segs, it);
+  else h16_convert_warps<false, WINDOW>(s, P, n_segs, it);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -345,6 +348,7 @@ __device__ __forceinline__ void h16_pv_role(H16Smem& s, const DecodeParams& P, i
 // same in both, so the pair votes at a named barrier once per tile and, only when some row outgrows its max by 2^8,
 // exchanges the maxima through shared memory. A quadrant without live rows only keeps the barriers going.
 // ---------------------------------------------------------------------------------------------------------------
+template <bool WINDOW>
 __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams& P, int n_segs, uint32_t& it, int cg) {
   const int lane = ptx::lane_id(), warp = threadIdx.x >> 5;
   const int quad = warp & 3, half = warp >> 2;
@@ -375,6 +379,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
     // A row sees the tokens up to its own query token: token i of q_len (rows [i, i + 1) * heads / q_len of the request) stops
     // q_len - 1 - i tokens before the request's end.
     int row_end = seg.tok_end;
+    const int2 dead = WINDOW ? P.dead[seg.b] : make_int2(0, 0);
     if (P.q_len > 1) {
       const int i = (r0 + hq) / (P.heads / P.q_len), end = P.kv_lens[seg.b] - (P.q_len - 1 - i);
       row_end = end < row_end ? end : row_end;
@@ -473,6 +478,13 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
 #pragma unroll
         for (int j = 0; j < 32; ++j) sr[j] = (ok && j < nvalid) ? sr[j] : 0xFF800000u;
       }
+      if constexpr (WINDOW) {  // the gap between the first tokens and the window
+        const int at = seg.tok0 + t * kH16Tile + 32 * half, d0 = dead.x - at, d1 = dead.y - at;
+        if (d0 < 32 && d1 > 0) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sr[j] = j >= d0 && j < d1 ? 0xFF800000u : sr[j];
+        }
+      }
       float mxs[4] = {__uint_as_float(sr[0]), __uint_as_float(sr[1]), __uint_as_float(sr[2]), __uint_as_float(sr[3])};
 #pragma unroll
       for (int j = 4; j + 8 <= 32; j += 8)  // four chains of three-input maxima
@@ -562,7 +574,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
           *reinterpret_cast<float4*>(orow + 4 * i * CKV + c0) = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
       }
     }
-    if (cg == 0 && half == 0 && h < live_rows) P.lse_part[slot * P.heads_per_cta + h] = lt > 0.f ? m + log2f(lt) : -INFINITY;
+    if (cg == 0 && half == 0 && h < live_rows) P.lse_part[slot * P.heads_per_cta + h] = (WINDOW ? lt != 0.f : lt > 0.f) ? m + log2f(lt) : -INFINITY;
     ptx::tc_fence_before_sync();
     ptx::bar_sync(pair_bar, 64);  // s.xl and s.xch are reused by the next segment
   }
@@ -573,7 +585,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
 // ---------------------------------------------------------------------------------------------------------------
 enum H16Role { kH16Softmax, kH16Convert, kH16Qk, kH16Prefetch, kH16Pv, kH16Idle };
 
-template <int ROLE>
+template <int ROLE, bool WINDOW>
 __device__ __forceinline__ void h16_run_role(H16Smem& s, const DecodeParams& P) {
   const int pair = blockIdx.x >> 1, cg = blockIdx.x & 1;
   const int2 range = P.cta_range[pair];
@@ -586,8 +598,8 @@ __device__ __forceinline__ void h16_run_role(H16Smem& s, const DecodeParams& P) 
       s.segs[threadIdx.x] = g;
     }
     __syncthreads();
-    if (ROLE == kH16Softmax) h16_softmax_role(s, P, n_segs, it, cg);
-    if (ROLE == kH16Convert) h16_convert_role(s, P, n_segs, it, cg);
+    if (ROLE == kH16Softmax) h16_softmax_role<WINDOW>(s, P, n_segs, it, cg);
+    if (ROLE == kH16Convert) h16_convert_role<WINDOW>(s, P, n_segs, it, cg);
     if (ROLE == kH16Qk) h16_qk_role(s, P, n_segs, it, seg_count, cg);
     if (ROLE == kH16Prefetch) h16_prefetch_role(s, P, n_segs, it, cg);
     if (ROLE == kH16Pv) h16_pv_role(s, P, n_segs, it, cg);
@@ -596,6 +608,7 @@ __device__ __forceinline__ void h16_run_role(H16Smem& s, const DecodeParams& P) 
   }
 }
 
+template <bool WINDOW>
 __global__ void __launch_bounds__(kH16Threads, 1) mla_decode_hm16_kernel(const DecodeParams P) {
   extern __shared__ uint8_t smem_raw[];
   H16Smem& s = *reinterpret_cast<H16Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -629,16 +642,16 @@ __global__ void __launch_bounds__(kH16Threads, 1) mla_decode_hm16_kernel(const D
   static_assert(8 * kSoftmaxRegs + 16 * kConvertRegs + 4 * kIssueRegs <= 28 * kLaunchRegs, "register budgets exceed the CTA's allocation");
   if (warp < 8) {
     ptx::reg_alloc<kSoftmaxRegs>();
-    h16_run_role<kH16Softmax>(s, P);
+    h16_run_role<kH16Softmax, WINDOW>(s, P);
   } else if (warp < 24) {
     ptx::reg_dealloc<kConvertRegs>();
-    h16_run_role<kH16Convert>(s, P);
+    h16_run_role<kH16Convert, WINDOW>(s, P);
   } else {
     ptx::reg_dealloc<kIssueRegs>();
-    if (warp == 24) h16_run_role<kH16Qk>(s, P);
-    else if (warp == 25) h16_run_role<kH16Prefetch>(s, P);
-    else if (warp == 26) h16_run_role<kH16Pv>(s, P);
-    else h16_run_role<kH16Idle>(s, P);
+    if (warp == 24) h16_run_role<kH16Qk, WINDOW>(s, P);
+    else if (warp == 25) h16_run_role<kH16Prefetch, WINDOW>(s, P);
+    else if (warp == 26) h16_run_role<kH16Pv, WINDOW>(s, P);
+    else h16_run_role<kH16Idle, WINDOW>(s, P);
   }
 
   ptx::tc_fence_before_sync();

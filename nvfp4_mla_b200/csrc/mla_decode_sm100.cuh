@@ -76,6 +76,7 @@ struct DecodeParams {
   int2* item_range;  // written by the CTA that holds an item's first tile (read by the combine kernel)
   int2* cta_range_out;
   Seg* segs_out;
+  const int2* dead;  // windowed decode: tokens [x, y) of the request are not seen (kernels with WINDOW only)
 };
 
 // ---------------------------------------------------------------------------------------------------------------

@@ -339,15 +339,23 @@ __device__ __forceinline__ bool vt_load_query(VtSmem& s, const DecodeParams& P, 
   return true;
 }
 
+// Whether token `tok` of the segment's request is seen: before its end and, with WINDOW, outside the gap between the first tokens
+// and the window.
+template <bool WINDOW>
+__device__ __forceinline__ bool vt_sees(const Seg& seg, int2 dead, int tok) {
+  return tok < seg.tok_end && (!WINDOW || tok < dead.x || tok >= dead.y);
+}
+
 // One tile of a K thread. Returns false if a wait gave up.
-__device__ __forceinline__ bool vt_k_step(VtSmem& s, const DecodeParams& P, const Seg& seg, int t, uint32_t it, int lane, int quad) {
+template <bool WINDOW>
+__device__ __forceinline__ bool vt_k_step(VtSmem& s, const DecodeParams& P, const Seg& seg, int2 dead, int t, uint32_t it, int lane, int quad) {
   const int r = quad * 32 + lane;
   const uint32_t tm_lane = s.tmem_base + (uint32_t(quad * 32) << 16);
   const int slot = it % kVtRawSlots;
   const uint32_t raw = ptx::smem_u32(s.raw[slot]);
   const uint32_t buf = it & 1;
   if (!__all_sync(~0u, ptx::mbar_wait(&s.raw_full[slot], (it / kVtRawSlots) & 1, &s.abort_flag))) return false;
-  const bool valid = seg.tok0 + t * TILE + r < seg.tok_end;
+  const bool valid = vt_sees<WINDOW>(seg, dead, seg.tok0 + t * TILE + r);
   // tests of the barriers needed further down, issued before the work that precedes them
   const uint32_t pr_kfree = ptx::mbar_probe(&s.k_free[buf], ((it >> 1) & 1) ^ 1), pr_rope = ptx::mbar_probe(&s.rope_free, (it & 1) ^ 1);
 
@@ -419,6 +427,7 @@ __device__ __forceinline__ bool vt_k_step(VtSmem& s, const DecodeParams& P, cons
 // A warp whose wait gave up does not leave at once: the 128 K threads meet at a named barrier at the start of every
 // segment, so it carries on (skipping the work) to the next such barrier, where the failure is OR-reduced and all
 // four warps leave together.
+template <bool WINDOW>
 __device__ __forceinline__ void vt_k_role(VtSmem& s, const DecodeParams& P, int n_segs, uint32_t& it, uint32_t& seg_count) {
   const int lane = ptx::lane_id();
   const int quad = (threadIdx.x >> 5) & 3;
@@ -431,8 +440,9 @@ __device__ __forceinline__ void vt_k_role(VtSmem& s, const DecodeParams& P, int 
     if (!vt_load_query(s, P, seg, quad * 32 + lane, seg_count & 3, lane, quad, dead, it != 0, &s.k_free[(it - 1) & 1], ((it - 1) >> 1) & 1))
       return;
     ++seg_count;
+    const int2 gap = WINDOW ? P.dead[seg.b] : make_int2(0, 0);
     for (int t = 0; t < seg.ntiles; ++t, ++it) {
-      if (!vt_k_step(s, P, seg, t, it, lane, quad)) {
+      if (!vt_k_step<WINDOW>(s, P, seg, gap, t, it, lane, quad)) {
         dead = true;
         break;
       }
@@ -628,6 +638,7 @@ __device__ __forceinline__ void vt_pv_role(VtSmem& s, const DecodeParams& P, int
 // ---------------------------------------------------------------------------------------------------------------
 // role: softmax + epilogue (4 warps; thread r = token row of S^T and channel-pair row of O^T)
 // ---------------------------------------------------------------------------------------------------------------
+template <bool WINDOW>
 __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P, int n_segs, uint32_t& it, uint32_t& seg_count) {
   constexpr int N = 16;
   const int lane = ptx::lane_id(), warp = threadIdx.x >> 5;
@@ -643,6 +654,7 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
     if (seg.ntiles <= 0) continue;
     const int par_q = seg_count & 3;
     ++seg_count;
+    const int2 dead = WINDOW ? P.dead[seg.b] : make_int2(0, 0);
     // running maximum and sum per head. The maximum starts at a finite sentinel far below any score rather than at
     // -inf: x - m and m - m' then never meet inf - inf, and no special case is needed anywhere below.
     constexpr float kNoMax = -1e30f;
@@ -665,7 +677,7 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
         }
       }
       if (ok) {
-        const bool valid = seg.tok0 + t * TILE + r < seg.tok_end;
+        const bool valid = vt_sees<WINDOW>(seg, dead, seg.tok0 + t * TILE + r);
         uint32_t sv[32];  // columns [0, 16): even terms + rope, [16, 32): odd terms
         ptx::tmem_ld32(tm_lane + VtCols::s(buf), sv);
         ptx::tmem_wait_ld();
@@ -785,7 +797,8 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
 #pragma unroll
       for (int h = 0; h < N; ++h)
         if (h == r) l = lsum[h], mm = m[h];
-      P.lse_part[slot * N + r] = l > 0.f ? mm + log2f(l) : -INFINITY;
+      // (with WINDOW a sum of NaN is carried on: a row that sees a NaN block scale is NaN)
+      P.lse_part[slot * N + r] = (WINDOW ? l != 0.f : l > 0.f) ? mm + log2f(l) : -INFINITY;
     }
     ptx::tc_fence_before_sync();
     ptx::bar_sync(1, 128);  // s.red is reused by the next segment
@@ -798,7 +811,7 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
 // ---------------------------------------------------------------------------------------------------------------
 enum VtRole { kVtSoftmax, kVtK, kVtV, kVtQk, kVtProducer, kVtPv, kVtIdle };
 
-template <int ROLE>
+template <int ROLE, bool WINDOW>
 __device__ __forceinline__ void vt_run_role(VtSmem& s, const DecodeParams& P, const CUtensorMap* ckv_map, const CUtensorMap* sf_map,
                                             const CUtensorMap* kpe_map) {
   const int2 range = P.cta_range[blockIdx.x];
@@ -811,8 +824,8 @@ __device__ __forceinline__ void vt_run_role(VtSmem& s, const DecodeParams& P, co
       s.segs[threadIdx.x] = g;
     }
     __syncthreads();
-    if (ROLE == kVtSoftmax) vt_softmax_role(s, P, n_segs, it, seg_count);
-    if (ROLE == kVtK) vt_k_role(s, P, n_segs, it, seg_count);
+    if (ROLE == kVtSoftmax) vt_softmax_role<WINDOW>(s, P, n_segs, it, seg_count);
+    if (ROLE == kVtK) vt_k_role<WINDOW>(s, P, n_segs, it, seg_count);
     if (ROLE == kVtV) vt_v_role(s, P, n_segs, it, (uint32_t(threadIdx.x) >> 7) - 2);
     if (ROLE == kVtQk) vt_qk_role(s, P, n_segs, it);
     if (ROLE == kVtProducer) vt_producer_role(s, P, ckv_map, sf_map, kpe_map, n_segs, it);
@@ -822,6 +835,7 @@ __device__ __forceinline__ void vt_run_role(VtSmem& s, const DecodeParams& P, co
   }
 }
 
+template <bool WINDOW>
 __global__ void __launch_bounds__(kVtThreads, 1)
 mla_decode_vt_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__ CUtensorMap sf_map,
                      const __grid_constant__ CUtensorMap kpe_map, const DecodeParams P) {
@@ -861,18 +875,18 @@ mla_decode_vt_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_c
   static_assert(4 * kSoftmaxRegs + 4 * kKRegs + 8 * kVRegs + 4 * kMiscRegs <= 20 * 96, "register budgets exceed the CTA's allocation");
   if (warp < 4) {
     ptx::reg_alloc<kSoftmaxRegs>();
-    vt_run_role<kVtSoftmax>(s, P, &ckv_map, &sf_map, &kpe_map);
+    vt_run_role<kVtSoftmax, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
   } else if (warp < 8) {
     ptx::reg_alloc<kKRegs>();
-    vt_run_role<kVtK>(s, P, &ckv_map, &sf_map, &kpe_map);
+    vt_run_role<kVtK, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
   } else if (warp < 16) {
-    vt_run_role<kVtV>(s, P, &ckv_map, &sf_map, &kpe_map);
+    vt_run_role<kVtV, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
   } else {
     ptx::reg_dealloc<kMiscRegs>();
-    if (warp == 16) vt_run_role<kVtQk>(s, P, &ckv_map, &sf_map, &kpe_map);
-    else if (warp == 17) vt_run_role<kVtProducer>(s, P, &ckv_map, &sf_map, &kpe_map);
-    else if (warp == 18) vt_run_role<kVtPv>(s, P, &ckv_map, &sf_map, &kpe_map);
-    else vt_run_role<kVtIdle>(s, P, &ckv_map, &sf_map, &kpe_map);
+    if (warp == 16) vt_run_role<kVtQk, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
+    else if (warp == 17) vt_run_role<kVtProducer, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
+    else if (warp == 18) vt_run_role<kVtPv, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
+    else vt_run_role<kVtIdle, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
   }
 
   ptx::tc_fence_before_sync();

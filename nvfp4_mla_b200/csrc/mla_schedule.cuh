@@ -177,7 +177,7 @@ __device__ __forceinline__ void merge_row(int n_parts, LseOf lse_of, OOf o_of, l
   M = warp_max(M);
   float den = 0.f;
   for (int i = lane; i < n_parts; i += 32) {
-    const float wl = M > -INFINITY ? exp2f(lse_of(i) - M) : 0.f;  // lse = -inf (empty partial) gives weight 0
+    const float li = lse_of(i), wl = li == -INFINITY ? 0.f : exp2f(li - M);  // lse = -inf (empty partial) gives weight 0, NaN stays NaN
     den += wl;
     if (threadIdx.x < 32 && i < kCombineMaxParts) weights[i] = wl;
   }
