@@ -126,8 +126,13 @@ NVFP4_MLA_API int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, 
  *   qo_indptr     [batch + 1] int32, non-decreasing, read on the device. Query tokens of no request (before qo_indptr[0], at or
  *                 behind qo_indptr[batch]) and tokens in front of a request's first (more new tokens than kv_lens) give zeros
  *   window        0: none
- *   others        as in nvfp4_mla_decode_window; 16-bit arithmetic
+ *   others        as in nvfp4_mla_decode_window; 16-bit arithmetic; any number of heads
+ *
+ * Chunks of more than a few tokens share one pass over the cache (nvfp4_mla_extend_shares: 1, 0: not, -1: error), which is dequantised
+ * once into the workspace: 1152 bytes per visible token, of which there are at most batch * max_kv_len (and with a window at most
+ * batch * (window + sink_tokens + 768) + total_q).
  * (No counterpart in the reference, which decodes one query token per request.) */
+NVFP4_MLA_API int nvfp4_mla_extend_shares(int batch, int total_q, int heads);
 NVFP4_MLA_API int64_t nvfp4_mla_extend_workspace_bytes(int batch, int total_q, int heads, int page_size, int page_table_width, int max_kv_len,
                                                        int window, int sink_tokens);
 NVFP4_MLA_API int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,

@@ -16,6 +16,8 @@
 #include "mla_decode_hm_sm100.cuh"
 #include "mla_decode_hm16_sm100.cuh"
 #include "mla_dequant.cuh"
+#include "mla_extend_prep.cuh"
+#include "mla_extend_sm100.cuh"
 #include "mla_gather.cuh"
 #include "mla_quantize.cuh"
 #include "mla_schedule.cuh"
@@ -47,6 +49,7 @@ struct DeviceInfo {
   bool ready = false;
   int sm_count = 0;
   int hm_pairs = 0;  // CTA pairs (clusters of two) of the 8-bit heads-as-M kernel that can be resident at once; 0 = do not use it
+  int ext_pairs = 0;  // the same of the chunk attention kernel
 };
 std::mutex g_mutex;
 DeviceInfo g_devices[kMaxDevices];
@@ -152,23 +155,29 @@ int device_info(DeviceInfo** out) {
     for (int hpc : {16, 128})
       MLA_CUDA(cudaFuncSetAttribute(decode_entry(NVFP4_MLA_PRECISION_BF16, hpc, true), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     int(decode_smem(NVFP4_MLA_PRECISION_BF16, hpc))));
-    {  // clusters of two need both SMs in one GPC: ask how many can be resident rather than assuming sm_count / 2
+    MLA_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(mla::mla_extend_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  int(mla::ext_smem_bytes())));
+    // clusters of two need both SMs in one GPC: ask how many can be resident rather than assuming sm_count / 2
+    auto resident_pairs = [&](const void* kernel, unsigned threads, size_t smem) {
       cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(unsigned(d.sm_count / 2 * 2)), cfg.blockDim = dim3(mla::kHmThreads);
-      cfg.dynamicSmemBytes = decode_smem(NVFP4_MLA_PRECISION_FP8, 128);
+      cfg.gridDim = dim3(unsigned(d.sm_count / 2 * 2)), cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = smem;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr, cfg.numAttrs = 1;
       int clusters = 0;
-      if (cudaOccupancyMaxActiveClusters(&clusters, decode_kernel(NVFP4_MLA_PRECISION_FP8, 128), &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
         (void)cudaGetLastError();
         clusters = 0;
       }
-      d.hm_pairs = clusters < d.sm_count / 2 ? clusters : d.sm_count / 2;
-      if (getenv("NVFP4_MLA_DEBUG"))
-        fprintf(stderr, "nvfp4_mla_b200: device %d: %d SMs, %d resident CTA pairs for the 128-head kernel\n", dev, d.sm_count, d.hm_pairs);
-    }
+      return clusters < d.sm_count / 2 ? clusters : d.sm_count / 2;
+    };
+    d.hm_pairs = resident_pairs(decode_entry(NVFP4_MLA_PRECISION_FP8, 128), mla::kHmThreads, decode_smem(NVFP4_MLA_PRECISION_FP8, 128));
+    d.ext_pairs = resident_pairs(reinterpret_cast<const void*>(mla::mla_extend_kernel), mla::kExtThreads, mla::ext_smem_bytes());
+    if (getenv("NVFP4_MLA_DEBUG"))
+      fprintf(stderr, "nvfp4_mla_b200: device %d: %d SMs, %d resident CTA pairs for the 128-head kernel, %d for chunk attention\n", dev, d.sm_count,
+              d.hm_pairs, d.ext_pairs);
     d.ready = true;
   }
   *out = &d;
@@ -515,37 +524,69 @@ int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, const uint8_t*
 }
 
 // ---- chunks of new tokens ------------------------------------------------------------------------------------------
+// Two forms. A few query tokens run as requests of their own through the windowed decode, which reads the cache once per token
+// (the later reads are L2 hits). Longer chunks dequantise every visible token once and share it among all rows of a request.
 namespace {
-// Every query token as a request of its own, this many at a time (the partial results of a slice take 2 KB per head and token)
-constexpr int kExtendSlice = 512;
-}  // namespace
+constexpr int kExtendSlice = 512;  // query tokens at a time in the first form (the partial results of a slice take 2 KB per head and token)
 
-int64_t nvfp4_mla_extend_workspace_bytes(int batch, int total_q, int heads, int page_size, int page_table_width, int max_kv_len, int window,
-                                         int sink_tokens) {
-  g_error[0] = 0;
-  WindowLayout l;
-  return window_layout(total_q < kExtendSlice ? total_q : kExtendSlice, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)
-             ? -1
-             : int64_t(l.total);
+struct ExtendLayout {
+  size_t counts, req_tile0, req_item0, req_map, items, pair, q_scale, lse_part, o_part, q16, kv16, total;
+  int pairs, max_items, max_tiles;
+};
+int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window, int sinks, const DeviceInfo& d, ExtendLayout* l) {
+  MLA_CHECK(batch <= mla::kExtMaxBatch, "at most %d requests, got %d", mla::kExtMaxBatch, batch);
+  MLA_CHECK(int64_t(total_q) * heads < (int64_t(1) << 31) - mla::kExtRows, "total_q * heads must be below 2^31");
+  const int64_t requests = batch < total_q ? batch : total_q;  // with query tokens
+  const int64_t len = max_kv_len > 1 ? max_kv_len : 1;
+  int64_t tiles = requests * ((len - 1) / mla::kExtTile + 1);
+  if (window > 0) {
+    const int64_t seen = requests * ((int64_t(sinks) + mla::kExtTile - 1) / mla::kExtTile + window / mla::kExtTile + 3) + total_q / mla::kExtTile;
+    if (seen < tiles) tiles = seen;
+  }
+  const int64_t items = requests + int64_t(total_q) * heads / mla::kExtRows;
+  MLA_CHECK(tiles * mla::kExtTile < (int64_t(1) << 31) && tiles + items < (int64_t(1) << 31) && items * ((len - 1) / mla::kExtTile + 1) < (int64_t(1) << 31),
+            "chunks of %d query tokens over %d requests of up to %lld tokens are too large for one call", total_q, batch, (long long)len);
+  l->pairs = d.ext_pairs, l->max_items = int(items), l->max_tiles = int(tiles);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off = mla::align_up(off + bytes, 256);
+    return at;
+  };
+  l->counts = take(64), l->req_tile0 = take(size_t(batch + 1) * 4), l->req_item0 = take(size_t(batch + 1) * 4), l->req_map = take(size_t(batch) * 16);
+  l->items = take(size_t(items) * sizeof(mla::ExtItem)), l->pair = take(size_t(l->pairs) * sizeof(mla::ExtPair));
+  l->q_scale = take(size_t(items) * mla::kExtRows * 4);
+  l->lse_part = take(size_t(l->pairs) * 2 * mla::kExtRows * 4), l->o_part = take(size_t(l->pairs) * 2 * mla::kExtRows * mla::CKV * 4);
+  l->q16 = take(size_t(items) * mla::kExtRows * mla::kExtRow * 2), l->kv16 = take(size_t(tiles) * mla::kExtTile * mla::kExtRow * 2);
+  l->total = off;
+  return 0;
 }
 
-int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, const uint8_t* kpe_cache,
-                     int64_t num_pages, int page_size, const int32_t* page_table, int64_t page_table_stride, int page_table_width,
-                     const int32_t* kv_lens, const int32_t* qo_indptr, int batch, int total_q, int heads, float sm_scale, float ckv_scale,
-                     float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, void* workspace, int64_t workspace_bytes,
-                     int32_t* status, void* stream) {
-  g_error[0] = 0;
-  MLA_CHECK(batch >= 0 && total_q >= 0, "batch and total_q must be non-negative");
-  WindowLayout l;
-  if (window_layout(total_q < kExtendSlice ? total_q : kExtendSlice, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)) return 1;
-  if (total_q == 0) return 0;
-  MLA_CHECK(batch > 0, "query tokens without requests");
-  MLA_CHECK((page_table || page_table_width == 0) && kv_lens && qo_indptr && workspace, "null pointer argument");
-  MLA_CHECK(page_table_stride >= 0, "page_table_stride must be non-negative");
-  MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes,
-            (long long)l.total);
-  MLA_CHECK(aligned(workspace, 256), "workspace must be 256-byte aligned");
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+// FP16 rows of 576 as a map of [rows, 576], boxes of 64 channels x `box_rows` rows with the 128-byte swizzle
+int make_half_map(const void* base, int64_t rows, int box_rows, CUtensorMap* map) {
+  EncodeTiledFn encode;
+  if (encode_fn(&encode)) return 1;
+  const cuuint64_t dims[2] = {cuuint64_t(mla::kExtRow), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(mla::kExtRow) * 2};
+  const cuuint32_t box[2] = {64, cuuint32_t(box_rows)};
+  const cuuint32_t elem_strides[2] = {1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, elem_strides,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  MLA_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with CUresult %d", int(r));
+  return 0;
+}
+
+bool extend_shares(int batch, int total_q, int heads, const DeviceInfo& d) {
+  if (d.ext_pairs < 2) return false;
+  if (heads % 16 != 0) return true;
+  return total_q > 2 * batch;
+}
+
+int extend_by_token(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, const uint8_t* kpe_cache,
+                    int64_t num_pages, int page_size, const int32_t* page_table, int64_t page_table_stride, int page_table_width,
+                    const int32_t* kv_lens, const int32_t* qo_indptr, int batch, int total_q, int heads, float sm_scale, float ckv_scale,
+                    float kpe_scale, int window, int sink_tokens, void* out, uint8_t* ws, const WindowLayout& l, int32_t* status, void* stream) {
   int* table = reinterpret_cast<int*>(ws + l.table);
   int* lens = reinterpret_cast<int*>(ws + l.lens);
   int2* dead = reinterpret_cast<int2*>(ws + l.dead);
@@ -559,10 +600,104 @@ int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_ca
     const size_t row = size_t(i) * heads;
     if (decode_impl(static_cast<const uint16_t*>(q_nope) + row * mla::CKV, static_cast<const uint16_t*>(q_pe) + row * mla::KPE, ckv_cache,
                     ckv_sf_cache, kpe_cache, num_pages, page_size, table, l.width, lens, n, heads, sm_scale, ckv_scale, kpe_scale, l.max_len, 0,
-                    NVFP4_MLA_PRECISION_BF16, static_cast<uint16_t*>(out) + row * mla::CKV, nullptr, nullptr, workspace, int64_t(l.table), stream,
+                    NVFP4_MLA_PRECISION_BF16, static_cast<uint16_t*>(out) + row * mla::CKV, nullptr, nullptr, ws, int64_t(l.table), stream,
                     128, 1, 0, dead, status))
       return 1;
   }
+  return 0;
+}
+}  // namespace
+
+int nvfp4_mla_extend_shares(int batch, int total_q, int heads) {
+  g_error[0] = 0;
+  DeviceInfo* d;
+  if (device_info(&d)) return -1;
+  return extend_shares(batch, total_q, heads, *d) ? 1 : 0;
+}
+
+// what both functions below check first
+static int check_extend(int batch, int total_q, int heads, int page_size, int page_table_width, int max_kv_len, int window, int sinks) {
+  MLA_CHECK(batch >= 0 && total_q >= 0 && heads > 0, "batch and total_q must be non-negative and heads positive");
+  MLA_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0, "page_size must be a power of two, got %d", page_size);
+  MLA_CHECK(window >= 0 && sinks >= 0, "window and sink_tokens must be non-negative, got %d and %d", window, sinks);
+  MLA_CHECK(page_table_width >= 0 && max_kv_len >= 0, "page_table_width and max_kv_len must be non-negative");
+  return 0;
+}
+
+int64_t nvfp4_mla_extend_workspace_bytes(int batch, int total_q, int heads, int page_size, int page_table_width, int max_kv_len, int window,
+                                         int sink_tokens) {
+  g_error[0] = 0;
+  if (check_extend(batch, total_q, heads, page_size, page_table_width, max_kv_len, window, sink_tokens)) return -1;
+  if (total_q == 0 || batch == 0) return 0;
+  DeviceInfo* d;
+  if (device_info(&d)) return -1;
+  if (extend_shares(batch, total_q, heads, *d)) {
+    ExtendLayout l;
+    return extend_layout(batch, total_q, heads, max_kv_len, window, sink_tokens, *d, &l) ? -1 : int64_t(l.total);
+  }
+  WindowLayout l;
+  return window_layout(total_q < kExtendSlice ? total_q : kExtendSlice, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)
+             ? -1
+             : int64_t(l.total);
+}
+
+int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, const uint8_t* kpe_cache,
+                     int64_t num_pages, int page_size, const int32_t* page_table, int64_t page_table_stride, int page_table_width,
+                     const int32_t* kv_lens, const int32_t* qo_indptr, int batch, int total_q, int heads, float sm_scale, float ckv_scale,
+                     float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, void* workspace, int64_t workspace_bytes,
+                     int32_t* status, void* stream) {
+  g_error[0] = 0;
+  if (check_extend(batch, total_q, heads, page_size, page_table_width, max_kv_len, window, sink_tokens)) return 1;
+  MLA_CHECK(num_pages > 0 && num_pages * page_size < (int64_t(1) << 31), "num_pages * page_size must be in [1, 2^31)");
+  MLA_CHECK(ckv_scale > 0.f && kpe_scale > 0.f, "ckv_scale and kpe_scale must be positive");
+  MLA_CHECK(page_table_stride >= 0, "page_table_stride must be non-negative");
+  if (total_q == 0) return 0;
+  MLA_CHECK(batch > 0, "query tokens without requests");
+  MLA_CHECK(q_nope && q_pe && ckv_cache && ckv_sf_cache && kpe_cache && (page_table || page_table_width == 0) && kv_lens && qo_indptr && out && workspace,
+            "null pointer argument");
+  MLA_CHECK(aligned(q_nope, 16) && aligned(q_pe, 16) && aligned(ckv_cache, 16) && aligned(ckv_sf_cache, 16) && aligned(kpe_cache, 16) &&
+                aligned(workspace, 256) && aligned(out, 16),
+            "q, caches and out must be 16-byte aligned and the workspace 256-byte aligned");
+  DeviceInfo* d;
+  if (device_info(&d)) return 1;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (!extend_shares(batch, total_q, heads, *d)) {
+    WindowLayout l;
+    if (window_layout(total_q < kExtendSlice ? total_q : kExtendSlice, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)) return 1;
+    MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes, (long long)l.total);
+    return extend_by_token(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, page_table, page_table_stride, page_table_width,
+                           kv_lens, qo_indptr, batch, total_q, heads, sm_scale, ckv_scale, kpe_scale, window, sink_tokens, out, ws, l, status, stream);
+  }
+  ExtendLayout l;
+  if (extend_layout(batch, total_q, heads, max_kv_len, window, sink_tokens, *d, &l)) return 1;
+  MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes, (long long)l.total);
+  CUtensorMap kv_map, q_map;
+  if (make_half_map(ws + l.kv16, int64_t(l.max_tiles) * mla::kExtTile, 128, &kv_map)) return 1;
+  if (make_half_map(ws + l.q16, int64_t(l.max_items) * mla::kExtRows, 64, &q_map)) return 1;
+
+  mla::ExtProblem E;
+  E.kv_lens = kv_lens, E.indptr = qo_indptr, E.batch = batch, E.total_q = total_q, E.heads = heads, E.max_kv_len = max_kv_len;
+  E.window = window, E.sinks = sink_tokens, E.pairs = l.pairs, E.max_items = l.max_items, E.max_tiles = l.max_tiles;
+  E.req_tile0 = reinterpret_cast<int*>(ws + l.req_tile0), E.req_item0 = reinterpret_cast<int*>(ws + l.req_item0);
+  E.req_map = reinterpret_cast<int4*>(ws + l.req_map), E.items = reinterpret_cast<mla::ExtItem*>(ws + l.items);
+  E.pair = reinterpret_cast<mla::ExtPair*>(ws + l.pair), E.counts = reinterpret_cast<int*>(ws + l.counts), E.status = status;
+  mla::ExtOperands O;
+  O.q_nope = static_cast<const __nv_bfloat16*>(q_nope), O.q_pe = static_cast<const __nv_bfloat16*>(q_pe), O.ckv = ckv_cache, O.sf = ckv_sf_cache;
+  O.kpe = kpe_cache, O.page_table = page_table, O.pt_stride = page_table_stride, O.pt_width = page_table_width;
+  O.page_shift = __builtin_ctz(unsigned(page_size)), O.num_pages = int(num_pages), O.ckv_scale = ckv_scale, O.kpe_scale = kpe_scale;
+  O.sm_scale_log2 = sm_scale * 1.4426950408889634f, O.kv16 = reinterpret_cast<__half*>(ws + l.kv16), O.q16 = reinterpret_cast<__half*>(ws + l.q16);
+  O.q_scale = reinterpret_cast<float*>(ws + l.q_scale), O.out = static_cast<uint4*>(out);
+  mla::ExtParams P;
+  P.E = E, P.q_scale = O.q_scale, P.ckv_scale = ckv_scale, P.lse_part = reinterpret_cast<float*>(ws + l.lse_part);
+  P.o_part = reinterpret_cast<float*>(ws + l.o_part), P.out = static_cast<uint16_t*>(out), P.status = status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  mla::mla_extend_schedule_kernel<<<1, mla::kExtSchedThreads, 0, st>>>(E);
+  MLA_CUDA(cudaGetLastError());
+  MLA_CUDA(launch_dependent(mla::mla_extend_prep_kernel, dim3(unsigned(l.max_tiles) + unsigned(l.max_items)), dim3(mla::kExtPrepThreads), 0, st, E, O));
+  MLA_CUDA(launch_dependent_cluster(mla::mla_extend_kernel, dim3(unsigned(2 * l.pairs)), dim3(mla::kExtThreads), mla::ext_smem_bytes(), st, 2u, kv_map,
+                                    q_map, P));
+  MLA_CUDA(launch_dependent(mla::mla_extend_combine_kernel<1>, dim3(unsigned(l.pairs), mla::kExtRows), dim3(128), 0, st, E,
+                            static_cast<const float*>(P.lse_part), static_cast<const float*>(P.o_part), out));
   return 0;
 }
 

@@ -376,6 +376,43 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+// tcgen05 by a pair of CTAs (cta_group::2, a cluster of two): the CTA of rank 0 issues for both. An MMA of M = 128 takes 64
+// rows of A from each CTA's shared memory and the halves of B along N from the two; descriptors and tensor-memory addresses are
+// the same in both CTAs. The accumulator of a CTA's 64 rows fills all 128 lanes: lanes 0..63 hold columns [0, N / 2) of rows 0..63,
+// lanes 64..127 columns [N / 2, N). Allocation and deallocation are made by one warp of each CTA.
+// ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t ncols) {  // whole warp, both CTAs
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {  // whole warp, both CTAs
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {  // whole warp, both CTAs
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D[tmem of both] (+)= A[smem of both] * B[smem of both], descriptors as low words with a common high word; ONE thread of rank 0
+__device__ __forceinline__ void mma_pair_f16_ss_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t a_hi, uint32_t b_hi, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %6, 0;\nmov.b64 da, {%1, %3};\nmov.b64 db, {%2, %4};\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(a_hi), "r"(b_hi), "r"(idesc), "r"(accum)
+      : "memory");
+}
+// the mbarrier at this address arrives in BOTH CTAs once every tcgen05 operation this thread issued so far has completed
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_u32(bar)), "h"(uint16_t(3))
+               : "memory");
+}
+// tiled load into this CTA's shared memory whose bytes are counted on an mbarrier of either CTA of the pair (address from map_to_cta)
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t mbar_cluster_addr) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(mbar_cluster_addr)
+      : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // narrow float conversions
 // ---------------------------------------------------------------------------------------------------------------
 // four bytes of packed E2M1 pairs (low nibble = even channel) -> four f16x2 (exact)
