@@ -13,8 +13,9 @@
 // one fused multiply-add, anything else by the real division. The block scale and the rope pair are treated alike; a
 // power-of-two rope scale needs no enclosure, its products are exact.
 //
-// 1152 bytes in, 352 bytes out per token, bound by instruction issue (343 warp instructions per token, 73 % of the issue slots):
-// 596415 tokens in 219.6 us, 233.7 with the divisions of the block scale and the rope (138 at the measured copy bandwidth).
+// 1152 bytes in, 352 bytes out per token, bound by instruction issue and the latency of the walk through the page tables (194 warp
+// instructions per token, 56 % of the issue slots): 274880 tokens in 82 us (63 at the measured copy bandwidth); 100 with one
+// instruction per product instead of two products per instruction and 64-bit rows.
 // Thirty-two tokens per warp with one walk through the page tables for all of them was slower (246.7 us).
 // One warp per token per trip; lane l owns scale block l
 // (channels 16l .. 16l+15: two 16-byte loads, one 8-byte store, the warp writes the token's 256 packed bytes as one
@@ -76,7 +77,7 @@ template <class Value>
 __device__ __forceinline__ QuantBlock quantize_block(const float (&x)[16], const QuantScales& Q, Value value) {
   float amax = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fmaxf(fabsf(x[2 * j]), fabsf(x[2 * j + 1])));
+  for (int j = 0; j < 8; ++j) amax = ptx::max3(amax, fabsf(x[2 * j]), fabsf(x[2 * j + 1]));
   const uint32_t sf2 = f32x2_to_e4m3x2_sat(amax * Q.six_dn, amax * Q.six_up);
   uint32_t sf8 = sf2 & 0xFFu;
   if (!Q.fast_sf || sf8 != sf2 >> 8) sf8 = f32x2_to_e4m3x2_sat(__fdiv_rn(__fdiv_rn(amax, 6.0f), Q.ckv_scale), 0.f) & 0xFFu;
@@ -86,7 +87,10 @@ __device__ __forceinline__ QuantBlock quantize_block(const float (&x)[16], const
     const float r = __frcp_rn(sf), rd = r * kQuantDown, ru = r * kQuantUp;
     float yd[16], yu[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) yd[j] = x[j] * rd, yu[j] = x[j] * ru;
+    for (int j = 0; j < 16; j += 2) {
+      const float2 d = ptx::mul_f32x2(make_float2(x[j], x[j + 1]), make_float2(rd, rd)), u = ptx::mul_f32x2(make_float2(x[j], x[j + 1]), make_float2(ru, ru));
+      yd[j] = d.x, yd[j + 1] = d.y, yu[j] = u.x, yu[j + 1] = u.y;
+    }
     lo = e2m1x8(reinterpret_cast<const float(&)[8]>(yd[0])), hi = e2m1x8(reinterpret_cast<const float(&)[8]>(yd[8]));
     const uint32_t dlo = lo ^ e2m1x8(reinterpret_cast<const float(&)[8]>(yu[0]));
     const uint32_t dhi = hi ^ e2m1x8(reinterpret_cast<const float(&)[8]>(yu[8]));
@@ -120,14 +124,13 @@ __device__ __forceinline__ uint32_t quantize_rope_pair(float x0, float x1, const
 }
 
 // cache row of position `pos` of request `b`; negative if the request, the position or the page lies outside the tables
-__device__ __forceinline__ long long cache_row(int b, int pos, long long num_pages, int page_shift, const int* kv_indices,
-                                               const int* kv_indptr, int batch) {
+__device__ __forceinline__ int cache_row(int b, int pos, int num_pages, int page_shift, const int* kv_indices, const int* kv_indptr, int batch) {
   if (b < 0 || b >= batch || pos < 0) return -1;
   const int first = kv_indptr[b], npages = kv_indptr[b + 1] - first, pi = pos >> page_shift;
   if (pi >= npages) return -1;
   const int page = kv_indices[first + pi];
   if (page < 0 || page >= num_pages) return -1;
-  return ((long long)page << page_shift) + (pos & ((1 << page_shift) - 1));
+  return (page << page_shift) + (pos & ((1 << page_shift) - 1));  // (the pool has fewer than 2^31 rows)
 }
 
 // status: optional device word, set to 1 if a token named a request, position or page outside the tables (the token
@@ -148,7 +151,7 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
     const uint4 w0 = src[0], w1 = src[1];
     const uint32_t rope = reinterpret_cast<const uint32_t*>(kpe + t * KPE)[lane];
     const int b = batch_indices[t], pos = positions[t];
-    const long long row = cache_row(b, pos, num_pages, page_shift, kv_indices, kv_indptr, batch);
+    const long long row = cache_row(b, pos, int(num_pages), page_shift, kv_indices, kv_indptr, batch);
     if (row < 0) {
       if (lane == 0 && status) *status = 1;
       continue;
@@ -176,16 +179,28 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 //   rope   : the pair (a, b) of position p turns into (a cos - b sin, b cos + a sin) with row p of the cos | sin table, as an
 //            fp32 number, then as BF16
 //   then the writer's own steps (above): the bytes are those of mla_quantize_append_kernel on the BF16 rows.
-// A code of the cache changes by a whole step where a value crosses a rounding border, so the BF16 values themselves are exact:
-// the sum of squares is taken in 64 bits, the product with the reciprocal root in fp32 (within two units in the last place of
-// the defined one), and a product that close to a BF16 border (one in ten thousand) again in 64 bits. The rope products are taken in
-// 64 bits at once: they cancel, and there are two per lane.
+// A code of the cache changes by a whole step where a value crosses a rounding border, so the BF16 values themselves are exact. They
+// are computed in fp32 with an error bound, and a value that close to a BF16 border is computed again in 64 bits:
+//   latent: the squares are exact in fp32 (eight bits times eight), their sum passes nine rounding additions (four levels of a tree in
+//           a lane, five shuffles): within 9 * 2^-24 of itself; eps and its addition (2 * 2^-24 of the mean, half of it in the root),
+//           the reciprocal root (two units) and the product (x w is exact) make y off by at most 11 units in its last place. One
+//           value in 2600 is that close to a border, one token in five has such a value.
+//   rope  : a cos - b sin as fma(a, cos, -p) - fma(b, sin, -p) with p = b sin rounded, which is within two units of the defined number.
 //
 // One warp per token per trip, lane l = scale block l, as above; a lane's normalised BF16 values sit in shared memory for the few that
-// have to be settled.
+// have to be settled, the weights there too. 1512 bytes per token, bound by the latency of a warp's chain of steps (414 warp
+// instructions per token, 65 % of the issue slots): 274880 tokens in 147 us (63 at the measured copy bandwidth; the writer above 82).
+// With the norm in 64 bits throughout it took 345 us, one instruction per value and step 273; fetching the next token's row
+// ahead gained nothing at the registers it took (149), and 24 or 40 warps per SM instead of 32 were 149 to 154.
 // ---------------------------------------------------------------------------------------------------------------
+// whether the fp32 number y, off by at most `units` in its last place, may round to another BF16 number than what it stands for: its low
+// half is within `units` of 0x8000
+__device__ __forceinline__ bool near_bf16_border(float y, uint32_t units) {
+  return ((__float_as_uint(y) - 0x8000u + units) & 0xFFFFu) <= 2 * units;
+}
+
 template <bool INTERLEAVED>
-__global__ void __launch_bounds__(kQuantThreads)
+__global__ void __launch_bounds__(kQuantThreads, 4)
 mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv_stride, const __nv_bfloat16* __restrict__ kpe,
                             long long kpe_stride, const __nv_bfloat16* __restrict__ weight, const float* __restrict__ cos_sin,
                             int max_pos, double eps, const int* __restrict__ batch_indices, const int* __restrict__ positions,
@@ -193,72 +208,103 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
                             uint8_t* __restrict__ kpe_cache, long long num_pages, int page_shift,
                             const int* __restrict__ kv_indices, const int* __restrict__ kv_indptr, int batch, float ckv_scale,
                             float kpe_scale, int* status) {
-  __shared__ uint32_t held[kQuantThreads][9];  // a lane's 16 values, rows of nine words: no bank conflicts
+  __shared__ uint4 held[2][kQuantThreads];  // a lane's 16 normalised values
+  __shared__ float4 gains[4][32];           // the weights: lane l's 16
   const int lane = threadIdx.x & 31;
   const QuantScales Q(ckv_scale, kpe_scale);
-  uint32_t wt[8];
-  {
-    const uint4* src = reinterpret_cast<const uint4*>(weight + 16 * lane);
-    const uint4 a = __ldg(src), b = __ldg(src + 1);
-    wt[0] = a.x, wt[1] = a.y, wt[2] = a.z, wt[3] = a.w, wt[4] = b.x, wt[5] = b.y, wt[6] = b.z, wt[7] = b.w;
+  const float eps_f = float(eps);
+  bool ordinary_gains = true;  // 0 or of ordinary size
+  for (int i = threadIdx.x; i < CKV; i += kQuantThreads) {
+    const float g = __bfloat162float(weight[i]);
+    reinterpret_cast<float*>(&gains[(i & 15) >> 2][i >> 4])[i & 3] = g;
+    ordinary_gains &= g == 0.f || (fabsf(g) > 0x1p-20f && fabsf(g) < 0x1p20f);
   }
+  ordinary_gains = __syncthreads_and(ordinary_gains);
   const long long warp0 = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   const long long stride = (long long)gridDim.x * (kQuantThreads / 32);
   for (long long t = warp0; t < nnz; t += stride) {
     const uint4* src = reinterpret_cast<const uint4*>(ckv + t * ckv_stride + 16 * lane);
-    const uint4 w0 = src[0], w1 = src[1];
+    const uint4 w0 = __ldcs(src), w1 = __ldcs(src + 1);
     const __nv_bfloat16* rp = kpe + t * kpe_stride;
-    float a, b;
-    if constexpr (INTERLEAVED) {
-      const uint32_t rope = reinterpret_cast<const uint32_t*>(rp)[lane];
-      a = __uint_as_float(rope << 16), b = __uint_as_float(rope & 0xFFFF0000u);
-    } else {
-      a = __bfloat162float(rp[lane]), b = __bfloat162float(rp[32 + lane]);
-    }
+    uint32_t rope;  // interleaved: the pair; else channel `lane` and, above it, channel 32 + lane
+    if constexpr (INTERLEAVED) rope = __ldcs(reinterpret_cast<const uint32_t*>(rp) + lane);
+    else rope = uint32_t(__ldcs(reinterpret_cast<const uint16_t*>(rp) + lane)) | uint32_t(__ldcs(reinterpret_cast<const uint16_t*>(rp) + 32 + lane)) << 16;
+    const float a = __uint_as_float(rope << 16), b = __uint_as_float(rope & 0xFFFF0000u);
     const int pos = positions[t];
-    const long long row = pos < max_pos ? cache_row(batch_indices[t], pos, num_pages, page_shift, kv_indices, kv_indptr, batch) : -1;
+    // (the slot is needed at the end only: the arithmetic does not wait for the walk through the page tables)
+    const long long row = pos < max_pos ? cache_row(batch_indices[t], pos, int(num_pages), page_shift, kv_indices, kv_indptr, batch) : -1;
+    const bool rotated = uint32_t(pos) < uint32_t(max_pos);
+    const float cs = rotated ? __ldg(cos_sin + (long long)pos * KPE + lane) : 0.f, sn = rotated ? __ldg(cos_sin + (long long)pos * KPE + 32 + lane) : 0.f;
+    const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+    auto two = [](uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); };
+    float2 sq[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sq[j] = ptx::mul_f32x2(two(w[j]), two(w[j]));
+#pragma unroll
+    for (int n = 4; n; n >>= 1)
+#pragma unroll
+      for (int j = 0; j < n; ++j) sq[j] = ptx::add_f32x2(sq[j], sq[j + n]);
+    float sum = __fadd_rn(sq[0].x, sq[0].y);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(~0u, sum, o));
+    const float mean = __fadd_rn(sum * (1.f / CKV), eps_f), r = rsqrtf(mean);
+    // (fp32 holds the row and the products well inside its range)
+    const bool ordinary = mean > 0x1p-60f && mean < 0x1p60f && ordinary_gains;
+    uint32_t held_[8], nearest = 0xFFFFFFFFu;  // smallest distance to a border seen, two at a time: (low half of y) - 0x8000 + 12
+    auto gain4 = [&](int k) { return gains[k][lane]; };  // weights 4k .. of the lane
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 g = gain4(k);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = 2 * k + e;
+        const float2 y = ptx::mul_f32x2(ptx::mul_f32x2(two(w[j]), e ? make_float2(g.z, g.w) : make_float2(g.x, g.y)), make_float2(r, r));
+        nearest = __viaddmin_u16x2(__byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x5410), 0x800C800Cu, nearest);
+        held_[j] = ptx::f32x2_to_bf16x2(y.x, y.y);
+      }
+    }
+    const bool near = (nearest & 0xFFFFu) <= 24u || nearest >> 16 <= 24u || !ordinary;
+    if (__any_sync(~0u, near)) {
+      double s2 = 0.;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double u = double(two(w[j]).x), v = double(two(w[j]).y);
+        s2 = fma(u, u, s2), s2 = fma(v, v, s2);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s2 += __shfl_xor_sync(~0u, s2, o);
+      const double rd = rsqrt(s2 * (1. / CKV) + eps);
+      if (near) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 g = gain4(j >> 1);
+          const float2 a2 = two(w[j]), g2 = j & 1 ? make_float2(g.z, g.w) : make_float2(g.x, g.y);
+          held_[j] = ptx::f32x2_to_bf16x2(float(double(a2.x) * double(g2.x) * rd), float(double(a2.y) * double(g2.y) * rd));
+        }
+      }
+    }
+    held[0][threadIdx.x] = make_uint4(held_[0], held_[1], held_[2], held_[3]), held[1][threadIdx.x] = make_uint4(held_[4], held_[5], held_[6], held_[7]);
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[2 * j] = two(held_[j]).x, x[2 * j + 1] = two(held_[j]).y;
+    const QuantBlock q = quantize_block(x, Q, [&](int j) {
+      const uint32_t v = reinterpret_cast<const uint32_t*>(&held[j >> 3][threadIdx.x])[j >> 1 & 3];
+      return __uint_as_float(j & 1 ? v & 0xFFFF0000u : v << 16);
+    });
     if (row < 0) {
       if (lane == 0 && status) *status = 1;
       continue;
     }
-    const float cs = __ldg(cos_sin + (long long)pos * KPE + lane), sn = __ldg(cos_sin + (long long)pos * KPE + 32 + lane);
-    const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-    double sum = 0.;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double u = double(__uint_as_float(w[j] << 16)), v = double(__uint_as_float(w[j] & 0xFFFF0000u));
-      sum = fma(u, u, sum), sum = fma(v, v, sum);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    const double r = rsqrt(sum * (1. / CKV) + eps);
-    const float rf = float(r);
-    const bool plain_row = rf > 0x1p-60f && rf < 0x1p60f;
-    float x[16];
-    uint32_t* const mine = held[threadIdx.x];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t pair = 0;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float xv = __uint_as_float(e ? w[j] & 0xFFFF0000u : w[j] << 16), wv = __uint_as_float(e ? wt[j] & 0xFFFF0000u : wt[j] << 16);
-        const float p = __fmul_rn(xv, wv);  // exact: eight bits times eight bits
-        float y = __fmul_rn(p, rf);
-        const uint32_t low = (__float_as_uint(y) - 0x7FFDu) & 0xFFFFu;  // up to 6: within three units of a BF16 border
-        const float size = fabsf(p);
-        if (low <= 6u || !plain_row || !(size > 0x1p-60f && size < 0x1p60f)) y = float(double(xv) * double(wv) * r);
-        const uint32_t h = __bfloat16_as_ushort(__float2bfloat16_rn(y));
-        x[2 * j + e] = __uint_as_float(h << 16);
-        pair |= h << (16 * e);
-      }
-      mine[j] = pair;
-    }
-    const QuantBlock q = quantize_block(x, Q, [&](int j) { return __uint_as_float(j & 1 ? mine[j >> 1] & 0xFFFF0000u : mine[j >> 1] << 16); });
     *reinterpret_cast<uint2*>(ckv_cache + row * (CKV / 2) + 8 * lane) = make_uint2(q.lo, q.hi);
     sf_cache[row * (CKV / 16) + lane] = uint8_t(q.sf8);
-    const double c = double(cs), s = double(sn);
-    const float x0 = __bfloat162float(__float2bfloat16_rn(float(fma(double(a), c, -(double(b) * s)))));
-    const float x1 = __bfloat162float(__float2bfloat16_rn(float(fma(double(b), c, double(a) * s))));
+    const float p0 = __fmul_rn(b, sn), p1 = __fmul_rn(a, sn);
+    float x0 = __fsub_rn(__fmaf_rn(a, cs, -p0), __fmaf_rn(b, sn, -p0)), x1 = __fadd_rn(__fmaf_rn(b, cs, p1), __fmaf_rn(a, sn, -p1));
+    const bool tiny = fabsf(x0) < 0x1p-60f || fabsf(x1) < 0x1p-60f;  // (the products' errors may be below fp32's range)
+    if (near_bf16_border(x0, 3) || near_bf16_border(x1, 3) || tiny || !(fabsf(x0) < 0x1p100f && fabsf(x1) < 0x1p100f)) {
+      const double da = double(a), db = double(b), dc = double(cs), ds = double(sn);
+      x0 = float(fma(da, dc, -(db * ds))), x1 = float(fma(db, dc, da * ds));
+    }
+    x0 = __bfloat162float(__float2bfloat16_rn(x0)), x1 = __bfloat162float(__float2bfloat16_rn(x1));
     const uint32_t k8 = quantize_rope_pair(x0, x1, Q);
     if constexpr (INTERLEAVED) {
       reinterpret_cast<uint16_t*>(kpe_cache + row * KPE)[lane] = uint16_t(k8);

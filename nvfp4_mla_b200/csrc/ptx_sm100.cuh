@@ -415,6 +415,12 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
 // ---------------------------------------------------------------------------------------------------------------
 // narrow float conversions
 // ---------------------------------------------------------------------------------------------------------------
+// two floats -> bf16x2, round to nearest even (lo in the low half)
+__device__ __forceinline__ uint32_t f32x2_to_bf16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
 // four bytes of packed E2M1 pairs (low nibble = even channel) -> four f16x2 (exact)
 __device__ __forceinline__ void e2m1x8_to_f16x8(uint32_t w, uint32_t (&h)[4]) {
   asm("{\n.reg .b8 b0, b1, b2, b3;\n"
@@ -505,6 +511,13 @@ __device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
       "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
 __device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
