@@ -174,7 +174,9 @@ int device_info(DeviceInfo** out) {
       return clusters < d.sm_count / 2 ? clusters : d.sm_count / 2;
     };
     d.hm_pairs = resident_pairs(decode_entry(NVFP4_MLA_PRECISION_FP8, 128), mla::kHmThreads, decode_smem(NVFP4_MLA_PRECISION_FP8, 128));
+    static_assert(mla::kExtMaxPairs >= 74, "more pairs than the chunk schedule has room for");
     d.ext_pairs = resident_pairs(reinterpret_cast<const void*>(mla::mla_extend_kernel), mla::kExtThreads, mla::ext_smem_bytes());
+    if (d.ext_pairs > mla::kExtMaxPairs) d.ext_pairs = mla::kExtMaxPairs;
     if (getenv("NVFP4_MLA_DEBUG"))
       fprintf(stderr, "nvfp4_mla_b200: device %d: %d SMs, %d resident CTA pairs for the 128-head kernel, %d for chunk attention\n", dev, d.sm_count,
               d.hm_pairs, d.ext_pairs);
@@ -530,7 +532,7 @@ namespace {
 constexpr int kExtendSlice = 512;  // query tokens at a time in the first form (the partial results of a slice take 2 KB per head and token)
 
 struct ExtendLayout {
-  size_t counts, req_tile0, req_item0, req_map, items, pair, q_scale, lse_part, o_part, q16, kv16, total;
+  size_t counts, req_tile0, req_map, items, pair, q_scale, lse_part, o_part, q16, kv16, total;
   int pairs, max_items, max_tiles;
 };
 int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window, int sinks, const DeviceInfo& d, ExtendLayout* l) {
@@ -553,7 +555,7 @@ int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window,
     off = mla::align_up(off + bytes, 256);
     return at;
   };
-  l->counts = take(64), l->req_tile0 = take(size_t(batch + 1) * 4), l->req_item0 = take(size_t(batch + 1) * 4), l->req_map = take(size_t(batch) * 16);
+  l->counts = take(64), l->req_tile0 = take(size_t(batch + 1) * 4), l->req_map = take(size_t(batch) * 16);
   l->items = take(size_t(items) * sizeof(mla::ExtItem)), l->pair = take(size_t(l->pairs) * sizeof(mla::ExtPair));
   l->q_scale = take(size_t(items) * mla::kExtRows * 4);
   l->lse_part = take(size_t(l->pairs) * 2 * mla::kExtRows * 4), l->o_part = take(size_t(l->pairs) * 2 * mla::kExtRows * mla::CKV * 4);
@@ -562,13 +564,13 @@ int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window,
   return 0;
 }
 
-// FP16 rows of 576 as a map of [rows, 576], boxes of 64 channels x `box_rows` rows with the 128-byte swizzle
-int make_half_map(const void* base, int64_t rows, int box_rows, CUtensorMap* map) {
+// FP16 rows of 576 as a map of [rows, 576], boxes of 64 channels x 64 rows with the 128-byte swizzle
+int make_half_map(const void* base, int64_t rows, CUtensorMap* map) {
   EncodeTiledFn encode;
   if (encode_fn(&encode)) return 1;
   const cuuint64_t dims[2] = {cuuint64_t(mla::kExtRow), cuuint64_t(rows)};
   const cuuint64_t strides[1] = {cuuint64_t(mla::kExtRow) * 2};
-  const cuuint32_t box[2] = {64, cuuint32_t(box_rows)};
+  const cuuint32_t box[2] = {64, 64};
   const cuuint32_t elem_strides[2] = {1, 1};
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, elem_strides,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -672,13 +674,13 @@ int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_ca
   if (extend_layout(batch, total_q, heads, max_kv_len, window, sink_tokens, *d, &l)) return 1;
   MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes, (long long)l.total);
   CUtensorMap kv_map, q_map;
-  if (make_half_map(ws + l.kv16, int64_t(l.max_tiles) * mla::kExtTile, 128, &kv_map)) return 1;
-  if (make_half_map(ws + l.q16, int64_t(l.max_items) * mla::kExtRows, 64, &q_map)) return 1;
+  if (make_half_map(ws + l.kv16, int64_t(l.max_tiles) * mla::kExtTile, &kv_map)) return 1;
+  if (make_half_map(ws + l.q16, int64_t(l.max_items) * mla::kExtRows, &q_map)) return 1;
 
   mla::ExtProblem E;
   E.kv_lens = kv_lens, E.indptr = qo_indptr, E.batch = batch, E.total_q = total_q, E.heads = heads, E.max_kv_len = max_kv_len;
   E.window = window, E.sinks = sink_tokens, E.pairs = l.pairs, E.max_items = l.max_items, E.max_tiles = l.max_tiles;
-  E.req_tile0 = reinterpret_cast<int*>(ws + l.req_tile0), E.req_item0 = reinterpret_cast<int*>(ws + l.req_item0);
+  E.req_tile0 = reinterpret_cast<int*>(ws + l.req_tile0);
   E.req_map = reinterpret_cast<int4*>(ws + l.req_map), E.items = reinterpret_cast<mla::ExtItem*>(ws + l.items);
   E.pair = reinterpret_cast<mla::ExtPair*>(ws + l.pair), E.counts = reinterpret_cast<int*>(ws + l.counts), E.status = status;
   mla::ExtOperands O;
@@ -693,11 +695,13 @@ int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_ca
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   mla::mla_extend_schedule_kernel<<<1, mla::kExtSchedThreads, 0, st>>>(E);
   MLA_CUDA(cudaGetLastError());
-  MLA_CUDA(launch_dependent(mla::mla_extend_prep_kernel, dim3(unsigned(l.max_tiles) + unsigned(l.max_items)), dim3(mla::kExtPrepThreads), 0, st, E, O));
+  const int64_t units = int64_t(l.max_tiles) * (mla::kExtTile / mla::kExtTokens) + int64_t(l.max_items) * (mla::kExtRows / mla::kExtQRows);
+  const int64_t resident = int64_t(d->sm_count) * (2048 / mla::kExtPrepThreads);
+  MLA_CUDA(launch_dependent(mla::mla_extend_prep_kernel, dim3(unsigned(units < resident ? units : resident)), dim3(mla::kExtPrepThreads), 0, st, E, O));
   MLA_CUDA(launch_dependent_cluster(mla::mla_extend_kernel, dim3(unsigned(2 * l.pairs)), dim3(mla::kExtThreads), mla::ext_smem_bytes(), st, 2u, kv_map,
                                     q_map, P));
-  MLA_CUDA(launch_dependent(mla::mla_extend_combine_kernel<1>, dim3(unsigned(l.pairs), mla::kExtRows), dim3(128), 0, st, E,
-                            static_cast<const float*>(P.lse_part), static_cast<const float*>(P.o_part), out));
+  MLA_CUDA(launch_dependent(mla::mla_extend_combine_kernel, dim3(unsigned(l.pairs), mla::kExtRows / 4), dim3(128), 0, st, E,
+                            static_cast<const float*>(P.lse_part), static_cast<const float*>(P.o_part), static_cast<uint2*>(out)));
   return 0;
 }
 

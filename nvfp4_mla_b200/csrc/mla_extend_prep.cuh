@@ -1,7 +1,11 @@
 // Chunks of new tokens, everything around the attention kernel (mla_extend_sm100.cuh): the schedule, the FP16 operands, the merge.
 //
 // The rows of a request (query token, head) are cut into tiles of 128, the ITEMS; an item's work is the 256-token tiles of the cache
-// that its rows see. The items' tiles are laid end to end and cut into equal pieces, one per CTA pair.
+// that its rows see. The items are dealt out whole, item i to CTA pair i % pairs, for as many rounds as leave every pair at or below
+// its even share of the tiles; the tiles of the items that are left are laid end to end and cut so that every pair ends up with its
+// share. Pairs that work at the same time thus work on neighbouring items, which read the same tokens: with one contiguous piece of
+// the flattened tiles per pair, 24 ragged chunks over 115 MB of FP16 rows read 1.6 GB from HBM (a third of the sectors missed L2) and
+// took 913 us.
 //
 // Window: the tokens that some query of the request sees are [0, S) and everything from the first query's window on. The cache is
 // read into a numbering of tiles that has no gap: the first `sink_tiles` tiles, then the tiles from the window's on, `shift` tokens
@@ -26,6 +30,7 @@ constexpr int kExtRows = 128;   // rows of an item
 constexpr int kExtTile = 256;   // tokens of a tile
 constexpr int kExtRow = CKV + KPE;
 constexpr int kExtMaxBatch = 8192;
+constexpr int kExtMaxPairs = 128;
 
 struct ExtItem {
   int prefix;      // tiles of the items before
@@ -41,8 +46,10 @@ struct ExtItem {
 static_assert(sizeof(ExtItem) == 64, "ExtItem is a cache line half");
 
 struct ExtPair {
-  int item, first, count;  // first item, first flattened tile, tiles
-  int split;               // item whose first tiles this pair holds and whose last ones another does, or -1
+  int rounds;              // whole items pair, pair + pairs, ...: this many
+  int item, first, count;  // and of the rest: first item, first flattened tile, tiles
+  int split, parts;        // item whose first tiles this pair holds and whose last ones another does, or -1; pairs that share it
+  int pad[2];
 };
 
 // What the caller gives and how much room there is
@@ -52,7 +59,6 @@ struct ExtProblem {
   int batch, total_q, heads, max_kv_len, window, sinks, pairs;
   int max_items, max_tiles;
   int* req_tile0;   // [batch + 1] workspace tiles before request b
-  int* req_item0;   // [batch + 1] items before request b
   int4* req_map;    // [batch] {shift, first tokens' tiles, tokens in the tiles (with the shift taken out), first token of the window}
   ExtItem* items;   // [max_items]
   ExtPair* pair;    // [pairs]
@@ -62,8 +68,8 @@ struct ExtProblem {
 
 constexpr int kExtSchedThreads = 1024;
 
-// inclusive scan over the block; `sums`: one int per warp
-__device__ __forceinline__ int block_scan(int v, int* sums) {
+// inclusive scan over the block (every thread takes part); `sums`: 33 ints; the block's sum in `all`
+__device__ __forceinline__ int block_scan(int v, int* sums, int& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -73,9 +79,18 @@ __device__ __forceinline__ int block_scan(int v, int* sums) {
   __syncthreads();
   if (lane == 31) sums[warp] = v;
   __syncthreads();
-  int base = 0;
-  for (int i = 0; i < warp; ++i) base += sums[i];
-  return base + v;
+  if (warp == 0) {
+    int w = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(~0u, w, o);
+      if (lane >= o) w += u;
+    }
+    sums[lane] = w;
+  }
+  __syncthreads();
+  all = sums[31];
+  return v + (warp ? sums[warp - 1] : 0);
 }
 
 struct ExtRequest {
@@ -106,37 +121,40 @@ __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
 
 __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kernel(const ExtProblem E) {
   __shared__ int item0[kExtMaxBatch + 1];
-  __shared__ int sums[kExtSchedThreads / 32];
+  __shared__ int sums[33];
+  __shared__ int cut[kExtMaxPairs + 1];  // tiles of the rest before pair p
+  __shared__ int rounds_s;
+  static_assert(kExtSchedThreads == 1024, "block_scan takes 32 warps");
   ptx::grid_launch_dependents();
   const int tid = threadIdx.x;
   int items = 0, tiles = 0;
+  ExtRequest r = {};
   for (int b0 = 0; b0 < E.batch; b0 += kExtSchedThreads) {
     const int b = b0 + tid;
-    ExtRequest r = {};
-    int mine = 0;
+    int mine = 0, all;
+    r = {};
     if (b < E.batch) {
       r = ext_request(E, b);
       mine = int(((long long)r.q * E.heads + kExtRows - 1) / kExtRows);
     }
-    const int ii = block_scan(mine, sums), it = block_scan(r.tiles, sums);
+    const int ii = items + block_scan(mine, sums, all) - mine;
+    items += all;
+    const int it = tiles + block_scan(r.tiles, sums, all) - r.tiles;
+    tiles += all;
     if (b < E.batch) {
-      item0[b] = items + ii - mine;
-      E.req_item0[b] = items + ii - mine, E.req_tile0[b] = tiles + it - r.tiles;
+      item0[b] = ii, E.req_tile0[b] = it;
       E.req_map[b] = make_int4(r.shift, r.sink_tiles, r.n - r.shift, r.begin);
     }
-    __shared__ int last[2];
-    if (tid == kExtSchedThreads - 1) last[0] = ii, last[1] = it;
-    __syncthreads();
-    items += last[0], tiles += last[1];
-    __syncthreads();
   }
   // (a query index that runs backwards could ask for more than there is room for)
   if (items > E.max_items || tiles > E.max_tiles) {
     if (tid == 0 && E.status) atomicExch(E.status, int(kBadSchedule));
     items = 0, tiles = 0;
   }
-  if (tid == 0) item0[E.batch] = items, E.req_item0[E.batch] = items, E.req_tile0[E.batch] = tiles, E.counts[0] = items, E.counts[1] = tiles;
+  if (tid == 0) E.req_tile0[E.batch] = tiles, E.counts[0] = items, E.counts[1] = tiles, rounds_s = items / E.pairs;
   __syncthreads();
+
+  // ---- items
   int total = 0;
   for (int i0 = 0; i0 < items; i0 += kExtSchedThreads) {
     const int i = i0 + tid;
@@ -148,7 +166,7 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
         if (item0[mid] <= i) lo = mid;
         else hi = mid - 1;
       }
-      const ExtRequest r = ext_request(E, lo);
+      r = ext_request(E, lo);
       m.r0 = (i - item0[lo]) * kExtRows;
       const long long rows = (long long)r.q * E.heads - m.r0;
       m.rows = int(rows < kExtRows ? rows : kExtRows);
@@ -156,9 +174,8 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
       const int first = r.pos0 + m.r0 / E.heads, last = r.pos0 + (m.r0 + m.rows - 1) / E.heads;  // positions of its query tokens
       const int end = last + 1 < r.n ? last + 1 : r.n;                                           // tokens before it are seen
       int e = (end - r.shift + kExtTile - 1) / kExtTile;                                         // tiles up to there
-      m.sinks = 0, m.skip = 0;
       if (E.window > 0) {
-        long long begin = (long long)first - E.window + 1 - r.shift;
+        const long long begin = (long long)first - E.window + 1 - r.shift;
         const int t = begin > 0 ? int(begin / kExtTile) : 0;
         m.sinks = r.sink_tiles;
         if (t > m.sinks) m.skip = t - m.sinks;
@@ -167,44 +184,76 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
       m.ntiles = e - m.skip;
       if (m.ntiles < 1) m.ntiles = 1, m.skip = 0;
     }
-    const int incl = block_scan(m.ntiles, sums);
+    int all;
+    const int incl = block_scan(m.ntiles, sums, all);
     if (i < items) {
       m.prefix = total + incl - m.ntiles;
       E.items[i] = m;
     }
-    __shared__ int last_sum;
-    if (tid == kExtSchedThreads - 1) last_sum = incl;
-    __syncthreads();
-    total += last_sum;
-    __syncthreads();
+    total += all;
   }
-  const int q = total > 0 ? (total + E.pairs - 1) / E.pairs : 1;
-  __threadfence_block();
   __syncthreads();
-  for (int p = tid; p < E.pairs; p += kExtSchedThreads) {
-    ExtPair o = {0, p * q, 0, -1};
-    if ((long long)p * q < total) {
-      o.count = total - o.first < q ? total - o.first : q;
-      auto item_of = [&](int g) {
-        int lo = 0, hi = items - 1;  // last item with prefix <= g
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (E.items[mid].prefix <= g) lo = mid;
-          else hi = mid - 1;
-        }
-        return lo;
-      };
-      o.item = item_of(o.first);
-      const int end = o.first + o.count, z = item_of(end - 1);
-      if (E.items[z].prefix >= o.first && E.items[z].prefix + E.items[z].ntiles > end) o.split = z;
+
+  // ---- rounds of whole items
+  const int share = total > 0 ? (total + E.pairs - 1) / E.pairs : 1, most = items / E.pairs;
+  constexpr int kAhead = 8;  // loads in flight
+  auto load_after = [&](int rounds, int limit, int& fits) {  // tiles of this pair's first `rounds` items; how many of them stay within `limit`
+    int sum = 0;
+    fits = 0;
+    for (int k = 0; k < rounds; k += kAhead) {
+      int n[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) n[j] = k + j < rounds ? E.items[tid + (k + j) * E.pairs].ntiles : 0;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        sum += n[j];
+        if (k + j < rounds && sum <= limit) fits = k + j + 1;
+      }
     }
-    E.pair[p] = o;
+    return sum;
+  };
+  int fits, load = 0;
+  if (tid < E.pairs) {
+    load = load_after(most, share, fits);
+    if (fits < most) atomicMin(&rounds_s, fits);
+  }
+  __syncthreads();
+  const int rounds = rounds_s;
+  if (tid < E.pairs && rounds < most) load = load_after(rounds, share, fits);
+  // ---- the rest: cut at the pairs' remaining shares
+  const int rest0 = rounds * E.pairs;                                       // first item of the rest
+  const int base = rest0 < items ? E.items[rest0].prefix : total, rest = total - base;
+  int room = tid < E.pairs ? share - load : 0, all;
+  const int at = block_scan(room, sums, all) - room;
+  if (tid < E.pairs) {
+    const int lo = at < rest ? at : rest, hi = at + room < rest ? at + room : rest;
+    cut[tid] = lo;
+    if (tid == E.pairs - 1) cut[E.pairs] = rest;
+    ExtPair o = {rounds, 0, base + lo, hi - lo, -1, 0, {0, 0}};
+    E.pair[tid] = o;
+  }
+  __syncthreads();
+  for (int i = rest0 + tid; i < items; i += kExtSchedThreads) {
+    const int a = E.items[i].prefix - base, z = a + E.items[i].ntiles;
+    auto holder = [&](int x) {  // last pair whose piece starts at or before tile x (pieces without tiles lie in front of it)
+      int lo = 0, hi = E.pairs - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cut[mid] <= x) lo = mid;
+        else hi = mid - 1;
+      }
+      return lo;
+    };
+    const int p0 = holder(a), p1 = holder(z - 1);
+    for (int p = cut[p0] == a ? p0 : p0 + 1; p <= p1; ++p)
+      if (cut[p + 1] > cut[p]) E.pair[p].item = i;
+    if (p1 > p0) E.pair[p0].split = i, E.pair[p0].parts = p1 - p0 + 1;
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Operands. Blocks [0, max_tiles): one 256-token tile of the workspace each; the others: one item's query rows each. All blocks
-// share the rows of no request (zeros in the output).
+// Operands. A unit of work is 64 tokens of a workspace tile or 32 rows of an item, 8 or 4 per warp: all loads of a warp's four rows are
+// issued before the first is used. All blocks share the rows of no request (zeros in the output).
 // ---------------------------------------------------------------------------------------------------------------
 struct ExtOperands {
   const __nv_bfloat16* q_nope;
@@ -223,19 +272,31 @@ struct ExtOperands {
 };
 
 constexpr int kExtPrepThreads = 256;
+constexpr int kExtTokens = 64;  // tokens of a unit
+constexpr int kExtQRows = 32;   // rows of a unit
 
-__device__ __forceinline__ void ext_convert_tile(const ExtProblem& E, const ExtOperands& O, int tile) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int lo = 0, hi = E.batch - 1;  // last b with req_tile0[b] <= tile
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (E.req_tile0[mid] <= tile) lo = mid;
-    else hi = mid - 1;
+// last b in [0, n) with a[b] <= x (a is non-decreasing, a[0] <= x), by the whole warp: 32 probes at a time
+__device__ __forceinline__ int warp_upper(const int* __restrict__ a, int n, int x) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 31) >> 5, i = lo + lane * step;
+    const uint32_t below = __ballot_sync(~0u, lane * step < n && a[i] <= x);  // a prefix of the lanes, lane 0 in it
+    const int k = 31 - __clz(below);
+    lo += k * step, n = n - k * step < step ? n - k * step : step;
   }
+  return lo;
+}
+
+__device__ __forceinline__ void ext_convert_tokens(const ExtProblem& E, const ExtOperands& O, int unit) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kPer = kExtTokens / (kExtPrepThreads / 32);  // tokens of a warp
+  const int t0 = unit * kExtTokens + kPer * warp, tile = t0 / kExtTile;
+  const int lo = warp_upper(E.req_tile0, E.batch, tile);
   const int4 map = E.req_map[lo];
-  const int v = (tile - E.req_tile0[lo]) * kExtTile + 32 * warp + lane;  // this lane's token among the request's
-  int src = -1;                                                          // its cache row; -1: zeros
-  if (v < map.z) {
+  const int v = t0 - E.req_tile0[lo] * kExtTile + lane;  // this lane's token among the request's
+  int src = -1;                                          // its cache row; -1: zeros
+  if (lane < kPer && v < map.z) {
     const int tok = v < map.y * kExtTile ? v : v + map.x;
     // (tokens between the first ones and the window belong to tiles that are read, but their pages may be gone)
     if (tok < E.sinks || tok >= map.w) {
@@ -245,10 +306,10 @@ __device__ __forceinline__ void ext_convert_tile(const ExtProblem& E, const ExtO
       else if (E.status) atomicExch(E.status, int(kBadPage));
     }
   }
-  __half* const dst = O.kv16 + ((long long)tile * kExtTile + 32 * warp) * kExtRow;
+  __half* const dst = O.kv16 + (long long)t0 * kExtRow;
   constexpr int U = 4;
-#pragma unroll 1
-  for (int i = 0; i < 32; i += U) {
+#pragma unroll
+  for (int i = 0; i < kPer; i += U) {
     uint2 w[U];
     uint32_t sc[U], rp[U];
     int at[U];
@@ -279,27 +340,35 @@ __device__ __forceinline__ void ext_convert_tile(const ExtProblem& E, const ExtO
   }
 }
 
-__device__ __forceinline__ void ext_convert_rows(const ExtProblem& E, const ExtOperands& O, int item) {
+__device__ __forceinline__ void ext_convert_rows(const ExtProblem& E, const ExtOperands& O, int unit) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int item = unit / (kExtRows / kExtQRows);
+  constexpr int U = kExtQRows / (kExtPrepThreads / 32);  // rows of a warp
+  const int r0 = (unit % (kExtRows / kExtQRows)) * kExtQRows + U * warp;
   const int row0 = E.items[item].row0, rows = E.items[item].rows;
   const float ratio = O.kpe_scale / O.ckv_scale;  // rope scores in units of the latent ones
-  for (int r = warp; r < kExtRows; r += kExtPrepThreads / 32) {
-    const long long at = (long long)row0 + (r < rows ? r : rows - 1);  // (dead rows repeat the last live one and are not written out)
+  uint4 w0[U], w1[U];
+  uint32_t rp[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long at = (long long)row0 + (r0 + u < rows ? r0 + u : rows - 1);  // (dead rows repeat the last live one and are not written out)
     const uint4* src = reinterpret_cast<const uint4*>(O.q_nope + at * CKV);
-    const uint4 w0 = __ldg(src + lane), w1 = __ldg(src + 32 + lane);  // channels 8 lane .. of both halves of the row
-    const uint32_t rp = __ldg(reinterpret_cast<const uint32_t*>(O.q_pe + at * KPE) + lane);
-    const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-    const float p0 = __uint_as_float(rp << 16) * ratio, p1 = __uint_as_float(rp & 0xFFFF0000u) * ratio;
+    w0[u] = __ldg(src + lane), w1[u] = __ldg(src + 32 + lane);  // channels 8 lane .. of both halves of the row
+    rp[u] = __ldg(reinterpret_cast<const uint32_t*>(O.q_pe + at * KPE) + lane);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t w[8] = {w0[u].x, w0[u].y, w0[u].z, w0[u].w, w1[u].x, w1[u].y, w1[u].z, w1[u].w};
+    const float p0 = __uint_as_float(rp[u] << 16) * ratio, p1 = __uint_as_float(rp[u] & 0xFFFF0000u) * ratio;
     uint32_t m = max(__float_as_uint(p0) & 0x7FFFFFFFu, __float_as_uint(p1) & 0x7FFFFFFFu);  // magnitudes, ordered like integers
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, max(w[j] << 16 & 0x7FFFFFFFu, w[j] & 0x7FFF0000u));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
+    m = __reduce_max_sync(~0u, m);
     int e = int(m >> 23) - 127 - 14;  // the row is held times 2^-e
     e = e < -100 ? -100 : e > 112 ? 112 : e;
     // the sign of the softmax scale goes into the row, so that a larger product is always a larger score
     const float up = (O.sm_scale_log2 < 0.f ? -1.f : 1.f) * __uint_as_float(uint32_t(127 - e) << 23);
-    __half* const dst = O.q16 + ((long long)item * kExtRows + r) * kExtRow;
+    __half* const dst = O.q16 + ((long long)item * kExtRows + r0 + u) * kExtRow;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t o[4];
@@ -310,7 +379,7 @@ __device__ __forceinline__ void ext_convert_rows(const ExtProblem& E, const ExtO
     reinterpret_cast<uint32_t*>(dst + CKV)[lane] = ptx::f32x2_to_f16x2(p0 * up, p1 * up);
     // (never 0: a masked score is -inf and must stay so; a row with a non-finite element is NaN)
     if (lane == 0)
-      O.q_scale[(long long)item * kExtRows + r] =
+      O.q_scale[(long long)item * kExtRows + r0 + u] =
           m < 0x7F800000u ? fmaxf(fabsf(O.sm_scale_log2) * O.ckv_scale * __uint_as_float(uint32_t(127 + e) << 23), 0x1p-149f) : __uint_as_float(0x7FC00000u);
   }
 }
@@ -325,33 +394,59 @@ __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const 
     const long long row = i < front ? i : i - front + (long long)last * E.heads;
     O.out[row * (CKV / 8) + (threadIdx.x & 63)] = make_uint4(0, 0, 0, 0);
   }
-  if (int(blockIdx.x) < E.max_tiles) {
-    if (int(blockIdx.x) < E.counts[1]) ext_convert_tile(E, O, blockIdx.x);
-  } else if (int(blockIdx.x) - E.max_tiles < E.counts[0]) {
-    ext_convert_rows(E, O, int(blockIdx.x) - E.max_tiles);
+  const int tokens = E.counts[1] * (kExtTile / kExtTokens), units = tokens + E.counts[0] * (kExtRows / kExtQRows);
+  for (int i = blockIdx.x; i < units; i += gridDim.x) {
+    if (i < tokens) ext_convert_tokens(E, O, i);
+    else ext_convert_rows(E, O, i - tokens);
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // Merge of the partial results of an item that several pairs worked on: pair p holds its first tiles, the pairs behind it the rest. The
-// partials of a pair: slot 2 p + 1 an item that it began, 2 p one that another pair began.
+// partials of a pair: slot 2 p + 1 an item that it began, 2 p one that another pair began. A warp takes a row (four 16-byte loads per
+// partial and lane, all of a partial's before the first is used); rows of many partials take the whole block.
 // ---------------------------------------------------------------------------------------------------------------
-template <int GROUPS>
-__global__ void __launch_bounds__(128 * GROUPS)
-mla_extend_combine_kernel(const ExtProblem E, const float* __restrict__ lse_part, const float* __restrict__ o_part, void* out) {
+constexpr int kExtFewParts = 8;
+__global__ void __launch_bounds__(128)
+mla_extend_combine_kernel(const ExtProblem E, const float* __restrict__ lse_part, const float* __restrict__ o_part, uint2* __restrict__ out) {
   __shared__ float weights[kCombineMaxParts];
-  __shared__ float4 partial[GROUPS > 1 ? (GROUPS - 1) * 128 : 1];
   ptx::grid_dependency_wait();
-  const int p = blockIdx.x, r = blockIdx.y, item = E.pair[p].split;
-  if (item < 0) return;
-  const ExtItem& m = E.items[item];
-  if (r >= m.rows) return;
-  const int q = E.pair[1].first;  // tiles per pair (a split item has a second pair)
-  const int parts = (m.prefix + m.ntiles - 1) / q - p + 1;
-  auto slot = [&](int i) { return (long long)(i ? 2 * (p + i) : 2 * p + 1) * kExtRows + r; };
-  merge_row<GROUPS>(
-      parts, [&](int i) { return lse_part[slot(i)]; }, [&](int i) { return o_part + slot(i) * CKV; }, (long long)m.row0 + r, out, nullptr, nullptr,
-      weights, partial);
+  const int p = blockIdx.x, lane = threadIdx.x & 31;
+  const ExtPair pair = E.pair[p];
+  if (pair.split < 0) return;
+  const int row0 = E.items[pair.split].row0, rows = E.items[pair.split].rows, parts = pair.parts;
+  auto slot = [&](int i, int r) { return (long long)(i ? 2 * (p + i) : 2 * p + 1) * kExtRows + r; };
+  auto lse_of = [&](int i, int r) { return i && E.pair[p + i].count == 0 ? -INFINITY : lse_part[slot(i, r)]; };  // (a pair may have none of the rest)
+  if (parts <= kExtFewParts) {
+    const int r = 4 * blockIdx.y + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const float lse = lane < parts ? lse_of(lane, r) : -INFINITY;
+    const float M = warp_max(lse), w = lse == -INFINITY ? 0.f : exp2f(lse - M);
+    const float den = warp_sum(w);
+    float4 acc[4] = {};
+#pragma unroll 2
+    for (int i = 0; i < parts; ++i) {
+      const float wi = __shfl_sync(~0u, w, i);
+      if (wi == 0.f) continue;
+      const float4* src = reinterpret_cast<const float4*>(o_part + slot(i, r) * CKV) + lane;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 v = src[32 * j];
+        acc[j].x += wi * v.x, acc[j].y += wi * v.y, acc[j].z += wi * v.z, acc[j].w += wi * v.w;
+      }
+    }
+    const float s = den != 0.f ? 1.f / den : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      out[((long long)row0 + r) * (CKV / 4) + 32 * j + lane] = make_uint2(pack_bf16x2(acc[j].x * s, acc[j].y * s), pack_bf16x2(acc[j].z * s, acc[j].w * s));
+    return;
+  }
+  for (int r = 4 * blockIdx.y; r < 4 * int(blockIdx.y) + 4 && r < rows; ++r) {
+    merge_row<1>(
+        parts, [&](int i) { return lse_of(i, r); }, [&](int i) { return o_part + slot(i, r) * CKV; }, (long long)row0 + r, out, nullptr, nullptr,
+        weights, nullptr);
+    __syncthreads();
+  }
 }
 
 }  // namespace mla

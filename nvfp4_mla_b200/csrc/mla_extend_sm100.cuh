@@ -14,8 +14,7 @@
 // What bounds it: the tensor pipe needs 36 * 64 + 32 * 64 = 4352 cycles per tile.
 //
 // Tensor memory: O: 0..255 | S: 256..511 (two buffers of 128).
-// Shared memory: Q 72 KB | P 32 KB | ring of three 32 KB units (K: 128 tokens x 128 channels; V: 128 tokens x 128 channels) | the rope
-// part of K 16 KB.
+// Shared memory: Q 72 KB | P 32 KB | ring of seven 16 KB units (K: 128 tokens x 64 channels; V: 64 tokens x 128 channels).
 // Warp roles (384 threads): 0-7 softmax + epilogue, 8 TMA producer, 9 MMA issue (rank 0), 10 tensor memory. Every wait is bounded.
 #pragma once
 #include <cuda_fp16.h>
@@ -25,21 +24,19 @@
 namespace mla {
 
 constexpr int kExtThreads = 384;
-constexpr int kExtUnits = 3;             // ring units
-constexpr int kExtUnit = 2 * 128 * 128;  // two panels of 128 tokens x 64 channels, 128-byte swizzle
-constexpr int kExtPanel = 128 * 128;
-constexpr int kExtQPanel = 64 * 128;     // 64 rows x 64 channels
+constexpr int kExtUnits = 7;             // ring units
+constexpr int kExtPanel = 64 * 128;      // 64 rows x 64 channels, 128-byte swizzle
+constexpr int kExtUnit = 2 * kExtPanel;  // K: 128 tokens x 64 channels (token halves one behind the other); V: 64 tokens x two 64-channel panels
 
 struct ExtSmem {
-  alignas(1024) uint8_t q[9][kExtQPanel];
-  alignas(1024) uint8_t p[4][kExtQPanel];  // 64 rows x 64 tokens
+  alignas(1024) uint8_t q[9][kExtPanel];
+  alignas(1024) uint8_t p[4][kExtPanel];  // 64 rows x 64 tokens
   alignas(1024) uint8_t ring[kExtUnits][kExtUnit];
-  alignas(1024) uint8_t rope[kExtPanel];
   float xch[4][64], xl[4][64];             // maxima / sums of a row's four threads
   // in rank 0: counted by both CTAs
-  alignas(8) uint64_t full[kExtUnits], rope_full, q_full, s_free[2], p_full, o_free;
+  alignas(8) uint64_t full[kExtUnits], q_full, s_free[2], p_full, o_free;
   // in both: MMA completion
-  uint64_t empty[kExtUnits], rope_empty, q_empty, s_full[2], pv_done;
+  uint64_t empty[kExtUnits], q_empty, s_full[2], pv_done;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -50,17 +47,23 @@ struct ExtCols {
   static constexpr uint32_t O = 0, S = 256;
 };
 
-// The pair's tiles, item by item: tiles [t0, t1) of `item`. Every role walks through the same sequence.
+// The pair's tiles, item by item: tiles [t0, t1) of `item`, whole items first. Every role walks through the same sequence.
 struct ExtWalk {
   const ExtProblem& E;
-  int left, at, item;
+  int rounds, left, at, next_item, round_item, item;
   __device__ __forceinline__ ExtWalk(const ExtProblem& e, int pair) : E(e) {
     const ExtPair p = e.pair[pair];
-    left = p.count, at = p.first, item = p.item - 1;
+    rounds = p.rounds, left = p.count, at = p.first, next_item = p.item, round_item = pair, item = 0;
   }
   __device__ __forceinline__ bool next(ExtItem& m, int& t0, int& t1) {
+    if (rounds > 0) {
+      --rounds, item = round_item, round_item += E.pairs;
+      m = E.items[item];
+      t0 = 0, t1 = m.ntiles;
+      return true;
+    }
     if (left <= 0) return false;
-    ++item;
+    item = next_item++;
     m = E.items[item];
     t0 = at - m.prefix;
     t1 = m.ntiles - t0 < left ? m.ntiles : t0 + left;
@@ -86,56 +89,47 @@ struct ExtParams {
 // ---------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void ext_producer_role(ExtSmem& s, const ExtParams& P, const CUtensorMap* kv_map, const CUtensorMap* q_map, int pair,
                                                   uint32_t rank) {
-  const uint32_t ring = ptx::smem_u32(s.ring[0]), rope = ptx::smem_u32(s.rope), q = ptx::smem_u32(s.q[0]);
-  const uint32_t full0 = ptx::map_to_cta(&s.full[0], 0), rope_full = ptx::map_to_cta(&s.rope_full, 0), q_full = ptx::map_to_cta(&s.q_full, 0);
-  uint32_t unit = 0;  // ring units so far
-  auto slot_of = [&](bool& ok) {
-    const uint32_t slot = unit % kExtUnits, round = unit / kExtUnits;
-    ok = ptx::mbar_wait(&s.empty[slot], (round & 1) ^ 1, &s.abort_flag);
+  const uint32_t ring = ptx::smem_u32(s.ring[0]), q = ptx::smem_u32(s.q[0]);
+  const uint32_t full0 = ptx::map_to_cta(&s.full[0], 0), q_full = ptx::map_to_cta(&s.q_full, 0);
+  uint32_t slot = 0, phase = 1;  // of the next ring unit; parity of the wait for it to be free
+  // two boxes of 64 rows x 64 channels into the next unit
+  auto load = [&](int x0, int y0, int x1, int y1) {
+    if (!ptx::mbar_wait(&s.empty[slot], phase, &s.abort_flag)) return false;
     if (rank == 0) ptx::mbar_arrive_expect_tx(&s.full[slot], 2 * kExtUnit);
-    ++unit;
-    return slot;
+    ptx::tma_load_2d_pair(ring + slot * kExtUnit, kv_map, x0, y0, full0 + 8 * slot);
+    ptx::tma_load_2d_pair(ring + slot * kExtUnit + kExtPanel, kv_map, x1, y1, full0 + 8 * slot);
+    if (++slot == kExtUnits) slot = 0, phase ^= 1;
+    return true;
   };
-  auto load_k = [&](int row, uint32_t g) {
-    bool ok;
+  auto load_k = [&](int row) {
+    const int y = row + 128 * int(rank);
 #pragma unroll 1
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t slot = slot_of(ok);
-      if (!ok) return false;
-      ptx::tma_load_2d_pair(ring + slot * kExtUnit, kv_map, 128 * u, row + 128 * rank, full0 + 8 * slot);
-      ptx::tma_load_2d_pair(ring + slot * kExtUnit + kExtPanel, kv_map, 128 * u + 64, row + 128 * rank, full0 + 8 * slot);
-    }
-    if (!ptx::mbar_wait(&s.rope_empty, (g & 1) ^ 1, &s.abort_flag)) return false;
-    if (rank == 0) ptx::mbar_arrive_expect_tx(&s.rope_full, 2 * kExtPanel);
-    ptx::tma_load_2d_pair(rope, kv_map, CKV, row + 128 * rank, rope_full);
+    for (int u = 0; u < 9; ++u)
+      if (!load(64 * u, y, 64 * u, y + 64)) return false;
     return true;
   };
   auto load_v = [&](int row) {
-    bool ok;
 #pragma unroll 1
-    for (int u = 0; u < 4; ++u) {  // token half u / 2, channel half u % 2
-      const uint32_t slot = slot_of(ok);
-      if (!ok) return false;
-      const int x = 256 * (u & 1) + 128 * int(rank), y = row + 128 * (u >> 1);
-      ptx::tma_load_2d_pair(ring + slot * kExtUnit, kv_map, x, y, full0 + 8 * slot);
-      ptx::tma_load_2d_pair(ring + slot * kExtUnit + kExtPanel, kv_map, x + 64, y, full0 + 8 * slot);
+    for (int u = 0; u < 8; ++u) {  // 64 tokens u / 2, channel half u % 2
+      const int x = 256 * (u & 1) + 128 * int(rank), y = row + 64 * (u >> 1);
+      if (!load(x, y, x + 64, y)) return false;
     }
     return true;
   };
   ExtWalk walk(P.E, pair);
   ExtItem m;
   int t0, t1, before = -1;  // workspace row of the tile whose V is due
-  uint32_t g = 0, n_items = 0;
+  uint32_t n_items = 0;
   while (walk.next(m, t0, t1)) {
     // the query, once every QK^T of the item before has read the old one
     if (!ptx::mbar_wait(&s.q_empty, (n_items & 1) ^ 1, &s.abort_flag)) return;
-    if (rank == 0) ptx::mbar_arrive_expect_tx(&s.q_full, 2 * 9 * kExtQPanel);
+    if (rank == 0) ptx::mbar_arrive_expect_tx(&s.q_full, 2 * 9 * kExtPanel);
 #pragma unroll 1
-    for (int p = 0; p < 9; ++p) ptx::tma_load_2d_pair(q + p * kExtQPanel, q_map, 64 * p, walk.item * kExtRows + 64 * int(rank), q_full);
+    for (int p = 0; p < 9; ++p) ptx::tma_load_2d_pair(q + p * kExtPanel, q_map, 64 * p, walk.item * kExtRows + 64 * int(rank), q_full);
     ++n_items;
-    for (int t = t0; t < t1; ++t, ++g) {
+    for (int t = t0; t < t1; ++t) {
       const int row = (m.tile0 + ext_tile(m, t)) * kExtTile;
-      if (!load_k(row, g)) return;
+      if (!load_k(row)) return;
       if (before >= 0 && !load_v(before)) return;
       before = row;
     }
@@ -151,26 +145,28 @@ __device__ __forceinline__ void ext_mma_role(ExtSmem& s, const ExtParams& P, int
   const uint32_t qk_desc = ptx::instr_desc(kExtRows, kExtTile, ptx::FMT_F16, ptx::FMT_F16, false, false);
   const uint32_t pv_desc = ptx::instr_desc(kExtRows, 256, ptx::FMT_F16, ptx::FMT_F16, false, true);
   const uint64_t q_d = ptx::smem_desc_sw128(ptx::smem_u32(s.q[0]), 16, 1024), p_d = ptx::smem_desc_sw128(ptx::smem_u32(s.p[0]), 16, 1024);
-  const uint64_t k_d = ptx::smem_desc_sw128(ptx::smem_u32(s.ring[0]), 16, 1024), r_d = ptx::smem_desc_sw128(ptx::smem_u32(s.rope), 16, 1024);
+  const uint64_t k_d = ptx::smem_desc_sw128(ptx::smem_u32(s.ring[0]), 16, 1024);
   const uint64_t v_d = ptx::smem_desc_sw128(ptx::smem_u32(s.ring[0]), kExtPanel, 1024);  // channels 64 .. of the unit are a panel further
   const uint32_t hi = uint32_t(q_d >> 32), v_hi = uint32_t(v_d >> 32);
-  uint32_t unit = 0, n_items = 0;
+  uint32_t slot = 0, phase = 0, n_items = 0;
+  auto advance = [&] {
+    ptx::mma_commit_pair(&s.empty[slot]);
+    if (++slot == kExtUnits) slot = 0, phase ^= 1;
+  };
   bool first_of_item = false;
   auto pv = [&](uint32_t g, bool first, uint32_t segment) {
     if (!ptx::mbar_wait(&s.p_full, g & 1, &s.abort_flag)) return false;
     // a new item's first product overwrites O: the one before must have been read out
     if (first && segment > 0 && !ptx::mbar_wait(&s.o_free, (segment - 1) & 1, &s.abort_flag)) return false;
 #pragma unroll 1
-    for (int u = 0; u < 4; ++u, ++unit) {
-      const uint32_t slot = unit % kExtUnits;
-      if (!ptx::mbar_wait(&s.full[slot], (unit / kExtUnits) & 1, &s.abort_flag)) return false;
+    for (int u = 0; u < 8; ++u) {
+      if (!ptx::mbar_wait(&s.full[slot], phase, &s.abort_flag)) return false;
       ptx::tc_fence_after_sync();
-      const uint32_t a = uint32_t(p_d) + (u >> 1) * (2 * kExtQPanel >> 4), b = uint32_t(v_d) + slot * (kExtUnit >> 4);
+      const uint32_t a = uint32_t(p_d) + (u >> 1) * (kExtPanel >> 4), b = uint32_t(v_d) + slot * (kExtUnit >> 4);
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks)
-        ptx::mma_pair_f16_ss_lo(tm + ExtCols::O + 128 * (u & 1), a + (ks >> 2) * (kExtQPanel >> 4) + 2 * (ks & 3), b + ks * (16 * 128 >> 4), hi, v_hi, pv_desc,
-                                !first || u > 1 || ks > 0);
-      ptx::mma_commit_pair(&s.empty[slot]);
+      for (int ks = 0; ks < 4; ++ks)
+        ptx::mma_pair_f16_ss_lo(tm + ExtCols::O + 128 * (u & 1), a + 2 * ks, b + ks * (16 * 128 >> 4), hi, v_hi, pv_desc, !first || u > 1 || ks > 0);
+      advance();
     }
     ptx::mma_commit_pair(&s.pv_done);
     return true;
@@ -187,21 +183,14 @@ __device__ __forceinline__ void ext_mma_role(ExtSmem& s, const ExtParams& P, int
       ptx::tc_fence_after_sync();
       const uint32_t d = tm + ExtCols::S + 128 * (g & 1);
 #pragma unroll 1
-      for (int u = 0; u < 4; ++u, ++unit) {
-        const uint32_t slot = unit % kExtUnits;
-        if (!ptx::mbar_wait(&s.full[slot], (unit / kExtUnits) & 1, &s.abort_flag)) return;
+      for (int u = 0; u < 9; ++u) {
+        if (!ptx::mbar_wait(&s.full[slot], phase, &s.abort_flag)) return;
         ptx::tc_fence_after_sync();
-        const uint32_t a = uint32_t(q_d) + u * (2 * kExtQPanel >> 4), b = uint32_t(k_d) + slot * (kExtUnit >> 4);
+        const uint32_t a = uint32_t(q_d) + u * (kExtPanel >> 4), b = uint32_t(k_d) + slot * (kExtUnit >> 4);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-          ptx::mma_pair_f16_ss_lo(d, a + (ks >> 2) * (kExtQPanel >> 4) + 2 * (ks & 3), b + (ks >> 2) * (kExtPanel >> 4) + 2 * (ks & 3), hi, hi, qk_desc, (u | ks) != 0);
-        ptx::mma_commit_pair(&s.empty[slot]);
+        for (int ks = 0; ks < 4; ++ks) ptx::mma_pair_f16_ss_lo(d, a + 2 * ks, b + 2 * ks, hi, hi, qk_desc, (u | ks) != 0);
+        advance();
       }
-      if (!ptx::mbar_wait(&s.rope_full, g & 1, &s.abort_flag)) return;
-      ptx::tc_fence_after_sync();
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) ptx::mma_pair_f16_ss_lo(d, uint32_t(q_d) + 8 * (kExtQPanel >> 4) + 2 * ks, uint32_t(r_d) + 2 * ks, hi, hi, qk_desc, 1u);
-      ptx::mma_commit_pair(&s.rope_empty);
       ptx::mma_commit_pair(&s.s_full[g & 1]);
       if (t + 1 == t1) ptx::mma_commit_pair(&s.q_empty);
       // PV of the tile before: in this item, or the last one of the item before
@@ -390,7 +379,7 @@ mla_extend_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_const
   const uint32_t rank = ptx::cluster_ctarank();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kExtUnits; ++i) ptx::mbar_init(&s.full[i], 1), ptx::mbar_init(&s.empty[i], 1);
-    ptx::mbar_init(&s.rope_full, 1), ptx::mbar_init(&s.rope_empty, 1), ptx::mbar_init(&s.q_full, 1), ptx::mbar_init(&s.q_empty, 1);
+    ptx::mbar_init(&s.q_full, 1), ptx::mbar_init(&s.q_empty, 1);
     for (int i = 0; i < 2; ++i) ptx::mbar_init(&s.s_full[i], 1), ptx::mbar_init(&s.s_free[i], 16);
     ptx::mbar_init(&s.p_full, 16), ptx::mbar_init(&s.pv_done, 1), ptx::mbar_init(&s.o_free, 16);
     s.abort_flag = 0;

@@ -54,6 +54,10 @@ RAGGED = [
     ([90, 4000], [20, 5], 64, 1),
     ([3, 300], [5, 300], 16, 256),      # more new tokens than the cache holds: the first ones see nothing
     ([50, 0, 77], [50, 0, 0], 16, 64),  # requests without query tokens, without anything
+    ([700, 3000, 90, 1500], [600, 300, 90, 1], 32, 64),  # more row tiles than CTA pairs, of unequal length
+    ([20000], [4], 32, 64),             # one row tile for all CTA pairs
+    ([900, 5000, 3], [30, 9, 3], 8, 64), ([300], [100], 24, 16), ([2000, 40], [70, 1], 3, 64), ([500], [260], 1, 32),
+    ([400] * 70, [1, 5] * 35, 16, 64),  # many requests
 ]
 
 
