@@ -180,25 +180,36 @@ def _window_bytes(device_index, batch, heads, page_size, width, window, sink_tok
     return nbytes
 
 
+def _raw_stream(dev):
+    """The current stream's handle (without making a Stream object: these calls' host time is a good part of a small one's)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _check_page_table(page_table):
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise RuntimeError("page_table must be int32 [batch, max_pages] with contiguous rows")
+    return page_table.shape
+
+
 def _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale):
-    """What the calls below refuse of queries and tables; ``(query tokens, heads, requests)``."""
-    if q_nope.dim() != 3 or q_nope.shape[2] != CKV or q_pe.dim() != 3 or tuple(q_pe.shape) != (*q_nope.shape[:2], KPE):
+    """What the calls below refuse of queries and tables; ``(query tokens, heads, requests, page size, page-table width)``."""
+    if q_nope.dim() != 3 or q_nope.shape[2] != CKV or q_pe.shape != (q_nope.shape[0], q_nope.shape[1], KPE):
         raise RuntimeError("q_nope must be [tokens, heads, 512] and q_pe [tokens, heads, 64]")
     if q_nope.dtype != torch.bfloat16 or q_pe.dtype != torch.bfloat16:
         raise RuntimeError("q must be bfloat16")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise RuntimeError("page_table must be int32 [batch, max_pages] with contiguous rows")
-    B = page_table.shape[0]
-    if kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (B,):
+    B, width = _check_page_table(page_table)
+    if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,):
         raise RuntimeError("kv_lens must be int32 [batch]")
-    for t in (q_nope, q_pe, page_table, kv_lens):
-        if t.device != ckv_cache.device or (t is not page_table and not t.is_contiguous()):
-            raise RuntimeError("inputs must be contiguous and on the cache device")
+    at = ckv_cache.get_device()
+    if (q_nope.get_device() != at or q_pe.get_device() != at or page_table.get_device() != at or kv_lens.get_device() != at
+            or not (q_nope.is_contiguous() and q_pe.is_contiguous() and kv_lens.is_contiguous())):
+        raise RuntimeError("inputs must be contiguous and on the cache device")
     if not (ckv_scale > 0 and kpe_scale > 0):
         raise RuntimeError("ckv_scale and kpe_scale must be positive")
-    if ckv_cache.shape[1] & (ckv_cache.shape[1] - 1):
+    ps = ckv_cache.shape[1]
+    if ps & (ps - 1):
         raise RuntimeError("page_size must be a power of two")
-    return (*q_nope.shape[:2], B)
+    return q_nope.shape[0], q_nope.shape[1], B, ps, width
 
 
 def _check_window(window, sink_tokens):
@@ -220,12 +231,12 @@ def decode_window(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, 
     reports bad pages."""
     window, sink_tokens = _check_window(window, sink_tokens)
     _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
-    N, H, B = _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale)
+    N, H, B, ps, width = _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale)
     if N != B:
         raise RuntimeError("q_nope must be [batch, heads, 512]")
     if H == 0 or H % 16 != 0:
         raise RuntimeError("heads must be a multiple of 16")
-    dev, ps, width = ckv_cache.device, ckv_cache.shape[1], page_table.shape[1]
+    dev = ckv_cache.device
     bound = min(width * ps, 2 ** 31 - 1)
     max_kv_len = bound if max_kv_len is None else min(int(max_kv_len), bound)
 
@@ -236,7 +247,7 @@ def decode_window(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, 
             q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), ckv_cache.shape[0], ps,
             page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), B, H, float(sm_scale), float(ckv_scale), float(kpe_scale),
             max_kv_len, window, sink_tokens, out.data_ptr(), None, None, ws.data_ptr(), ws.numel(), _ptr(_status(dev)),
-            torch.cuda.current_stream(dev).cuda_stream))
+            _raw_stream(dev)))
         return out
 
     return _on_device(dev, launch)
@@ -271,12 +282,12 @@ def extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens
     """
     window, sink_tokens = _check_window(window, sink_tokens) if window else (0, _check_window(1, sink_tokens)[1])
     _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
-    N, H, B = _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale)
-    if qo_indptr.dtype != torch.int32 or tuple(qo_indptr.shape) != (B + 1,) or not qo_indptr.is_contiguous() or qo_indptr.device != ckv_cache.device:
+    N, H, B, ps, width = _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale)
+    if qo_indptr.dtype != torch.int32 or qo_indptr.shape != (B + 1,) or not qo_indptr.is_contiguous() or qo_indptr.get_device() != ckv_cache.get_device():
         raise RuntimeError("qo_indptr must be a contiguous int32 [batch + 1] tensor on the cache device")
     if H == 0:
         raise RuntimeError("heads must be positive")
-    dev, ps, width = ckv_cache.device, ckv_cache.shape[1], page_table.shape[1]
+    dev = ckv_cache.device
     bound = min(width * ps, 2 ** 31 - 1)
     max_kv_len = bound if max_kv_len is None else min(int(max_kv_len), bound)
 
@@ -287,7 +298,7 @@ def extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens
             q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), ckv_cache.shape[0], ps,
             page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), qo_indptr.data_ptr(), B, N, H, float(sm_scale),
             float(ckv_scale), float(kpe_scale), max_kv_len, window, sink_tokens, out.data_ptr(), ws.data_ptr(), ws.numel(),
-            _ptr(_status(dev)), torch.cuda.current_stream(dev).cuda_stream))
+            _ptr(_status(dev)), _raw_stream(dev)))
         return out
 
     return _on_device(dev, launch)
@@ -489,28 +500,32 @@ def norm_rope_append_paged_mla_kv_cache(ckv, kpe, norm_weight, cos_sin, batch_in
     if ckv.dtype != torch.bfloat16 or kpe.dtype != torch.bfloat16 or norm_weight.dtype != torch.bfloat16 or cos_sin.dtype != torch.float32:
         raise RuntimeError("ckv, kpe and norm_weight must be bfloat16 and cos_sin float32")
     nnz = ckv.shape[0]
-    if tuple(ckv.shape) != (nnz, CKV) or tuple(kpe.shape) != (nnz, KPE):
+    if ckv.shape != (nnz, CKV) or kpe.shape != (nnz, KPE):
         raise RuntimeError("ckv must be [nnz, 512] and kpe [nnz, 64]")
-    strides = tuple(t.stride(0) if nnz > 1 else t.shape[1] for t in (ckv, kpe))  # (a single row has no stride to speak of)
-    if ckv.stride(1) != 1 or kpe.stride(1) != 1 or strides[0] < CKV or strides[0] % 8 or strides[1] < KPE or strides[1] % 2:
+    (rows, inner), (pe_rows, pe_inner) = ckv.stride(), kpe.stride()
+    if nnz <= 1:  # (a single row has no stride to speak of)
+        rows, pe_rows = CKV, KPE
+    if inner != 1 or pe_inner != 1 or rows < CKV or rows % 8 or pe_rows < KPE or pe_rows % 2:
         raise RuntimeError("rows of ckv and kpe must be contiguous, their strides multiples of 8 and 2 elements")
-    if tuple(norm_weight.shape) != (CKV,) or cos_sin.dim() != 2 or cos_sin.shape[1] != KPE or not (norm_weight.is_contiguous() and cos_sin.is_contiguous()):
+    if norm_weight.shape != (CKV,) or cos_sin.dim() != 2 or cos_sin.shape[1] != KPE or not (norm_weight.is_contiguous() and cos_sin.is_contiguous()):
         raise RuntimeError("norm_weight must be a contiguous [512] and cos_sin a contiguous [positions, 64] tensor")
-    for name, t, n in (("batch_indices", batch_indices, nnz), ("positions", positions, nnz), ("kv_indices", kv_indices, None),
-                       ("kv_indptr", kv_indptr, None)):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
-            raise RuntimeError(f"{name} must be a contiguous 1-D int32 tensor" + (f" of {n} elements" if n is not None else ""))
-    dev = ckv_cache.device
-    if any(t.device != dev for t in (ckv, kpe, norm_weight, cos_sin, batch_indices, positions, kv_indices, kv_indptr)):
+    if batch_indices.dtype != torch.int32 or positions.dtype != torch.int32 or kv_indices.dtype != torch.int32 or kv_indptr.dtype != torch.int32:
+        raise RuntimeError("batch_indices, positions, kv_indices and kv_indptr must be int32")
+    if (batch_indices.shape != (nnz,) or positions.shape != (nnz,) or kv_indices.dim() != 1 or kv_indptr.dim() != 1
+            or not (batch_indices.is_contiguous() and positions.is_contiguous() and kv_indices.is_contiguous() and kv_indptr.is_contiguous())):
+        raise RuntimeError(f"batch_indices and positions must be contiguous [{nnz}], kv_indices and kv_indptr contiguous 1-D tensors")
+    dev, at = ckv_cache.device, ckv_cache.get_device()
+    if (ckv.get_device() != at or kpe.get_device() != at or norm_weight.get_device() != at or cos_sin.get_device() != at
+            or batch_indices.get_device() != at or positions.get_device() != at or kv_indices.get_device() != at or kv_indptr.get_device() != at):
         raise RuntimeError("inputs must be on the cache device")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    pages, ps = ckv_cache.shape[:2]
     _on_device(dev, lambda: _lib.check(_lib.load().nvfp4_mla_norm_rope_append(
-        _ptr(ckv), strides[0], _ptr(kpe), strides[1], _ptr(norm_weight), _ptr(cos_sin), cos_sin.shape[0], float(eps), int(bool(interleaved)),
-        _ptr(batch_indices), _ptr(positions), nnz, _ptr(ckv_cache), _ptr(ckv_sf_cache), _ptr(kpe_cache), *ckv_cache.shape[:2],
-        _ptr(kv_indices), _ptr(kv_indptr), kv_indptr.numel() - 1, float(ckv_scale), float(kpe_scale), _ptr(status),
-        torch.cuda.current_stream(dev).cuda_stream)))
+        ckv.data_ptr(), rows, kpe.data_ptr(), pe_rows, norm_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], eps, 1 if interleaved else 0,
+        batch_indices.data_ptr(), positions.data_ptr(), nnz, ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), pages, ps,
+        kv_indices.data_ptr(), kv_indptr.data_ptr(), kv_indptr.shape[0] - 1, ckv_scale, kpe_scale, _ptr(status), _raw_stream(dev))))
     if check and int(status.item()) != 0:
         raise RuntimeError("norm_rope_append: a token named a request, position or page outside the tables")
 
@@ -528,32 +543,32 @@ def gather_paged_mla_kv_cache(ckv_cache, ckv_sf_cache, kpe_cache, page_table, in
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"dtype must be bfloat16 or float32, got {dtype}")
     _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
-    dev = ckv_cache.device
+    dev, at = ckv_cache.device, ckv_cache.get_device()
     total = operator.index(total)
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise RuntimeError("page_table must be int32 [batch, max_pages] with contiguous rows")
-    B = page_table.shape[0]
-    if indptr.dtype != torch.int32 or tuple(indptr.shape) != (B + 1,) or not indptr.is_contiguous():
+    B, width = _check_page_table(page_table)
+    if indptr.dtype != torch.int32 or indptr.shape != (B + 1,) or not indptr.is_contiguous():
         raise RuntimeError("indptr must be a contiguous int32 [batch + 1] tensor")
-    if starts is not None and (starts.dtype != torch.int32 or tuple(starts.shape) != (B,) or not starts.is_contiguous()):
+    if starts is not None and (starts.dtype != torch.int32 or starts.shape != (B,) or not starts.is_contiguous()):
         raise RuntimeError("starts must be a contiguous int32 [batch] tensor")
-    if any(t is not None and t.device != dev for t in (page_table, indptr, starts)):
+    if page_table.get_device() != at or indptr.get_device() != at or (starts is not None and starts.get_device() != at):
         raise RuntimeError("inputs must be on the cache device")
     if total < 0:
         raise ValueError("total must not be negative")
     if not (ckv_scale > 0 and kpe_scale > 0):
         raise RuntimeError("ckv_scale and kpe_scale must be positive")
     if out is None:
-        out = torch.empty(total, CKV, dtype=dtype, device=dev), torch.empty(total, KPE, dtype=dtype, device=dev)
-    ckv, kpe = out
-    if not (ckv.dtype == kpe.dtype == dtype and tuple(ckv.shape) == (total, CKV) and tuple(kpe.shape) == (total, KPE)
-            and ckv.is_contiguous() and kpe.is_contiguous() and ckv.device == dev and kpe.device == dev):
-        raise RuntimeError("out must be contiguous ([total, 512], [total, 64]) tensors of dtype on the cache device")
+        ckv, kpe = torch.empty(total, CKV, dtype=dtype, device=dev), torch.empty(total, KPE, dtype=dtype, device=dev)
+    else:
+        ckv, kpe = out
+        if not (ckv.dtype == kpe.dtype == dtype and ckv.shape == (total, CKV) and kpe.shape == (total, KPE)
+                and ckv.is_contiguous() and kpe.is_contiguous() and ckv.get_device() == at and kpe.get_device() == at):
+            raise RuntimeError("out must be contiguous ([total, 512], [total, 64]) tensors of dtype on the cache device")
     status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    pages, ps = ckv_cache.shape[:2]
     _on_device(dev, lambda: _lib.check(_lib.load().nvfp4_mla_gather(
-        _ptr(ckv_cache), _ptr(ckv_sf_cache), _ptr(kpe_cache), *ckv_cache.shape[:2], _ptr(page_table), page_table.stride(0),
-        page_table.shape[1], _ptr(indptr), _ptr(starts), B, total, float(ckv_scale), float(kpe_scale), int(dtype == torch.bfloat16),
-        _ptr(ckv), _ptr(kpe), _ptr(status), torch.cuda.current_stream(dev).cuda_stream)))
+        ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), pages, ps, page_table.data_ptr(), page_table.stride(0), width,
+        indptr.data_ptr(), _ptr(starts), B, total, ckv_scale, kpe_scale, 1 if dtype == torch.bfloat16 else 0, ckv.data_ptr(), kpe.data_ptr(),
+        _ptr(status), _raw_stream(dev))))
     if check and int(status.item()) != 0:
         raise RuntimeError("gather: a token lies outside the page table or on a page outside the cache")
     return ckv, kpe
