@@ -173,8 +173,8 @@ def _status(dev):
 
 
 @functools.lru_cache(maxsize=4096)
-def _window_bytes(device_index, batch, heads, page_size, width, window, sink_tokens):
-    nbytes = _lib.load().nvfp4_mla_decode_window_workspace_bytes(batch, heads, page_size, width, window, sink_tokens)
+def _window_bytes(device_index, *sizes):
+    nbytes = _lib.load().nvfp4_mla_decode_window_workspace_bytes(*sizes)
     if nbytes < 0:
         raise RuntimeError(_lib.load().nvfp4_mla_last_error().decode())
     return nbytes
@@ -242,7 +242,7 @@ def decode_window(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, 
 
     def launch():
         out = torch.empty(B, H, CKV, dtype=torch.bfloat16, device=dev)
-        ws = torch.empty(_window_bytes(dev.index, B, H, ps, width, window, sink_tokens), dtype=torch.uint8, device=dev)
+        ws = torch.empty(_window_bytes(dev.index, B, H, ps, width, max_kv_len, window, sink_tokens), dtype=torch.uint8, device=dev)
         _lib.check(_lib.load().nvfp4_mla_decode_window(
             q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), ckv_cache.shape[0], ps,
             page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), B, H, float(sm_scale), float(ckv_scale), float(kpe_scale),

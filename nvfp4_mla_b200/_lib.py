@@ -23,10 +23,10 @@ SIGNATURES = {
     "nvfp4_mla_decode_multi_folds": (_i32, [_i32, _i32, _i32, _i32, _i32]),
     "nvfp4_mla_decode_multi": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _i32, _f32, _f32, _f32,
                                       _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
-    "nvfp4_mla_decode_window_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "nvfp4_mla_decode_window_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "nvfp4_mla_decode_window": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i32, _f32, _f32, _f32, _i32, _i32, _i32,
                                        _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
-    "nvfp4_mla_extend_shares": (_i32, [_i32, _i32, _i32]),
+    "nvfp4_mla_extend_shares": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "nvfp4_mla_extend_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "nvfp4_mla_extend": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _f32, _f32, _i32, _i32,
                                 _i32, _vp, _vp, _i64, _vp, _vp]),

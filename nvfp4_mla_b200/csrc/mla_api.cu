@@ -1,5 +1,6 @@
 // C ABI of libnvfp4_mla_b200.so: argument validation, the TMA descriptor of the cache, and kernel launches.
 // Declarations and their documentation: include/nvfp4_mla_b200.h.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdarg>
@@ -489,42 +490,6 @@ int window_layout(int batch, int heads, int page_size, int page_table_width, int
 }
 }  // namespace
 
-int64_t nvfp4_mla_decode_window_workspace_bytes(int batch, int heads, int page_size, int page_table_width, int window, int sink_tokens) {
-  g_error[0] = 0;
-  WindowLayout l;
-  if (window <= 0) return fail("window must be positive, got %d", window), -1;
-  return window_layout(batch, heads, page_size, page_table_width, 0, window, sink_tokens, &l) ? -1 : int64_t(l.total);
-}
-
-int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
-                            const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table,
-                            int64_t page_table_stride, int page_table_width, const int32_t* kv_lens, int batch, int heads, float sm_scale,
-                            float ckv_scale, float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, float* out_f32,
-                            float* lse, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
-  g_error[0] = 0;
-  WindowLayout l;
-  MLA_CHECK(window > 0, "window must be positive, got %d", window);
-  if (window_layout(batch, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)) return 1;
-  if (batch == 0) return 0;
-  MLA_CHECK((page_table || page_table_width == 0) && kv_lens && workspace, "null pointer argument");
-  MLA_CHECK(page_table_stride >= 0, "page_table_stride must be non-negative");
-  MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes,
-            (long long)l.total);
-  MLA_CHECK(aligned(workspace, 256), "workspace must be 256-byte aligned");
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  int* table = reinterpret_cast<int*>(ws + l.table);
-  int* lens = reinterpret_cast<int*>(ws + l.lens);
-  int2* dead = reinterpret_cast<int2*>(ws + l.dead);
-  constexpr int per_block = mla::kWindowThreads / 32;
-  mla::mla_window_plan_kernel<<<unsigned((batch + per_block - 1) / per_block), mla::kWindowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      page_table, page_table_stride, page_table_width, kv_lens, mla::ChunkTokens{nullptr, batch, 0}, batch, __builtin_ctz(unsigned(page_size)),
-      window, sink_tokens, l.width, table, lens, dead);
-  MLA_CUDA(cudaGetLastError());
-  return decode_impl(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, table, l.width, lens, batch, heads, sm_scale,
-                     ckv_scale, kpe_scale, l.max_len, 0, NVFP4_MLA_PRECISION_BF16, out, out_f32, lse, workspace, int64_t(l.table), stream, 128,
-                     1, 0, dead, status);
-}
-
 // ---- chunks of new tokens ------------------------------------------------------------------------------------------
 // Two forms. A few query tokens run as requests of their own through the windowed decode, which reads the cache once per token
 // (the later reads are L2 hits). Longer chunks dequantise every visible token once and share it among all rows of a request.
@@ -533,18 +498,28 @@ constexpr int kExtendSlice = 512;  // query tokens at a time in the first form (
 
 struct ExtendLayout {
   size_t counts, req_tile0, req_map, items, pair, q_scale, lse_part, o_part, q16, kv16, total;
+  int group;  // requests at a time
   int pairs, max_items, max_tiles;
 };
+// The dequantised tokens of as many requests at a time as fit this (one at least): a bound far above the lengths must not ask for
+// more memory than there is. 7 million tokens.
+constexpr int64_t kExtTokenBytes = int64_t(8) << 30;
 int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window, int sinks, const DeviceInfo& d, ExtendLayout* l) {
   MLA_CHECK(batch <= mla::kExtMaxBatch, "at most %d requests, got %d", mla::kExtMaxBatch, batch);
   MLA_CHECK(int64_t(total_q) * heads < (int64_t(1) << 31) - mla::kExtRows, "total_q * heads must be below 2^31");
-  const int64_t requests = batch < total_q ? batch : total_q;  // with query tokens
   const int64_t len = max_kv_len > 1 ? max_kv_len : 1;
-  int64_t tiles = requests * ((len - 1) / mla::kExtTile + 1);
-  if (window > 0) {
-    const int64_t seen = requests * ((int64_t(sinks) + mla::kExtTile - 1) / mla::kExtTile + window / mla::kExtTile + 3) + total_q / mla::kExtTile;
-    if (seen < tiles) tiles = seen;
-  }
+  auto tiles_of = [&](int64_t requests) {
+    int64_t tiles = requests * ((len - 1) / mla::kExtTile + 1);
+    if (window > 0) {
+      const int64_t seen = requests * ((int64_t(sinks) + mla::kExtTile - 1) / mla::kExtTile + window / mla::kExtTile + 3) + total_q / mla::kExtTile;
+      if (seen < tiles) tiles = seen;
+    }
+    return tiles;
+  };
+  constexpr int64_t tile_bytes = int64_t(mla::kExtTile) * mla::kExtRow * 2;
+  l->group = batch;
+  while (l->group > 1 && tiles_of(std::min(l->group, total_q)) * tile_bytes > kExtTokenBytes) l->group = (l->group + 1) / 2;
+  const int64_t requests = std::min(l->group, total_q), tiles = tiles_of(requests);  // (at most total_q requests have query tokens)
   const int64_t items = requests + int64_t(total_q) * heads / mla::kExtRows;
   MLA_CHECK(tiles * mla::kExtTile < (int64_t(1) << 31) && tiles + items < (int64_t(1) << 31) && items * ((len - 1) / mla::kExtTile + 1) < (int64_t(1) << 31),
             "chunks of %d query tokens over %d requests of up to %lld tokens are too large for one call", total_q, batch, (long long)len);
@@ -555,7 +530,7 @@ int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window,
     off = mla::align_up(off + bytes, 256);
     return at;
   };
-  l->counts = take(64), l->req_tile0 = take(size_t(batch + 1) * 4), l->req_map = take(size_t(batch) * 16);
+  l->counts = take(64), l->req_tile0 = take(size_t(l->group + 1) * 4), l->req_map = take(size_t(l->group) * 16);
   l->items = take(size_t(items) * sizeof(mla::ExtItem)), l->pair = take(size_t(l->pairs) * sizeof(mla::ExtPair));
   l->q_scale = take(size_t(items) * mla::kExtRows * 4);
   l->lse_part = take(size_t(l->pairs) * 2 * mla::kExtRows * 4), l->o_part = take(size_t(l->pairs) * 2 * mla::kExtRows * mla::CKV * 4);
@@ -579,10 +554,72 @@ int make_half_map(const void* base, int64_t rows, CUtensorMap* map) {
   return 0;
 }
 
-bool extend_shares(int batch, int total_q, int heads, const DeviceInfo& d) {
-  if (d.ext_pairs < 2) return false;
+// Which of the two forms: cost estimates in us, fitted to 158 sizes (16 to 128 heads, 1 to 64 requests, 1 to 8 query tokens each, 200
+// to 16000 tokens).
+//   by token: those of the decode kernels (wants_hm16), every query token a request
+//   shared  : 21 + 0.3 per thousand dequantised tokens + 4.2 per 256-token tile of the fullest pair + 0.2 per thousand rows
+// Measured (by token / shared), heads, requests, query tokens, tokens: 16,1,1,1000: 20 / 26; 16,64,1,4000: 61 / 180; 16,4,8,16000: 78 / 73;
+// 16,64,8,1000: 114 / 59; 32,16,4,4000: 84 / 59; 64,16,8,4000: 240 / 108; 128,16,1,4000: 61 / 59; 128,16,1,16000: 134 / 177;
+// 128,64,1,200: 47 / 30; 128,64,4,4000: 508 / 331.
+bool extend_shares(int batch, int total_q, int heads, int max_kv_len, int window, int sinks, const DeviceInfo& d) {
+  if (d.ext_pairs < 2 || batch <= 0 || total_q <= 0) return false;
   if (heads % 16 != 0) return true;
-  return total_q > 2 * batch;
+  const double requests = batch < total_q ? batch : total_q, q = total_q / requests;
+  double len = max_kv_len > 1 ? max_kv_len : 1, held = len;  // tokens that a query sees; tokens of a request that are dequantised
+  if (window > 0) {
+    len = std::min(len, double(window) + sinks), held = std::min(held, double(window) + sinks + q);
+  }
+  const int groups16 = heads / 16, groups = (heads + mla::kH16Rows - 1) / mla::kH16Rows;
+  const double tiles = total_q * ceil(len / mla::TILE), sms = d.sm_count, pairs = d.sm_count / 2;
+  const double by16 = 20. + 2.4 * ceil(tiles * groups16 / sms) + 9. * total_q * groups16 / sms;
+  const double as_m = heads < kHm16MinHeads ? by16 : 42. + 3.6 * ceil(tiles * groups / pairs) + 8.4 * total_q * groups / pairs;
+  const double rows = double(total_q) * heads, items = requests * ceil(rows / requests / mla::kExtRows);
+  const double shared = 21. + 0.3e-3 * requests * held + 4.2 * ceil(items * ceil(len / mla::kExtTile) / d.ext_pairs) + 0.2e-3 * rows;
+  return shared < std::min(by16, as_m);
+}
+
+// the second form
+int extend_shared(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, const uint8_t* kpe_cache,
+                  int64_t num_pages, int page_size, const int32_t* page_table, int64_t page_table_stride, int page_table_width,
+                  const int32_t* kv_lens, const int32_t* qo_indptr, int batch, int total_q, int heads, float sm_scale, float ckv_scale,
+                  float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, uint8_t* ws, const ExtendLayout& l, const DeviceInfo& d,
+                  int32_t* status, cudaStream_t st) {
+  CUtensorMap kv_map, q_map;
+  if (make_half_map(ws + l.kv16, int64_t(l.max_tiles) * mla::kExtTile, &kv_map)) return 1;
+  if (make_half_map(ws + l.q16, int64_t(l.max_items) * mla::kExtRows, &q_map)) return 1;
+
+  mla::ExtProblem E;
+  E.total_q = total_q, E.heads = heads, E.max_kv_len = max_kv_len;
+  E.window = window, E.sinks = sink_tokens, E.pairs = l.pairs, E.max_items = l.max_items, E.max_tiles = l.max_tiles;
+  E.req_tile0 = reinterpret_cast<int*>(ws + l.req_tile0);
+  E.req_map = reinterpret_cast<int4*>(ws + l.req_map), E.items = reinterpret_cast<mla::ExtItem*>(ws + l.items);
+  E.pair = reinterpret_cast<mla::ExtPair*>(ws + l.pair), E.counts = reinterpret_cast<int*>(ws + l.counts), E.status = status;
+  mla::ExtOperands O;
+  O.q_nope = static_cast<const __nv_bfloat16*>(q_nope), O.q_pe = static_cast<const __nv_bfloat16*>(q_pe), O.ckv = ckv_cache, O.sf = ckv_sf_cache;
+  O.kpe = kpe_cache, O.pt_stride = page_table_stride, O.pt_width = page_table_width;
+  O.page_shift = __builtin_ctz(unsigned(page_size)), O.num_pages = int(num_pages), O.ckv_scale = ckv_scale, O.kpe_scale = kpe_scale;
+  O.sm_scale_log2 = sm_scale * 1.4426950408889634f, O.kv16 = reinterpret_cast<__half*>(ws + l.kv16), O.q16 = reinterpret_cast<__half*>(ws + l.q16);
+  O.q_scale = reinterpret_cast<float*>(ws + l.q_scale), O.out = static_cast<uint4*>(out);
+  mla::ExtParams P;
+  P.q_scale = O.q_scale, P.ckv_scale = ckv_scale, P.lse_part = reinterpret_cast<float*>(ws + l.lse_part);
+  P.o_part = reinterpret_cast<float*>(ws + l.o_part), P.out = static_cast<uint16_t*>(out), P.status = status;
+  const int64_t units = int64_t(l.max_tiles) * (mla::kExtTile / mla::kExtTokens) + int64_t(l.max_items) * (mla::kExtRows / mla::kExtQRows);
+  const int64_t resident = int64_t(d.sm_count) * (2048 / mla::kExtPrepThreads);
+  for (int b = 0; b < batch; b += l.group) {
+    E.batch = batch - b < l.group ? batch - b : l.group;
+    E.kv_lens = kv_lens + b, E.indptr = qo_indptr ? qo_indptr + b : nullptr, E.first_q = qo_indptr ? 0 : b;
+    E.edges = (b == 0 ? 1 : 0) | (b + l.group >= batch ? 2 : 0);
+    O.page_table = page_table + b * page_table_stride;
+    P.E = E;
+    mla::mla_extend_schedule_kernel<<<1, mla::kExtSchedThreads, 0, st>>>(E);
+    MLA_CUDA(cudaGetLastError());
+    MLA_CUDA(launch_dependent(mla::mla_extend_prep_kernel, dim3(unsigned(units < resident ? units : resident)), dim3(mla::kExtPrepThreads), 0, st, E, O));
+    MLA_CUDA(launch_dependent_cluster(mla::mla_extend_kernel, dim3(unsigned(2 * l.pairs)), dim3(mla::kExtThreads), mla::ext_smem_bytes(), st, 2u,
+                                      kv_map, q_map, P));
+    MLA_CUDA(launch_dependent(mla::mla_extend_combine_kernel, dim3(unsigned(l.pairs), mla::kExtRows / 4), dim3(128), 0, st, E,
+                              static_cast<const float*>(P.lse_part), static_cast<const float*>(P.o_part), static_cast<uint2*>(out)));
+  }
+  return 0;
 }
 
 int extend_by_token(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, const uint8_t* kpe_cache,
@@ -610,11 +647,11 @@ int extend_by_token(const void* q_nope, const void* q_pe, const uint8_t* ckv_cac
 }
 }  // namespace
 
-int nvfp4_mla_extend_shares(int batch, int total_q, int heads) {
+int nvfp4_mla_extend_shares(int batch, int total_q, int heads, int max_kv_len, int window, int sink_tokens) {
   g_error[0] = 0;
   DeviceInfo* d;
   if (device_info(&d)) return -1;
-  return extend_shares(batch, total_q, heads, *d) ? 1 : 0;
+  return extend_shares(batch, total_q, heads, max_kv_len, window, sink_tokens, *d) ? 1 : 0;
 }
 
 // what both functions below check first
@@ -633,7 +670,7 @@ int64_t nvfp4_mla_extend_workspace_bytes(int batch, int total_q, int heads, int 
   if (total_q == 0 || batch == 0) return 0;
   DeviceInfo* d;
   if (device_info(&d)) return -1;
-  if (extend_shares(batch, total_q, heads, *d)) {
+  if (extend_shares(batch, total_q, heads, max_kv_len, window, sink_tokens, *d)) {
     ExtendLayout l;
     return extend_layout(batch, total_q, heads, max_kv_len, window, sink_tokens, *d, &l) ? -1 : int64_t(l.total);
   }
@@ -655,7 +692,7 @@ int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_ca
   MLA_CHECK(page_table_stride >= 0, "page_table_stride must be non-negative");
   if (total_q == 0) return 0;
   MLA_CHECK(batch > 0, "query tokens without requests");
-  MLA_CHECK(q_nope && q_pe && ckv_cache && ckv_sf_cache && kpe_cache && (page_table || page_table_width == 0) && kv_lens && qo_indptr && out && workspace,
+  MLA_CHECK(q_nope && q_pe && ckv_cache && ckv_sf_cache && kpe_cache && (page_table || page_table_width == 0) && kv_lens && out && workspace && (qo_indptr || total_q == batch),
             "null pointer argument");
   MLA_CHECK(aligned(q_nope, 16) && aligned(q_pe, 16) && aligned(ckv_cache, 16) && aligned(ckv_sf_cache, 16) && aligned(kpe_cache, 16) &&
                 aligned(workspace, 256) && aligned(out, 16),
@@ -663,7 +700,7 @@ int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_ca
   DeviceInfo* d;
   if (device_info(&d)) return 1;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (!extend_shares(batch, total_q, heads, *d)) {
+  if (!extend_shares(batch, total_q, heads, max_kv_len, window, sink_tokens, *d)) {
     WindowLayout l;
     if (window_layout(total_q < kExtendSlice ? total_q : kExtendSlice, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)) return 1;
     MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes, (long long)l.total);
@@ -673,36 +710,58 @@ int nvfp4_mla_extend(const void* q_nope, const void* q_pe, const uint8_t* ckv_ca
   ExtendLayout l;
   if (extend_layout(batch, total_q, heads, max_kv_len, window, sink_tokens, *d, &l)) return 1;
   MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes, (long long)l.total);
-  CUtensorMap kv_map, q_map;
-  if (make_half_map(ws + l.kv16, int64_t(l.max_tiles) * mla::kExtTile, &kv_map)) return 1;
-  if (make_half_map(ws + l.q16, int64_t(l.max_items) * mla::kExtRows, &q_map)) return 1;
+  return extend_shared(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, page_table, page_table_stride, page_table_width, kv_lens,
+                       qo_indptr, batch, total_q, heads, sm_scale, ckv_scale, kpe_scale, max_kv_len, window, sink_tokens, out, ws, l, *d, status,
+                       static_cast<cudaStream_t>(stream));
+}
 
-  mla::ExtProblem E;
-  E.kv_lens = kv_lens, E.indptr = qo_indptr, E.batch = batch, E.total_q = total_q, E.heads = heads, E.max_kv_len = max_kv_len;
-  E.window = window, E.sinks = sink_tokens, E.pairs = l.pairs, E.max_items = l.max_items, E.max_tiles = l.max_tiles;
-  E.req_tile0 = reinterpret_cast<int*>(ws + l.req_tile0);
-  E.req_map = reinterpret_cast<int4*>(ws + l.req_map), E.items = reinterpret_cast<mla::ExtItem*>(ws + l.items);
-  E.pair = reinterpret_cast<mla::ExtPair*>(ws + l.pair), E.counts = reinterpret_cast<int*>(ws + l.counts), E.status = status;
-  mla::ExtOperands O;
-  O.q_nope = static_cast<const __nv_bfloat16*>(q_nope), O.q_pe = static_cast<const __nv_bfloat16*>(q_pe), O.ckv = ckv_cache, O.sf = ckv_sf_cache;
-  O.kpe = kpe_cache, O.page_table = page_table, O.pt_stride = page_table_stride, O.pt_width = page_table_width;
-  O.page_shift = __builtin_ctz(unsigned(page_size)), O.num_pages = int(num_pages), O.ckv_scale = ckv_scale, O.kpe_scale = kpe_scale;
-  O.sm_scale_log2 = sm_scale * 1.4426950408889634f, O.kv16 = reinterpret_cast<__half*>(ws + l.kv16), O.q16 = reinterpret_cast<__half*>(ws + l.q16);
-  O.q_scale = reinterpret_cast<float*>(ws + l.q_scale), O.out = static_cast<uint4*>(out);
-  mla::ExtParams P;
-  P.E = E, P.q_scale = O.q_scale, P.ckv_scale = ckv_scale, P.lse_part = reinterpret_cast<float*>(ws + l.lse_part);
-  P.o_part = reinterpret_cast<float*>(ws + l.o_part), P.out = static_cast<uint16_t*>(out), P.status = status;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  mla::mla_extend_schedule_kernel<<<1, mla::kExtSchedThreads, 0, st>>>(E);
+int64_t nvfp4_mla_decode_window_workspace_bytes(int batch, int heads, int page_size, int page_table_width, int max_kv_len, int window,
+                                                int sink_tokens) {
+  g_error[0] = 0;
+  WindowLayout l;
+  if (window <= 0) return fail("window must be positive, got %d", window), -1;
+  if (window_layout(batch, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)) return -1;
+  DeviceInfo* d;
+  if (device_info(&d)) return -1;
+  if (!extend_shares(batch, batch, heads, max_kv_len, window, sink_tokens, *d)) return int64_t(l.total);
+  ExtendLayout e;  // (the call takes the other form where more than the BF16 output is asked for)
+  if (extend_layout(batch, batch, heads, max_kv_len, window, sink_tokens, *d, &e)) return -1;
+  return int64_t(std::max(l.total, e.total));
+}
+
+int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
+                            const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table,
+                            int64_t page_table_stride, int page_table_width, const int32_t* kv_lens, int batch, int heads, float sm_scale,
+                            float ckv_scale, float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, float* out_f32,
+                            float* lse, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  g_error[0] = 0;
+  WindowLayout l;
+  MLA_CHECK(window > 0, "window must be positive, got %d", window);
+  if (window_layout(batch, heads, page_size, page_table_width, max_kv_len, window, sink_tokens, &l)) return 1;
+  if (batch == 0) return 0;
+  MLA_CHECK((page_table || page_table_width == 0) && kv_lens && workspace, "null pointer argument");
+  MLA_CHECK(page_table_stride >= 0, "page_table_stride must be non-negative");
+  MLA_CHECK(workspace_bytes >= int64_t(l.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes,
+            (long long)l.total);
+  MLA_CHECK(aligned(workspace, 256), "workspace must be 256-byte aligned");
+  DeviceInfo* d;
+  if (device_info(&d)) return 1;
+  if (out && !out_f32 && !lse && extend_shares(batch, batch, heads, max_kv_len, window, sink_tokens, *d))
+    return nvfp4_mla_extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, page_table, page_table_stride, page_table_width,
+                            kv_lens, nullptr, batch, batch, heads, sm_scale, ckv_scale, kpe_scale, max_kv_len, window, sink_tokens, out, workspace,
+                            workspace_bytes, status, stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  int* table = reinterpret_cast<int*>(ws + l.table);
+  int* lens = reinterpret_cast<int*>(ws + l.lens);
+  int2* dead = reinterpret_cast<int2*>(ws + l.dead);
+  constexpr int per_block = mla::kWindowThreads / 32;
+  mla::mla_window_plan_kernel<<<unsigned((batch + per_block - 1) / per_block), mla::kWindowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      page_table, page_table_stride, page_table_width, kv_lens, mla::ChunkTokens{nullptr, batch, 0}, batch, __builtin_ctz(unsigned(page_size)),
+      window, sink_tokens, l.width, table, lens, dead);
   MLA_CUDA(cudaGetLastError());
-  const int64_t units = int64_t(l.max_tiles) * (mla::kExtTile / mla::kExtTokens) + int64_t(l.max_items) * (mla::kExtRows / mla::kExtQRows);
-  const int64_t resident = int64_t(d->sm_count) * (2048 / mla::kExtPrepThreads);
-  MLA_CUDA(launch_dependent(mla::mla_extend_prep_kernel, dim3(unsigned(units < resident ? units : resident)), dim3(mla::kExtPrepThreads), 0, st, E, O));
-  MLA_CUDA(launch_dependent_cluster(mla::mla_extend_kernel, dim3(unsigned(2 * l.pairs)), dim3(mla::kExtThreads), mla::ext_smem_bytes(), st, 2u, kv_map,
-                                    q_map, P));
-  MLA_CUDA(launch_dependent(mla::mla_extend_combine_kernel, dim3(unsigned(l.pairs), mla::kExtRows / 4), dim3(128), 0, st, E,
-                            static_cast<const float*>(P.lse_part), static_cast<const float*>(P.o_part), static_cast<uint2*>(out)));
-  return 0;
+  return decode_impl(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, table, l.width, lens, batch, heads, sm_scale,
+                     ckv_scale, kpe_scale, l.max_len, 0, NVFP4_MLA_PRECISION_BF16, out, out_f32, lse, workspace, int64_t(l.table), stream, 128,
+                     1, 0, dead, status);
 }
 
 // ---- decode without caller-provided scratch -----------------------------------------------------------------------

@@ -55,9 +55,11 @@ struct ExtPair {
 // What the caller gives and how much room there is
 struct ExtProblem {
   const int* kv_lens;
-  const int* indptr;
+  const int* indptr;  // null: one query token per request
   int batch, total_q, heads, max_kv_len, window, sinks, pairs;
   int max_items, max_tiles;
+  int first_q;      // without an indptr: index of the first request's query token
+  int edges;        // 1: the rows in front of the first request's are this call's to fill with zeros, 2: those behind the last one's
   int* req_tile0;   // [batch + 1] workspace tiles before request b
   int4* req_map;    // [batch] {shift, first tokens' tiles, tokens in the tiles (with the shift taken out), first token of the window}
   ExtItem* items;   // [max_items]
@@ -96,9 +98,11 @@ __device__ __forceinline__ int block_scan(int v, int* sums, int& all) {
 struct ExtRequest {
   int q0, q, n, pos0, begin, shift, sink_tiles, tiles;
 };
+// index of request b's first query token; without an indptr every request has one
+__device__ __forceinline__ int ext_first(const ExtProblem& E, int b) { return E.indptr ? E.indptr[b] : E.first_q + b; }
 __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
   ExtRequest r;
-  const int a = E.indptr[b], z = E.indptr[b + 1];
+  const int a = ext_first(E, b), z = ext_first(E, b + 1);
   const int lo = a < 0 ? 0 : a, hi = z < E.total_q ? z : E.total_q;
   r.q0 = lo, r.q = hi > lo ? hi - lo : 0;
   const int n = E.kv_lens[b];
@@ -387,9 +391,9 @@ __device__ __forceinline__ void ext_convert_rows(const ExtProblem& E, const ExtO
 __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const ExtProblem E, const ExtOperands O) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const int first = E.indptr[0] < 0 ? 0 : E.indptr[0] < E.total_q ? E.indptr[0] : E.total_q;
-  const int z = E.indptr[E.batch], last = z < first ? first : z < E.total_q ? z : E.total_q;
-  const long long front = (long long)first * E.heads, none = front + (long long)(E.total_q - last) * E.heads;
+  const int a = ext_first(E, 0), first = a < 0 ? 0 : a < E.total_q ? a : E.total_q;
+  const int z = ext_first(E, E.batch), last = z < first ? first : z < E.total_q ? z : E.total_q;
+  const long long front = E.edges & 1 ? (long long)first * E.heads : 0, none = front + (E.edges & 2 ? (long long)(E.total_q - last) * E.heads : 0);
   for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < none; i += (long long)gridDim.x * 4) {
     const long long row = i < front ? i : i - front + (long long)last * E.heads;
     O.out[row * (CKV / 8) + (threadIdx.x & 63)] = make_uint4(0, 0, 0, 0);
@@ -403,50 +407,59 @@ __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const 
 
 // ---------------------------------------------------------------------------------------------------------------
 // Merge of the partial results of an item that several pairs worked on: pair p holds its first tiles, the pairs behind it the rest. The
-// partials of a pair: slot 2 p + 1 an item that it began, 2 p one that another pair began. A warp takes a row (four 16-byte loads per
-// partial and lane, all of a partial's before the first is used); rows of many partials take the whole block.
+// partials of a pair: slot 2 p + 1 an item that it began, 2 p one that another pair began. A warp takes a row, four partials at a time
+// (sixteen 16-byte loads per lane in flight).
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kExtFewParts = 8;
 __global__ void __launch_bounds__(128)
 mla_extend_combine_kernel(const ExtProblem E, const float* __restrict__ lse_part, const float* __restrict__ o_part, uint2* __restrict__ out) {
-  __shared__ float weights[kCombineMaxParts];
   ptx::grid_dependency_wait();
   const int p = blockIdx.x, lane = threadIdx.x & 31;
   const ExtPair pair = E.pair[p];
   if (pair.split < 0) return;
   const int row0 = E.items[pair.split].row0, rows = E.items[pair.split].rows, parts = pair.parts;
-  auto slot = [&](int i, int r) { return (long long)(i ? 2 * (p + i) : 2 * p + 1) * kExtRows + r; };
-  auto lse_of = [&](int i, int r) { return i && E.pair[p + i].count == 0 ? -INFINITY : lse_part[slot(i, r)]; };  // (a pair may have none of the rest)
-  if (parts <= kExtFewParts) {
-    const int r = 4 * blockIdx.y + (threadIdx.x >> 5);
-    if (r >= rows) return;
-    const float lse = lane < parts ? lse_of(lane, r) : -INFINITY;
-    const float M = warp_max(lse), w = lse == -INFINITY ? 0.f : exp2f(lse - M);
-    const float den = warp_sum(w);
-    float4 acc[4] = {};
-#pragma unroll 2
-    for (int i = 0; i < parts; ++i) {
-      const float wi = __shfl_sync(~0u, w, i);
-      if (wi == 0.f) continue;
-      const float4* src = reinterpret_cast<const float4*>(o_part + slot(i, r) * CKV) + lane;
+  const int r = 4 * blockIdx.y + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  auto slot = [&](int i) { return (long long)(i ? 2 * (p + i) : 2 * p + 1) * kExtRows + r; };
+  // the weights, one partial per lane and round (a pair may have got none of the rest: nothing is in its slot)
+  constexpr int kRounds = (kExtMaxPairs + 31) / 32;
+  float w[kRounds], M = -INFINITY, den = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 v = src[32 * j];
-        acc[j].x += wi * v.x, acc[j].y += wi * v.y, acc[j].z += wi * v.z, acc[j].w += wi * v.w;
+  for (int k = 0; k < kRounds; ++k) {
+    const int i = 32 * k + lane;
+    w[k] = i < parts && (i == 0 || E.pair[p + i].count > 0) ? lse_part[slot(i)] : -INFINITY;
+    M = fmaxf(M, w[k]);
+  }
+  M = warp_max(M);
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) w[k] = w[k] == -INFINITY ? 0.f : exp2f(w[k] - M), den += w[k];
+  den = warp_sum(den);
+  float4 acc[4] = {};
+  auto add = [&](float wi, const float4 (&v)[4]) {
+    if (wi == 0.f) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j].x += wi * v[j].x, acc[j].y += wi * v[j].y, acc[j].z += wi * v[j].z, acc[j].w += wi * v[j].w;
+  };
+  constexpr int U = 4;  // partials in flight
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    for (int i = 0; i < 32 && 32 * k + i < parts; i += U) {
+      float wi[U];
+      float4 v[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        wi[u] = __shfl_sync(~0u, w[k], i + u);
+        const float4* src = reinterpret_cast<const float4*>(o_part + slot(32 * k + i + u) * CKV) + lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[u][j] = wi[u] != 0.f ? src[32 * j] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-    }
-    const float s = den != 0.f ? 1.f / den : 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      out[((long long)row0 + r) * (CKV / 4) + 32 * j + lane] = make_uint2(pack_bf16x2(acc[j].x * s, acc[j].y * s), pack_bf16x2(acc[j].z * s, acc[j].w * s));
-    return;
+      for (int u = 0; u < U; ++u) add(wi[u], v[u]);
+    }
   }
-  for (int r = 4 * blockIdx.y; r < 4 * int(blockIdx.y) + 4 && r < rows; ++r) {
-    merge_row<1>(
-        parts, [&](int i) { return lse_of(i, r); }, [&](int i) { return o_part + slot(i, r) * CKV; }, (long long)row0 + r, out, nullptr, nullptr,
-        weights, nullptr);
-    __syncthreads();
-  }
+  const float s = den != 0.f ? 1.f / den : 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    out[((long long)row0 + r) * (CKV / 4) + 32 * j + lane] = make_uint2(pack_bf16x2(acc[j].x * s, acc[j].y * s), pack_bf16x2(acc[j].z * s, acc[j].w * s));
 }
 
 }  // namespace mla

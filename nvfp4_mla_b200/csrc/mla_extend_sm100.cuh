@@ -285,19 +285,31 @@ __device__ __forceinline__ void ext_softmax_role(ExtSmem& s, const ExtParams& P,
       }
       // P = 2^(s qa - m) as FP16, 64 tokens of the row = 128 bytes
       const float neg_m = mx_run == -INFINITY ? 0.f : -mx_run;
-      uint32_t pk[32];
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      auto eight = [&](int c, uint32_t (&pk)[4]) {  // weights of tokens 8 c ..
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const float2 x = ptx::fma_f32x2(make_float2(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1])), make_float2(qa, qa), make_float2(neg_m, neg_m));
-        const float2 e = make_float2(ptx::ex2(x.x), ptx::ex2(x.y));
-        ls[c & 1] = ptx::add_f32x2(ls[c & 1], e);
-        pk[c] = ptx::f32x2_to_f16x2(e.x, e.y);
-      }
-      l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = ptx::fma_f32x2(make_float2(__uint_as_float(sr[8 * c + 2 * k]), __uint_as_float(sr[8 * c + 2 * k + 1])), make_float2(qa, qa),
+                                          make_float2(neg_m, neg_m));
+          const float2 e = make_float2(ptx::ex2(x.x), ptx::ex2(x.y));
+          ls[k & 1] = ptx::add_f32x2(ls[k & 1], e);
+          pk[k] = ptx::f32x2_to_f16x2(e.x, e.y);
+        }
+      };
+      constexpr int kHeld = 4;  // sixteen-byte chunks that are ready before the products of the tile before have released P
+      uint32_t pk[kHeld > 0 ? kHeld : 1][4];
+#pragma unroll
+      for (int c = 0; c < kHeld; ++c) eight(c, pk[c]);
       if (g >= 1) ptx::mbar_wait(&s.pv_done, (g - 1) & 1, &s.abort_flag);  // (one that gives up raises the flag; the next vote ends the role)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) ptx::sts128(p_row + (uint32_t(c ^ (h & 7)) << 4), pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+      for (int c = 0; c < kHeld; ++c) ptx::sts128(p_row + (uint32_t(c ^ (h & 7)) << 4), pk[c][0], pk[c][1], pk[c][2], pk[c][3]);
+#pragma unroll
+      for (int c = kHeld; c < 8; ++c) {
+        uint32_t w[4];
+        eight(c, w);
+        ptx::sts128(p_row + (uint32_t(c ^ (h & 7)) << 4), w[0], w[1], w[2], w[3]);
+      }
+      l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
       ptx::fence_proxy_async_smem();
       ptx::tc_fence_before_sync();
       __syncwarp();

@@ -50,7 +50,7 @@ def test_nothing_to_do_needs_no_gpu(lib):
 
 @pytest.mark.parametrize("ps,window,sinks,text", [(48, 5, 0, "page_size"), (16, 0, 0, "window"), (16, -3, 0, "window"), (16, 5, -1, "sink")])
 def test_the_window_decode_refuses(lib, ps, window, sinks, text):
-    assert lib.nvfp4_mla_decode_window_workspace_bytes(2, 16, ps, 4, window, sinks) == -1
+    assert lib.nvfp4_mla_decode_window_workspace_bytes(2, 16, ps, 4, 64, window, sinks) == -1
     assert text in lib.nvfp4_mla_last_error().decode()
     refused(lib, lib.nvfp4_mla_decode_window(A, A, A, A, A, 8, ps, A, 4, 4, A, 2, 16, 0.1, 1.0, 1.0, 64, window, sinks, A, None, None, A, 1 << 40, None, None), text)
 

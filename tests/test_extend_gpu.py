@@ -222,3 +222,17 @@ def test_refusals():
         mla.decode_window(c.q_nope, c.q_pe, *args[2:], 5)
     with pytest.raises(RuntimeError):
         mla.decode_window(c.q_nope[:2, :8].contiguous(), c.q_pe[:2, :8].contiguous(), *args[2:], 5)
+
+
+@pytest.mark.parametrize("window", [0, 500])
+def test_a_loose_bound_takes_the_requests_in_groups(window):
+    """The bound of the lengths sizes the workspace (1152 bytes per token and request): far above what a group of requests may take."""
+    kv_lens, q_lens = [300, 2, 129, 1, 700, 40], [70, 2, 100, 1, 0, 33]
+    c = chunk(kv_lens, q_lens, 24, 64, pad=5)
+    table = torch.zeros(6, 100000, dtype=torch.int32, device="cuda")
+    table[:, :c.page_table.shape[1]] = c.page_table
+    small = run(c, window=window, sink_tokens=3)
+    c.page_table = table
+    out = run(c, max_kv_len=6_000_000, window=window, sink_tokens=3)
+    assert worst_row(out[:-5], reference(c, window, 3)) <= ROW_TOL and (out[-5:] == 0).all()
+    assert worst_row(out, small.double()) <= 2 * ROW_TOL
