@@ -497,9 +497,9 @@ namespace {
 constexpr int kExtendSlice = 512;  // query tokens at a time in the first form (the partial results of a slice take 2 KB per head and token)
 
 struct ExtendLayout {
-  size_t counts, req_tile0, req_map, items, pair, q_scale, lse_part, o_part, q16, kv16, total;
+  size_t counts, req_block0, req_map, items, pair, q_scale, lse_part, o_part, q16, kv16, total;
   int group;  // requests at a time
-  int pairs, max_items, max_tiles;
+  int pairs, max_items, max_blocks;
 };
 // The dequantised tokens of as many requests at a time as fit this (one at least): a bound far above the lengths must not ask for
 // more memory than there is. 7 million tokens.
@@ -508,33 +508,33 @@ int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window,
   MLA_CHECK(batch <= mla::kExtMaxBatch, "at most %d requests, got %d", mla::kExtMaxBatch, batch);
   MLA_CHECK(int64_t(total_q) * heads < (int64_t(1) << 31) - mla::kExtRows, "total_q * heads must be below 2^31");
   const int64_t len = max_kv_len > 1 ? max_kv_len : 1;
-  auto tiles_of = [&](int64_t requests) {
-    int64_t tiles = requests * ((len - 1) / mla::kExtTile + 1);
+  auto blocks_of = [&](int64_t requests) {
+    int64_t blocks = requests * ((len - 1) / mla::kExtBlock + 1);
     if (window > 0) {
-      const int64_t seen = requests * ((int64_t(sinks) + mla::kExtTile - 1) / mla::kExtTile + window / mla::kExtTile + 3) + total_q / mla::kExtTile;
-      if (seen < tiles) tiles = seen;
+      const int64_t seen = requests * ((int64_t(sinks) + mla::kExtBlock - 1) / mla::kExtBlock + window / mla::kExtBlock + 3) + total_q / mla::kExtBlock;
+      if (seen < blocks) blocks = seen;
     }
-    return tiles;
+    return blocks;
   };
-  constexpr int64_t tile_bytes = int64_t(mla::kExtTile) * mla::kExtRow * 2;
+  constexpr int64_t block_bytes = int64_t(mla::kExtBlock) * mla::kExtRow * 2;
   l->group = batch;
-  while (l->group > 1 && tiles_of(std::min(l->group, total_q)) * tile_bytes > kExtTokenBytes) l->group = (l->group + 1) / 2;
-  const int64_t requests = std::min(l->group, total_q), tiles = tiles_of(requests);  // (at most total_q requests have query tokens)
+  while (l->group > 1 && blocks_of(std::min(l->group, total_q)) * block_bytes > kExtTokenBytes) l->group = (l->group + 1) / 2;
+  const int64_t requests = std::min(l->group, total_q), blocks = blocks_of(requests);  // (at most total_q requests have query tokens)
   const int64_t items = requests + int64_t(total_q) * heads / mla::kExtRows;
-  MLA_CHECK(tiles * mla::kExtTile < (int64_t(1) << 31) && tiles + items < (int64_t(1) << 31) && items * ((len - 1) / mla::kExtTile + 1) < (int64_t(1) << 31),
+  MLA_CHECK((blocks + 4) * mla::kExtBlock < (int64_t(1) << 31) && blocks + items < (int64_t(1) << 29) && items * ((len - 1) / mla::kExtTile + 1) < (int64_t(1) << 31),
             "chunks of %d query tokens over %d requests of up to %lld tokens are too large for one call", total_q, batch, (long long)len);
-  l->pairs = d.ext_pairs, l->max_items = int(items), l->max_tiles = int(tiles);
+  l->pairs = d.ext_pairs, l->max_items = int(items), l->max_blocks = int(blocks);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
     off = mla::align_up(off + bytes, 256);
     return at;
   };
-  l->counts = take(64), l->req_tile0 = take(size_t(l->group + 1) * 4), l->req_map = take(size_t(l->group) * 16);
+  l->counts = take(64), l->req_block0 = take(size_t(l->group + 1) * 4), l->req_map = take(size_t(l->group) * 16);
   l->items = take(size_t(items) * sizeof(mla::ExtItem)), l->pair = take(size_t(l->pairs) * sizeof(mla::ExtPair));
   l->q_scale = take(size_t(items) * mla::kExtRows * 4);
   l->lse_part = take(size_t(l->pairs) * 2 * mla::kExtRows * 4), l->o_part = take(size_t(l->pairs) * 2 * mla::kExtRows * mla::CKV * 4);
-  l->q16 = take(size_t(items) * mla::kExtRows * mla::kExtRow * 2), l->kv16 = take(size_t(tiles) * mla::kExtTile * mla::kExtRow * 2);
+  l->q16 = take(size_t(items) * mla::kExtRows * mla::kExtRow * 2), l->kv16 = take(size_t(blocks) * block_bytes);
   l->total = off;
   return 0;
 }
@@ -585,13 +585,13 @@ int extend_shared(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache
                   float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, uint8_t* ws, const ExtendLayout& l, const DeviceInfo& d,
                   int32_t* status, cudaStream_t st) {
   CUtensorMap kv_map, q_map;
-  if (make_half_map(ws + l.kv16, int64_t(l.max_tiles) * mla::kExtTile, &kv_map)) return 1;
+  if (make_half_map(ws + l.kv16, int64_t(l.max_blocks) * mla::kExtBlock, &kv_map)) return 1;
   if (make_half_map(ws + l.q16, int64_t(l.max_items) * mla::kExtRows, &q_map)) return 1;
 
   mla::ExtProblem E;
   E.total_q = total_q, E.heads = heads, E.max_kv_len = max_kv_len;
-  E.window = window, E.sinks = sink_tokens, E.pairs = l.pairs, E.max_items = l.max_items, E.max_tiles = l.max_tiles;
-  E.req_tile0 = reinterpret_cast<int*>(ws + l.req_tile0);
+  E.window = window, E.sinks = sink_tokens, E.pairs = l.pairs, E.max_items = l.max_items, E.max_blocks = l.max_blocks;
+  E.req_block0 = reinterpret_cast<int*>(ws + l.req_block0);
   E.req_map = reinterpret_cast<int4*>(ws + l.req_map), E.items = reinterpret_cast<mla::ExtItem*>(ws + l.items);
   E.pair = reinterpret_cast<mla::ExtPair*>(ws + l.pair), E.counts = reinterpret_cast<int*>(ws + l.counts), E.status = status;
   mla::ExtOperands O;
@@ -603,7 +603,7 @@ int extend_shared(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache
   mla::ExtParams P;
   P.q_scale = O.q_scale, P.ckv_scale = ckv_scale, P.lse_part = reinterpret_cast<float*>(ws + l.lse_part);
   P.o_part = reinterpret_cast<float*>(ws + l.o_part), P.out = static_cast<uint16_t*>(out), P.status = status;
-  const int64_t units = int64_t(l.max_tiles) * (mla::kExtTile / mla::kExtTokens) + int64_t(l.max_items) * (mla::kExtRows / mla::kExtQRows);
+  const int64_t units = int64_t(l.max_blocks) + int64_t(l.max_items) * (mla::kExtRows / mla::kExtQRows);
   const int64_t resident = int64_t(d.sm_count) * (2048 / mla::kExtPrepThreads);
   for (int b = 0; b < batch; b += l.group) {
     E.batch = batch - b < l.group ? batch - b : l.group;

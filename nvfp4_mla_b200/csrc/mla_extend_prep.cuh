@@ -1,15 +1,16 @@
 // Chunks of new tokens, everything around the attention kernel (mla_extend_sm100.cuh): the schedule, the FP16 operands, the merge.
 //
-// The rows of a request (query token, head) are cut into tiles of 128, the ITEMS; an item's work is the 256-token tiles of the cache
-// that its rows see. The items are dealt out whole, item i to CTA pair i % pairs, for as many rounds as leave every pair at or below
+// The rows of a request (query token, head) are cut into tiles of 128, the ITEMS; an item's work is the 64-token BLOCKS of the cache
+// that its rows see, four to a tile of the attention kernel. The items are dealt out whole, item i to CTA pair i % pairs, for as many rounds as leave every pair at or below
 // its even share of the tiles; the tiles of the items that are left are laid end to end and cut so that every pair ends up with its
 // share. Pairs that work at the same time thus work on neighbouring items, which read the same tokens: with one contiguous piece of
 // the flattened tiles per pair, 24 ragged chunks over 115 MB of FP16 rows read 1.6 GB from HBM (a third of the sectors missed L2) and
 // took 913 us.
 //
 // Window: the tokens that some query of the request sees are [0, S) and everything from the first query's window on. The cache is
-// read into a numbering of tiles that has no gap: the first `sink_tiles` tiles, then the tiles from the window's on, `shift` tokens
-// further in the request. An item skips the tiles between the first tokens' and its own window.
+// read into a numbering of blocks that has no gap: the first `sink_blocks` blocks, then the blocks from the window's on, `shift` tokens
+// further in the request. An item skips the blocks between the first tokens' and its own window; its tiles are four of its blocks
+// each, wherever these lie (with whole 256-token tiles, 8 windowed chunks of 4096 + 128 tokens took 18 tiles per item instead of 17).
 //
 // Operands: the attention kernel multiplies FP16. Every visible token is dequantised once per call into a workspace row of 576 (latent
 // 512, rope 64, exact: e2m1 x e4m3 has six significant bits), every query row once into a row of the same shape, held times a power
@@ -27,6 +28,7 @@
 namespace mla {
 
 constexpr int kExtRows = 128;   // rows of an item
+constexpr int kExtBlock = 64;   // tokens of a block
 constexpr int kExtTile = 256;   // tokens of a tile
 constexpr int kExtRow = CKV + KPE;
 constexpr int kExtMaxBatch = 8192;
@@ -35,9 +37,9 @@ constexpr int kExtMaxPairs = 128;
 struct ExtItem {
   int prefix;      // tiles of the items before
   int ntiles;      // at least 1 (an item that sees nothing has one tile, all masked)
-  int tile0;       // first workspace tile of the request
-  int sinks, skip; // tiles: the first tokens' ones, and how many follow them that no row sees
-  int shift;       // tokens: position of a token in the request minus its place in the request's workspace tiles, behind the first tokens' tiles
+  int block0;      // first workspace block of the request
+  int sinks, skip; // blocks: the first tokens' ones, and how many follow them that no row sees
+  int shift;       // tokens: position of a token in the request minus its place in the request's workspace blocks, behind the first tokens' blocks
   int row0, rows;  // first row in [total_q * heads], number of rows
   int r0;          // first row within the request
   int pos0;        // position of the request's first query token
@@ -57,14 +59,14 @@ struct ExtProblem {
   const int* kv_lens;
   const int* indptr;  // null: one query token per request
   int batch, total_q, heads, max_kv_len, window, sinks, pairs;
-  int max_items, max_tiles;
+  int max_items, max_blocks;
   int first_q;      // without an indptr: index of the first request's query token
   int edges;        // 1: the rows in front of the first request's are this call's to fill with zeros, 2: those behind the last one's
-  int* req_tile0;   // [batch + 1] workspace tiles before request b
-  int4* req_map;    // [batch] {shift, first tokens' tiles, tokens in the tiles (with the shift taken out), first token of the window}
+  int* req_block0;  // [batch + 1] workspace blocks before request b
+  int4* req_map;    // [batch] {shift, first tokens' blocks, tokens in the blocks (with the shift taken out), first token of the window}
   ExtItem* items;   // [max_items]
   ExtPair* pair;    // [pairs]
-  int* counts;      // [0] items, [1] workspace tiles
+  int* counts;      // [0] items, [1] workspace blocks
   int* status;
 };
 
@@ -96,7 +98,7 @@ __device__ __forceinline__ int block_scan(int v, int* sums, int& all) {
 }
 
 struct ExtRequest {
-  int q0, q, n, pos0, begin, shift, sink_tiles, tiles;
+  int q0, q, n, pos0, begin, shift, sink_blocks, blocks;
 };
 // index of request b's first query token; without an indptr every request has one
 __device__ __forceinline__ int ext_first(const ExtProblem& E, int b) { return E.indptr ? E.indptr[b] : E.first_q + b; }
@@ -108,18 +110,18 @@ __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
   const int n = E.kv_lens[b];
   r.n = n < 0 ? 0 : n < E.max_kv_len ? n : E.max_kv_len;
   r.pos0 = r.n - (z - a) + (lo - a);
-  r.shift = 0, r.sink_tiles = 0, r.begin = 0;
+  r.shift = 0, r.sink_blocks = 0, r.begin = 0;
   if (E.window > 0) {
-    const long long s = ((long long)E.sinks + kExtTile - 1) / kExtTile;
+    const long long s = ((long long)E.sinks + kExtBlock - 1) / kExtBlock;
     const long long begin = (long long)r.pos0 - E.window + 1;  // first token in the window of the first query token
     r.begin = begin > 0 ? int(begin) : 0;
-    const long long t = r.begin / kExtTile;
-    if (t > s) r.shift = int(t - s) * kExtTile;
-    r.sink_tiles = int(s < (r.n + kExtTile - 1) / kExtTile ? s : (r.n + kExtTile - 1) / kExtTile);
+    const long long t = r.begin / kExtBlock;
+    if (t > s) r.shift = int(t - s) * kExtBlock;
+    r.sink_blocks = int(s < (r.n + kExtBlock - 1) / kExtBlock ? s : (r.n + kExtBlock - 1) / kExtBlock);
   }
-  r.tiles = (r.n - r.shift + kExtTile - 1) / kExtTile;
-  if (r.tiles < 1) r.tiles = 1;
-  if (r.q == 0) r.tiles = 0;
+  r.blocks = (r.n - r.shift + kExtBlock - 1) / kExtBlock;
+  if (r.blocks < 1) r.blocks = 1;
+  if (r.q == 0) r.blocks = 0;
   return r;
 }
 
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
   static_assert(kExtSchedThreads == 1024, "block_scan takes 32 warps");
   ptx::grid_launch_dependents();
   const int tid = threadIdx.x;
-  int items = 0, tiles = 0;
+  int items = 0, blocks = 0;
   ExtRequest r = {};
   for (int b0 = 0; b0 < E.batch; b0 += kExtSchedThreads) {
     const int b = b0 + tid;
@@ -143,19 +145,19 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
     }
     const int ii = items + block_scan(mine, sums, all) - mine;
     items += all;
-    const int it = tiles + block_scan(r.tiles, sums, all) - r.tiles;
-    tiles += all;
+    const int ib = blocks + block_scan(r.blocks, sums, all) - r.blocks;
+    blocks += all;
     if (b < E.batch) {
-      item0[b] = ii, E.req_tile0[b] = it;
-      E.req_map[b] = make_int4(r.shift, r.sink_tiles, r.n - r.shift, r.begin);
+      item0[b] = ii, E.req_block0[b] = ib;
+      E.req_map[b] = make_int4(r.shift, r.sink_blocks, r.n - r.shift, r.begin);
     }
   }
   // (a query index that runs backwards could ask for more than there is room for)
-  if (items > E.max_items || tiles > E.max_tiles) {
+  if (items > E.max_items || blocks > E.max_blocks) {
     if (tid == 0 && E.status) atomicExch(E.status, int(kBadSchedule));
-    items = 0, tiles = 0;
+    items = 0, blocks = 0;
   }
-  if (tid == 0) E.req_tile0[E.batch] = tiles, E.counts[0] = items, E.counts[1] = tiles, rounds_s = items / E.pairs;
+  if (tid == 0) E.req_block0[E.batch] = blocks, E.counts[0] = items, E.counts[1] = blocks, rounds_s = items / E.pairs;
   __syncthreads();
 
   // ---- items
@@ -174,18 +176,18 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
       m.r0 = (i - item0[lo]) * kExtRows;
       const long long rows = (long long)r.q * E.heads - m.r0;
       m.rows = int(rows < kExtRows ? rows : kExtRows);
-      m.row0 = r.q0 * E.heads + m.r0, m.pos0 = r.pos0, m.shift = r.shift, m.tile0 = E.req_tile0[lo];
+      m.row0 = r.q0 * E.heads + m.r0, m.pos0 = r.pos0, m.shift = r.shift, m.block0 = E.req_block0[lo];
       const int first = r.pos0 + m.r0 / E.heads, last = r.pos0 + (m.r0 + m.rows - 1) / E.heads;  // positions of its query tokens
       const int end = last + 1 < r.n ? last + 1 : r.n;                                           // tokens before it are seen
-      int e = (end - r.shift + kExtTile - 1) / kExtTile;                                         // tiles up to there
+      int e = (end - r.shift + kExtBlock - 1) / kExtBlock;                                       // blocks up to there
       if (E.window > 0) {
         const long long begin = (long long)first - E.window + 1 - r.shift;
-        const int t = begin > 0 ? int(begin / kExtTile) : 0;
-        m.sinks = r.sink_tiles;
+        const int t = begin > 0 ? int(begin / kExtBlock) : 0;
+        m.sinks = r.sink_blocks;
         if (t > m.sinks) m.skip = t - m.sinks;
       }
-      if (e > r.tiles) e = r.tiles;
-      m.ntiles = e - m.skip;
+      if (e > r.blocks) e = r.blocks;
+      m.ntiles = (e - m.skip + kExtTile / kExtBlock - 1) / (kExtTile / kExtBlock);
       if (m.ntiles < 1) m.ntiles = 1, m.skip = 0;
     }
     int all;
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Operands. A unit of work is 64 tokens of a workspace tile or 32 rows of an item, 8 or 4 per warp: all loads of a warp's four rows are
+// Operands. A unit of work is a block of 64 tokens or 32 rows of an item, 8 or 4 per warp: all loads of a warp's four rows are
 // issued before the first is used. All blocks share the rows of no request (zeros in the output).
 // ---------------------------------------------------------------------------------------------------------------
 struct ExtOperands {
@@ -269,14 +271,13 @@ struct ExtOperands {
   long long pt_stride;
   int pt_width, page_shift, num_pages;
   float ckv_scale, kpe_scale, sm_scale_log2;
-  __half* kv16;     // [max_tiles * 256][576]
+  __half* kv16;     // [max_blocks * 64][576]
   __half* q16;      // [max_items * 128][576]
   float* q_scale;   // [max_items * 128]: factor of a row's scores, log2 units
   uint4* out;       // [total_q * heads][512] BF16
 };
 
 constexpr int kExtPrepThreads = 256;
-constexpr int kExtTokens = 64;  // tokens of a unit
 constexpr int kExtQRows = 32;   // rows of a unit
 
 // last b in [0, n) with a[b] <= x (a is non-decreasing, a[0] <= x), by the whole warp: 32 probes at a time
@@ -294,15 +295,15 @@ __device__ __forceinline__ int warp_upper(const int* __restrict__ a, int n, int 
 
 __device__ __forceinline__ void ext_convert_tokens(const ExtProblem& E, const ExtOperands& O, int unit) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int kPer = kExtTokens / (kExtPrepThreads / 32);  // tokens of a warp
-  const int t0 = unit * kExtTokens + kPer * warp, tile = t0 / kExtTile;
-  const int lo = warp_upper(E.req_tile0, E.batch, tile);
+  constexpr int kPer = kExtBlock / (kExtPrepThreads / 32);  // tokens of a warp
+  const int t0 = unit * kExtBlock + kPer * warp;
+  const int lo = warp_upper(E.req_block0, E.batch, unit);
   const int4 map = E.req_map[lo];
-  const int v = t0 - E.req_tile0[lo] * kExtTile + lane;  // this lane's token among the request's
+  const int v = t0 - E.req_block0[lo] * kExtBlock + lane;  // this lane's token among the request's
   int src = -1;                                          // its cache row; -1: zeros
-  if (lane < kPer && v < map.z) {
-    const int tok = v < map.y * kExtTile ? v : v + map.x;
-    // (tokens between the first ones and the window belong to tiles that are read, but their pages may be gone)
+  if (lane < kPer && v < map.z && unit < E.counts[1]) {
+    const int tok = v < map.y * kExtBlock ? v : v + map.x;
+    // (tokens between the first ones and the window belong to blocks that are read, but their pages may be gone)
     if (tok < E.sinks || tok >= map.w) {
       const int pi = tok >> O.page_shift;
       const int page = pi < O.pt_width ? O.page_table[(long long)lo * O.pt_stride + pi] : -1;
@@ -398,7 +399,8 @@ __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const 
     const long long row = i < front ? i : i - front + (long long)last * E.heads;
     O.out[row * (CKV / 8) + (threadIdx.x & 63)] = make_uint4(0, 0, 0, 0);
   }
-  const int tokens = E.counts[1] * (kExtTile / kExtTokens), units = tokens + E.counts[0] * (kExtRows / kExtQRows);
+  // (the last tile reads up to three blocks behind the last one, with weight 0: zeros)
+  const int tokens = E.counts[1] + 3 < E.max_blocks ? E.counts[1] + 3 : E.max_blocks, units = tokens + E.counts[0] * (kExtRows / kExtQRows);
   for (int i = blockIdx.x; i < units; i += gridDim.x) {
     if (i < tokens) ext_convert_tokens(E, O, i);
     else ext_convert_rows(E, O, i - tokens);
@@ -407,10 +409,10 @@ __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const 
 
 // ---------------------------------------------------------------------------------------------------------------
 // Merge of the partial results of an item that several pairs worked on: pair p holds its first tiles, the pairs behind it the rest. The
-// partials of a pair: slot 2 p + 1 an item that it began, 2 p one that another pair began. A warp takes a row, four partials at a time
-// (sixteen 16-byte loads per lane in flight).
+// partials of a pair: slot 2 p + 1 an item that it began, 2 p one that another pair began. A warp takes a row, two partials at a time
+// (eight 16-byte loads per lane in flight).
 // ---------------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, 8)
 mla_extend_combine_kernel(const ExtProblem E, const float* __restrict__ lse_part, const float* __restrict__ o_part, uint2* __restrict__ out) {
   ptx::grid_dependency_wait();
   const int p = blockIdx.x, lane = threadIdx.x & 31;
@@ -439,7 +441,7 @@ mla_extend_combine_kernel(const ExtProblem E, const float* __restrict__ lse_part
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j].x += wi * v[j].x, acc[j].y += wi * v[j].y, acc[j].z += wi * v[j].z, acc[j].w += wi * v[j].w;
   };
-  constexpr int U = 4;  // partials in flight
+  constexpr int U = 2;  // partials in flight
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
     for (int i = 0; i < 32 && 32 * k + i < parts; i += U) {

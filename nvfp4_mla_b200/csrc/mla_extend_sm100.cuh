@@ -71,8 +71,8 @@ struct ExtWalk {
     return true;
   }
 };
-// workspace tile of tile t of an item, within the request
-__device__ __forceinline__ int ext_tile(const ExtItem& m, int t) { return t < m.sinks ? t : t + m.skip; }
+// workspace block of block j of an item, within the request (blocks behind the item's last are read and masked)
+__device__ __forceinline__ int ext_block(const ExtItem& m, int j) { return j < m.sinks ? j : j + m.skip; }
 
 struct ExtParams {
   ExtProblem E;
@@ -101,24 +101,24 @@ __device__ __forceinline__ void ext_producer_role(ExtSmem& s, const ExtParams& P
     if (++slot == kExtUnits) slot = 0, phase ^= 1;
     return true;
   };
-  auto load_k = [&](int row) {
-    const int y = row + 128 * int(rank);
+  auto load_k = [&](const int (&row)[4]) {
+    const int y0 = rank ? row[2] : row[0], y1 = rank ? row[3] : row[1];
 #pragma unroll 1
     for (int u = 0; u < 9; ++u)
-      if (!load(64 * u, y, 64 * u, y + 64)) return false;
+      if (!load(64 * u, y0, 64 * u, y1)) return false;
     return true;
   };
-  auto load_v = [&](int row) {
-#pragma unroll 1
-    for (int u = 0; u < 8; ++u) {  // 64 tokens u / 2, channel half u % 2
-      const int x = 256 * (u & 1) + 128 * int(rank), y = row + 64 * (u >> 1);
-      if (!load(x, y, x + 64, y)) return false;
+  auto load_v = [&](const int (&row)[4]) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {  // block u / 2, channel half u % 2
+      const int x = 256 * (u & 1) + 128 * int(rank);
+      if (!load(x, row[u >> 1], x + 64, row[u >> 1])) return false;
     }
     return true;
   };
   ExtWalk walk(P.E, pair);
   ExtItem m;
-  int t0, t1, before = -1;  // workspace row of the tile whose V is due
+  int t0, t1, before[4] = {-1, -1, -1, -1};  // workspace rows of the blocks of the tile whose V is due
   uint32_t n_items = 0;
   while (walk.next(m, t0, t1)) {
     // the query, once every QK^T of the item before has read the old one
@@ -128,13 +128,16 @@ __device__ __forceinline__ void ext_producer_role(ExtSmem& s, const ExtParams& P
     for (int p = 0; p < 9; ++p) ptx::tma_load_2d_pair(q + p * kExtPanel, q_map, 64 * p, walk.item * kExtRows + 64 * int(rank), q_full);
     ++n_items;
     for (int t = t0; t < t1; ++t) {
-      const int row = (m.tile0 + ext_tile(m, t)) * kExtTile;
+      int row[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) row[j] = (m.block0 + ext_block(m, 4 * t + j)) * kExtBlock;
       if (!load_k(row)) return;
-      if (before >= 0 && !load_v(before)) return;
-      before = row;
+      if (before[0] >= 0 && !load_v(before)) return;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) before[j] = row[j];
     }
   }
-  if (before >= 0) load_v(before);
+  if (before[0] >= 0) load_v(before);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -245,11 +248,11 @@ __device__ __forceinline__ void ext_softmax_role(ExtSmem& s, const ExtParams& P,
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cta(s_free0 + 8 * buf);
       // position of this thread's first token
-      const int at = ext_tile(m, t) * kExtTile + 64 * part + (t < m.sinks ? 0 : m.shift);
+      const int j = 4 * t + part, at = ext_block(m, j) * kExtBlock + (j < m.sinks ? 0 : m.shift);
       const int hi_t = end - at, lo_t = begin - at, sk_t = sinks - at;
       if (!ok || hi_t < 64 || (lo_t > 0 && sk_t < 64)) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) sr[j] = ok && j < hi_t && (j >= lo_t || j < sk_t) ? sr[j] : 0xFF800000u;
+        for (int k = 0; k < 64; ++k) sr[k] = ok && k < hi_t && (k >= lo_t || k < sk_t) ? sr[k] : 0xFF800000u;
       }
       float mxs[4] = {__uint_as_float(sr[0]), __uint_as_float(sr[1]), __uint_as_float(sr[2]), __uint_as_float(sr[3])};
 #pragma unroll

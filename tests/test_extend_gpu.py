@@ -236,3 +236,24 @@ def test_a_loose_bound_takes_the_requests_in_groups(window):
     out = run(c, max_kv_len=6_000_000, window=window, sink_tokens=3)
     assert worst_row(out[:-5], reference(c, window, 3)) <= ROW_TOL and (out[-5:] == 0).all()
     assert worst_row(out, small.double()) <= 2 * ROW_TOL
+
+
+@pytest.mark.parametrize("kv_lens,q_lens,window,sinks", [([300, 65, 1], [90, 2, 1], 0, 0), ([1000, 70], [60, 60], 130, 70), ([64], [64], 0, 0), ([130], [2], 1, 0)])
+def test_what_the_workspace_held_before_does_not_matter(kv_lens, q_lens, window, sinks):
+    """The C entry with a workspace full of NaN and one just as large as asked for."""
+    lib, heads, ps = mla._lib.load(), 24, 64
+    c = chunk(kv_lens, q_lens, heads, ps)
+    sizes = (len(kv_lens), sum(q_lens), heads, ps, c.page_table.shape[1], max(kv_lens), window, sinks)
+    ws = torch.full((lib.nvfp4_mla_extend_workspace_bytes(*sizes),), 0xFF, dtype=torch.uint8, device="cuda")
+    out = torch.full((sum(q_lens), heads, 512), float("nan"), dtype=torch.bfloat16, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def call(nbytes):
+        return lib.nvfp4_mla_extend(c.q_nope.data_ptr(), c.q_pe.data_ptr(), *(t.data_ptr() for t in c.cache), c.ckv_cache.shape[0], ps, c.page_table.data_ptr(),
+                                    c.page_table.stride(0), c.page_table.shape[1], c.kv_lens.data_ptr(), c.indptr.data_ptr(), len(kv_lens), sum(q_lens), heads, SM_SCALE,
+                                    c.ckv_scale, c.kpe_scale, max(kv_lens), window, sinks, out.data_ptr(), ws.data_ptr(), nbytes, status.data_ptr(),
+                                    torch.cuda.current_stream().cuda_stream)
+
+    assert call(ws.numel() - 1) != 0 and "workspace" in lib.nvfp4_mla_last_error().decode()
+    assert call(ws.numel()) == 0
+    assert worst_row(out, reference(c, window, sinks)) <= ROW_TOL and int(status) == 0
