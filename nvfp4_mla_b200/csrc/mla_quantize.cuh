@@ -189,9 +189,9 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 //
 // One warp per token per trip, lane l = scale block l, as above; a lane's normalised BF16 values sit in shared memory for the few that
 // have to be settled, the weights there too. 1512 bytes per token, bound by the latency of a warp's chain of steps (414 warp
-// instructions per token, 65 % of the issue slots): 274880 tokens in 147 us (63 at the measured copy bandwidth; the writer above 82).
+// instructions per token, 65 % of the issue slots): 274880 tokens in 150 us (63 at the measured copy bandwidth; the writer above 82).
 // With the norm in 64 bits throughout it took 345 us, one instruction per value and step 273; fetching the next token's row
-// ahead gained nothing at the registers it took (149), and 24 or 40 warps per SM instead of 32 were 149 to 154.
+// ahead gained nothing at the registers it took (149), and 24 or 40 warps per SM instead of 32 made it 182 and 176.
 // ---------------------------------------------------------------------------------------------------------------
 // whether the fp32 number y, off by at most `units` in its last place, may round to another BF16 number than what it stands for: its low
 // half is within `units` of 0x8000
@@ -230,9 +230,9 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
     if constexpr (INTERLEAVED) rope = __ldcs(reinterpret_cast<const uint32_t*>(rp) + lane);
     else rope = uint32_t(__ldcs(reinterpret_cast<const uint16_t*>(rp) + lane)) | uint32_t(__ldcs(reinterpret_cast<const uint16_t*>(rp) + 32 + lane)) << 16;
     const float a = __uint_as_float(rope << 16), b = __uint_as_float(rope & 0xFFFF0000u);
-    const int pos = positions[t];
+    const int pos = positions[t], request = batch_indices[t];
     // (the slot is needed at the end only: the arithmetic does not wait for the walk through the page tables)
-    const long long row = pos < max_pos ? cache_row(batch_indices[t], pos, int(num_pages), page_shift, kv_indices, kv_indptr, batch) : -1;
+    const long long row = pos < max_pos ? cache_row(request, pos, int(num_pages), page_shift, kv_indices, kv_indptr, batch) : -1;
     const bool rotated = uint32_t(pos) < uint32_t(max_pos);
     const float cs = rotated ? __ldg(cos_sin + (long long)pos * KPE + lane) : 0.f, sn = rotated ? __ldg(cos_sin + (long long)pos * KPE + 32 + lane) : 0.f;
     const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
