@@ -486,16 +486,9 @@ def _append(nnz, ckv, kpe, batch_indices, positions, ckv_cache, ckv_sf_cache, kp
         float(kpe_scale), _ptr(status), torch.cuda.current_stream(dev).cuda_stream)))
 
 
-def norm_rope_append_paged_mla_kv_cache(ckv, kpe, norm_weight, cos_sin, batch_indices, positions, ckv_cache, ckv_sf_cache, kpe_cache,
-                                        kv_indices, kv_indptr, eps=1e-6, ckv_scale=1.0, kpe_scale=1.0, interleaved=True, check=False):
-    """RMS-normalises, rotates, quantises and writes the latent projection's raw rows into the paged cache, in place and in one pass.
-
-    ``ckv [nnz, 512]`` and ``kpe [nnz, 64]`` are bfloat16 with contiguous rows; the row strides are free (multiples of 8 and 2
-    elements), so both may be columns of one ``[nnz, 576]`` projection. ``norm_weight [512]`` bfloat16, ``cos_sin [positions, 64]``
-    float32 (the 32 cosines of a position, then its sines); a token is rotated by the angles of its ``positions`` entry, in pairs
-    ``(2k, 2k + 1)`` (``interleaved``) or ``(k, k + 32)``. The normalised and the rotated row are rounded to bfloat16 once, from
-    64-bit arithmetic by way of fp32, and the cache receives the bytes that ``quantize_append_paged_mla_kv_cache`` makes of them;
-    the tables and ``check`` are that call's. A token past the end of ``cos_sin`` counts as outside the tables."""
+def _check_norm_append(ckv, kpe, norm_weight, cos_sin, batch_indices, positions, ckv_cache, ckv_sf_cache, kpe_cache, kv_indices, kv_indptr, eps,
+                       ckv_scale, kpe_scale):
+    """What the writer behind the latent projection refuses; returns the row strides of ckv and kpe."""
     _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
     if ckv.dtype != torch.bfloat16 or kpe.dtype != torch.bfloat16 or norm_weight.dtype != torch.bfloat16 or cos_sin.dtype != torch.float32:
         raise RuntimeError("ckv, kpe and norm_weight must be bfloat16 and cos_sin float32")
@@ -514,18 +507,46 @@ def norm_rope_append_paged_mla_kv_cache(ckv, kpe, norm_weight, cos_sin, batch_in
     if (batch_indices.shape != (nnz,) or positions.shape != (nnz,) or kv_indices.dim() != 1 or kv_indptr.dim() != 1
             or not (batch_indices.is_contiguous() and positions.is_contiguous() and kv_indices.is_contiguous() and kv_indptr.is_contiguous())):
         raise RuntimeError(f"batch_indices and positions must be contiguous [{nnz}], kv_indices and kv_indptr contiguous 1-D tensors")
-    dev, at = ckv_cache.device, ckv_cache.get_device()
+    at = ckv_cache.get_device()
     if (ckv.get_device() != at or kpe.get_device() != at or norm_weight.get_device() != at or cos_sin.get_device() != at
             or batch_indices.get_device() != at or positions.get_device() != at or kv_indices.get_device() != at or kv_indptr.get_device() != at):
         raise RuntimeError("inputs must be on the cache device")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    if not (ckv_scale > 0 and kpe_scale > 0):
+        raise RuntimeError("ckv_scale and kpe_scale must be positive")
+    if nnz and (ckv.data_ptr() % 16 or kpe.data_ptr() % 4 or norm_weight.data_ptr() % 16):
+        raise RuntimeError("rows of ckv and norm_weight must be 16-byte and rows of kpe 4-byte aligned")
+    return rows, pe_rows
+
+
+def _norm_append(strides, ckv, kpe, norm_weight, cos_sin, batch_indices, positions, ckv_cache, ckv_sf_cache, kpe_cache, kv_indices, kv_indptr, eps,
+                 ckv_scale, kpe_scale, interleaved, status=None):
+    """That writer, its arguments checked."""
     pages, ps = ckv_cache.shape[:2]
+    dev = ckv_cache.device
     _on_device(dev, lambda: _lib.check(_lib.load().nvfp4_mla_norm_rope_append(
-        ckv.data_ptr(), rows, kpe.data_ptr(), pe_rows, norm_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], eps, 1 if interleaved else 0,
-        batch_indices.data_ptr(), positions.data_ptr(), nnz, ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), pages, ps,
-        kv_indices.data_ptr(), kv_indptr.data_ptr(), kv_indptr.shape[0] - 1, ckv_scale, kpe_scale, _ptr(status), _raw_stream(dev))))
+        ckv.data_ptr(), strides[0], kpe.data_ptr(), strides[1], norm_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], eps,
+        1 if interleaved else 0, batch_indices.data_ptr(), positions.data_ptr(), ckv.shape[0], ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(),
+        kpe_cache.data_ptr(), pages, ps, kv_indices.data_ptr(), kv_indptr.data_ptr(), kv_indptr.shape[0] - 1, ckv_scale, kpe_scale, _ptr(status),
+        _raw_stream(dev))))
+
+
+def norm_rope_append_paged_mla_kv_cache(ckv, kpe, norm_weight, cos_sin, batch_indices, positions, ckv_cache, ckv_sf_cache, kpe_cache,
+                                        kv_indices, kv_indptr, eps=1e-6, ckv_scale=1.0, kpe_scale=1.0, interleaved=True, check=False):
+    """RMS-normalises, rotates, quantises and writes the latent projection's raw rows into the paged cache, in place and in one pass.
+
+    ``ckv [nnz, 512]`` and ``kpe [nnz, 64]`` are bfloat16 with contiguous rows; the row strides are free (multiples of 8 and 2
+    elements), so both may be columns of one ``[nnz, 576]`` projection. ``norm_weight [512]`` bfloat16, ``cos_sin [positions, 64]``
+    float32 (the 32 cosines of a position, then its sines); a token is rotated by the angles of its ``positions`` entry, in pairs
+    ``(2k, 2k + 1)`` (``interleaved``) or ``(k, k + 32)``. The normalised and the rotated row are rounded to bfloat16 once, from
+    64-bit arithmetic by way of fp32, and the cache receives the bytes that ``quantize_append_paged_mla_kv_cache`` makes of them;
+    the tables and ``check`` are that call's. A token past the end of ``cos_sin`` counts as outside the tables."""
+    strides = _check_norm_append(ckv, kpe, norm_weight, cos_sin, batch_indices, positions, ckv_cache, ckv_sf_cache, kpe_cache, kv_indices, kv_indptr, eps,
+                                 ckv_scale, kpe_scale)
+    status = torch.zeros(1, dtype=torch.int32, device=ckv_cache.device) if check else None
+    _norm_append(strides, ckv, kpe, norm_weight, cos_sin, batch_indices, positions, ckv_cache, ckv_sf_cache, kpe_cache, kv_indices, kv_indptr, eps, ckv_scale,
+                 kpe_scale, interleaved, status)
     if check and int(status.item()) != 0:
         raise RuntimeError("norm_rope_append: a token named a request, position or page outside the tables")
 

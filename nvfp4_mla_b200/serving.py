@@ -1,6 +1,6 @@
 """The callers either side of the decode path, as a serving engine would use them: a paged latent-KV pool that appends
-through the CUDA cache writer and decodes through the decode kernel, multi-token (speculative / MTP verify) decode, and
-the W_UV projection after the latent output.
+through the CUDA cache writers, attends to chunks of new tokens, decodes (over everything or a sliding window) and reads rows back, multi-token
+(speculative / MTP verify) decode, and the W_UV projection after the latent output.
 
 The reference lists these as what comes next around its kernel (README.md:88, 118-119, 414-415 of the reference
 project): it has none of them, so there is no reference code to mirror; the arithmetic is the decode path's own and is
@@ -11,7 +11,8 @@ import operator
 import numpy as np
 import torch
 
-from . import _PRECISIONS, CKV, KPE, _append, _check_append, _decode, _lib, decode
+from . import (_PRECISIONS, CKV, KPE, _append, _check_append, _check_norm_append, _decode, _lib, _norm_append, decode, decode_window, extend,
+               gather_paged_mla_kv_cache)
 
 
 def decode_multi_token(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens, sm_scale,
@@ -94,6 +95,36 @@ class PagedLatentCache:
         """Appends ``counts[i]`` new tokens to ``requests[i]``: ``requests`` is a list of ``(request, count)`` pairs and
         ``ckv [sum(counts), 512]`` / ``kpe [sum(counts), 64]`` (bfloat16) hold their latent rows in that order. A request may be
         named more than once: its shares follow each other. Whatever refuses the call does so before the pool changes."""
+        def check(*where):
+            if _check_append(ckv, kpe, *where) and (ckv.data_ptr() % 16 or kpe.data_ptr() % 4):  # (the C entry would refuse that too late)
+                raise RuntimeError("ckv must be 16-byte and kpe 4-byte aligned")
+
+        def write(nnz, *where):
+            _append(nnz, ckv, kpe, *where, self.ckv_scale, self.kpe_scale)
+
+        self._append_rows(requests, check, write)
+
+    def append_projected(self, requests, kv_a, norm_weight, cos_sin, eps=1e-6, interleaved=True):
+        """``append`` of the latent projection's raw rows ``kv_a [sum(counts), 576]`` (latent, rope): they are RMS-normalised with
+        ``norm_weight [512]``, rotated by the rows of ``cos_sin [positions, 64]`` at their places in the request, and written in one pass
+        (``norm_rope_append_paged_mla_kv_cache``). A request that would grow past the table of angles is refused."""
+        if kv_a.dim() != 2 or kv_a.shape[1] != CKV + KPE:
+            raise RuntimeError("kv_a must be [tokens, 576]")
+        ckv, kpe = kv_a[:, :CKV], kv_a[:, CKV:]
+        strides = []
+
+        def check(*where):
+            strides[:] = _check_norm_append(ckv, kpe, norm_weight, cos_sin, *where, eps, self.ckv_scale, self.kpe_scale)
+
+        def write(nnz, *where):
+            if nnz:
+                _norm_append(strides, ckv, kpe, norm_weight, cos_sin, *where, eps, self.ckv_scale, self.kpe_scale, interleaved)
+
+        self._append_rows(requests, check, write, cos_sin.shape[0])
+
+    def _append_rows(self, requests, check, write, longest=None):
+        """The bookkeeping of an append: ``check`` refuses the rows and their places before the pool changes, ``write`` writes them. No
+        request may become longer than ``longest``."""
         if not requests:
             raise IndexError("append needs at least one request")
         width, known, free, n_free, page_size = self.page_table.shape[1], len(self._lens), self._free, len(self._free), self.page_size
@@ -110,6 +141,8 @@ class PagedLatentCache:
                 to = grown[r] = [self._lens[r], len(self._pages[r]), []]
             end, held, fresh = to
             to[0] = end = end + n
+            if longest is not None and end > longest:
+                raise RuntimeError(f"request {r} would have {end} tokens, and there are angles for {longest}")
             need = -(-end // page_size) - held
             if need > 0:
                 if taken + need > n_free or held + need > width:
@@ -139,12 +172,11 @@ class PagedLatentCache:
 
         told = self._to_device(12 * n_slots + 8 * nnz, fill)
         words = told[8 * n_slots:].view(torch.int32)
-        write = (ckv, kpe, words[n_slots:n_slots + nnz], words[n_slots + nnz:], self.ckv_cache, self.ckv_sf_cache, self.kpe_cache,
+        where = (words[n_slots:n_slots + nnz], words[n_slots + nnz:], self.ckv_cache, self.ckv_sf_cache, self.kpe_cache,
                  self.page_table.view(-1), self._kv_indptr)
-        if _check_append(*write) and (ckv.data_ptr() % 16 or kpe.data_ptr() % 4):  # (the C entry would refuse that too late)
-            raise RuntimeError("ckv must be 16-byte and kpe 4-byte aligned")
+        check(*where)
         self._tables.index_copy_(0, told[:8 * n_slots].view(torch.int64), words[:n_slots])
-        _append(nnz, *write, self.ckv_scale, self.kpe_scale)
+        write(nnz, *where)
         del free[n_free - taken:]
         for r, (end, _, fresh) in grown.items():
             self._lens[r] = end
@@ -159,13 +191,67 @@ class PagedLatentCache:
         fill(staged.numpy())
         return staged.to(self.ckv_cache.device, non_blocking=True)
 
-    def decode(self, requests, q_nope, q_pe, sm_scale, w_uv=None, precision="bf16"):
+    def _named(self, ids, *more):
+        """Page-table rows and lengths of the requests ``ids`` (a list), and a device copy of each int32 array in ``more``: one copy from
+        the host."""
+        ids = np.array(ids, dtype=np.int64)
+
+        def fill(host):
+            host[:8 * ids.size].view(np.int64)[:] = ids
+            host[8 * ids.size:].view(np.int32)[:] = np.concatenate([np.asarray(m, dtype=np.int32) for m in more]) if more else 0
+
+        told = self._to_device(8 * ids.size + 4 * sum(len(m) for m in more), fill)
+        idx, words, out, at = told[:8 * ids.size].view(torch.int64), told[8 * ids.size:].view(torch.int32), [], 0
+        for m in more:
+            out.append(words[at:at + len(m)])
+            at += len(m)
+        return (self.page_table.index_select(0, idx), self.kv_lens.index_select(0, idx), *out)
+
+    def _known(self, request):
+        """The request's index; a negative id counts from the end."""
+        return range(len(self._lens))[operator.index(request)]
+
+    def extend(self, requests, q_nope, q_pe, sm_scale, w_uv=None, window=0, sink_tokens=0):
+        """Attention of the chunks that were appended last: ``requests`` is a list of ``(request, count)`` pairs as for ``append`` (each
+        request once), ``q_nope [sum(counts), heads, 512]`` and ``q_pe [sum(counts), heads, 64]`` are the queries of each request's last
+        ``count`` tokens. Causal, with ``window`` and ``sink_tokens`` as in ``nvfp4_mla_b200.extend``. Returns ``[sum(counts), heads, 512]``, or with
+        ``w_uv`` the value-space output as in ``decode``."""
+        if not requests:
+            raise IndexError("extend needs at least one request")
+        ids, counts = [self._known(r) for r, _ in requests], [operator.index(n) for _, n in requests]
+        if len(set(ids)) < len(ids):
+            raise ValueError("a request is named twice: its chunk is one run of tokens")
+        for r, n in zip(ids, counts):
+            if not 0 <= n <= self._lens[r]:
+                raise ValueError(f"request {r} holds {self._lens[r]} tokens, its chunk {n}")
+        if sum(counts) != q_nope.shape[0]:
+            raise RuntimeError(f"q_nope must hold the {sum(counts)} tokens of the chunks, it has {q_nope.shape[0]}")
+        table, lens, indptr = self._named(ids, np.concatenate([[0], np.cumsum(counts)]))
+        out = extend(q_nope, q_pe, self.ckv_cache, self.ckv_sf_cache, self.kpe_cache, table, lens, indptr, sm_scale, self.ckv_scale, self.kpe_scale,
+                     max_kv_len=max(self._lens[r] for r in ids), window=window, sink_tokens=sink_tokens)
+        return out if w_uv is None else torch.einsum("bhc,hcv->bhv", out, w_uv.to(out.dtype))
+
+    def gather(self, ranges, dtype=torch.bfloat16):
+        """Rows of the pool, dequantised: ``ranges`` is a list of ``(request, start, count)``; returns ``(ckv [sum(counts), 512], kpe
+        [sum(counts), 64])`` in that order (``gather_paged_mla_kv_cache``)."""
+        ids, starts, counts = [self._known(r) for r, _, _ in ranges], [operator.index(s) for _, s, _ in ranges], [operator.index(n) for _, _, n in ranges]
+        for r, s, n in zip(ids, starts, counts):
+            if s < 0 or n < 0 or s + n > self._lens[r]:
+                raise ValueError(f"request {r} holds {self._lens[r]} tokens, not [{s}, {s + n})")
+        table, _, first, indptr = self._named(ids, starts, np.concatenate([[0], np.cumsum(counts)]))
+        return gather_paged_mla_kv_cache(self.ckv_cache, self.ckv_sf_cache, self.kpe_cache, table, indptr, sum(counts), first, self.ckv_scale,
+                                         self.kpe_scale, dtype)
+
+    def decode(self, requests, q_nope, q_pe, sm_scale, w_uv=None, precision="bf16", window=0, sink_tokens=0):
         """One decode step for ``requests`` (a list of request ids): ``q_nope [len(requests), heads, 512]``,
         ``q_pe [len(requests), heads, 64]``. Returns the latent output ``[n, heads, 512]``, or, with
         ``w_uv [heads, 512, v_head_dim]``, the value-space output ``[n, heads, v_head_dim]`` (the absorbed W_UV applied
-        after attention)."""
+        after attention). With ``window > 0`` (16-bit precision) a request attends to its last ``window`` and its first ``sink_tokens``
+        tokens."""
         if precision not in _PRECISIONS:
             raise ValueError(f"precision must be one of {list(_PRECISIONS)}, got {precision!r}")
+        if window and precision != "bf16":
+            raise ValueError("a window needs precision 'bf16'")
         longest = 0  # (the bound is the pool's capacity: by itself it would choose the kernel for long requests)
         if torch.is_tensor(requests):
             table, lens = self.page_table[requests.to(self.page_table.device)], self.kv_lens[requests.to(self.page_table.device)]
@@ -187,6 +273,10 @@ class PagedLatentCache:
             else:  # a mask over all requests; what is neither ids nor a mask is refused by the indexing
                 idx = ids.to(self.page_table.device)
                 table, lens = self.page_table[idx].contiguous(), self.kv_lens[idx].contiguous()
+        if window:
+            out = decode_window(q_nope, q_pe, self.ckv_cache, self.ckv_sf_cache, self.kpe_cache, table, lens, sm_scale, window, sink_tokens, self.ckv_scale,
+                                self.kpe_scale, max_kv_len=longest or None)
+            return out if w_uv is None else torch.einsum("bhc,hcv->bhv", out, w_uv.to(out.dtype))
         out = _decode(q_nope, q_pe, self.ckv_cache, self.ckv_sf_cache, self.kpe_cache, table, lens, sm_scale, self.ckv_scale, self.kpe_scale,
                       self.max_kv_len, 0, _PRECISIONS[precision], True, False, expected_kv_len=longest)[0]
         return out if w_uv is None else torch.einsum("bhc,hcv->bhv", out, w_uv.to(out.dtype))
