@@ -108,8 +108,8 @@ NVFP4_MLA_API int nvfp4_mla_decode_multi(const void* q_nope, const void* q_pe, c
  *                     workspace's first word receives them
  *   workspace         at least nvfp4_mla_decode_window_workspace_bytes() bytes, 256-byte aligned; nothing in it is kept between calls
  *
- * What is read and multiplied is the visible tokens, in whole pages. Kernels launched: one more than nvfp4_mla_decode's. (No
- * counterpart in the reference.) */
+ * What is read and multiplied is the visible tokens, in whole pages. With many heads the call takes the form of nvfp4_mla_extend where
+ * that is estimated to be faster and only `out` is asked for. (No counterpart in the reference.) */
 NVFP4_MLA_API int64_t nvfp4_mla_decode_window_workspace_bytes(int batch, int heads, int page_size, int page_table_width, int max_kv_len,
                                                               int window, int sink_tokens);
 NVFP4_MLA_API int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,

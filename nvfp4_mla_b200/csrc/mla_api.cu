@@ -266,6 +266,7 @@ int problem_of(int batch, int heads, int max_kv_len, int num_splits, int n_cta, 
   const long long chunk = ((len + splits - 1) / splits + mla::TILE - 1) / mla::TILE * mla::TILE;
   pb->batch = batch, pb->heads = heads, pb->heads_per_cta = hpc, pb->head_groups = (heads + hpc - 1) / hpc;
   pb->splits = splits, pb->chunk = int(chunk), pb->n_cta = n_cta;
+  pb->window = 0, pb->sinks = 0, pb->page_shift = 0, pb->pt_width = 0;
   MLA_CHECK((long long)batch * splits <= mla::kSchedMaxBZ, "batch * num_splits = %lld exceeds %d", (long long)batch * splits,
             mla::kSchedMaxBZ);
   MLA_CHECK(splits + n_cta <= 512, "num_splits %d too large (at most %d)", splits, 512 - n_cta);
@@ -328,21 +329,23 @@ int64_t nvfp4_mla_decode_workspace_bytes(int batch, int heads, int num_splits) {
 
 // The decode call proper; `heads` counts the rows of all q_len query tokens of a request, `hpc_limit` caps the heads per CTA
 // (see heads_per_cta), which are chosen for requests of `expected_kv_len` tokens (0: of the bound max_kv_len). `dead`: the tokens of
-// each request that are not seen (windowed decode, 16-bit mode), or null; `status`: where the kernels report, or null for the
+// each request that are not seen (kernels with WINDOW, 16-bit mode), or null; `window`: a sliding window, the page table's width with it;
+// `status`: where the kernels report, or null for the
 // workspace's first word.
 static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
                        const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table,
                        int64_t page_table_stride, const int32_t* kv_lens, int batch, int heads, float sm_scale, float ckv_scale,
                        float kpe_scale, int max_kv_len, int num_splits, int precision, void* out, float* out_f32, float* lse,
                        void* workspace, int64_t workspace_bytes, void* stream, int hpc_limit, int q_len = 1, int expected_kv_len = 0,
-                       const int2* dead = nullptr, int* status = nullptr) {
+                       const int2* dead = nullptr, int* status = nullptr, int window = 0, int sinks = 0, int pt_width = 0) {
   g_error[0] = 0;
   MLA_CHECK(precision == NVFP4_MLA_PRECISION_BF16 || precision == NVFP4_MLA_PRECISION_FP8,
             "precision must be 0 (bf16) or 1 (fp8), got %d", precision);
   MLA_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0, "page_size must be a power of two, got %d", page_size);
   MLA_CHECK(num_pages > 0 && num_pages * page_size < (int64_t(1) << 31), "num_pages * page_size must be in [1, 2^31)");
   MLA_CHECK(ckv_scale > 0.f && kpe_scale > 0.f, "ckv_scale and kpe_scale must be positive");
-  MLA_CHECK(q_nope && q_pe && ckv_cache && ckv_sf_cache && kpe_cache && page_table && kv_lens && workspace, "null pointer argument");
+  MLA_CHECK(q_nope && q_pe && ckv_cache && ckv_sf_cache && kpe_cache && (page_table || (window > 0 && pt_width == 0)) && kv_lens && workspace,
+            "null pointer argument");
   MLA_CHECK(out || out_f32 || lse, "at least one of out, out_f32 and lse must be given");
   MLA_CHECK(aligned(q_nope, 16) && aligned(q_pe, 16) && aligned(ckv_cache, 16) && aligned(ckv_sf_cache, 16) &&
                 aligned(kpe_cache, 16) && aligned(workspace, 256) && aligned(out, 16) && aligned(out_f32, 16),
@@ -354,6 +357,8 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   const int hpc = heads_per_cta(heads, precision, *d, hpc_limit, batch, expected_kv_len > 0 ? expected_kv_len : max_kv_len);
   if (problem_of(batch, heads, max_kv_len, num_splits, schedule_units(*d, precision, hpc), hpc, &pb)) return 1;
   if (batch == 0) return 0;
+  if (window > 0) pb.window = window, pb.sinks = sinks, pb.page_shift = __builtin_ctz(unsigned(page_size)), pb.pt_width = pt_width;
+  const bool windowed = dead || window > 0;
   const mla::WsLayout L = mla::ws_layout(pb.n_cta, pb.items(), pb.heads_per_cta);
   MLA_CHECK(workspace_bytes >= int64_t(L.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes,
             (long long)L.total);
@@ -398,9 +403,9 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   if (prof) MLA_CUDA(cudaEventRecord(prof->start[prof->used], st));
   const dim3 grid(pb.n_cta * ctas_per_unit(hpc)), block(decode_threads(precision, hpc));
   if (hm16)
-    MLA_CUDA(launch_dependent(hm16_kernel(dead != nullptr), grid, block, decode_smem(precision, hpc), st, P));
+    MLA_CUDA(launch_dependent(hm16_kernel(windowed), grid, block, decode_smem(precision, hpc), st, P));
   else
-    MLA_CUDA(launch_dependent_cluster(decode_kernel(precision, hpc, dead != nullptr), grid, block, decode_smem(precision, hpc), st,
+    MLA_CUDA(launch_dependent_cluster(decode_kernel(precision, hpc, windowed), grid, block, decode_smem(precision, hpc), st,
                                       unsigned(ctas_per_unit(hpc)), ckv_map, sf_map, kpe_map, P));
   if (prof) MLA_CUDA(cudaEventRecord(prof->stop[prof->used++], st));
 
@@ -460,8 +465,8 @@ int nvfp4_mla_decode_multi(const void* q_nope, const void* q_pe, const uint8_t* 
                      workspace, workspace_bytes, stream, 128, q_len);
 }
 
-// ---- windowed decode ------------------------------------------------------------------------------------------------
-// Workspace: the decode call's | page table of the visible pages | lengths | gaps
+// ---- a few query tokens as requests ------------------------------------------------------------------------------------
+// Workspace: the decode call's | page tables of the visible pages | lengths | unseen intervals
 namespace {
 struct WindowLayout {
   size_t decode, table, lens, dead, total;
@@ -750,18 +755,9 @@ int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, const uint8_t*
     return nvfp4_mla_extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, page_table, page_table_stride, page_table_width,
                             kv_lens, nullptr, batch, batch, heads, sm_scale, ckv_scale, kpe_scale, max_kv_len, window, sink_tokens, out, workspace,
                             workspace_bytes, status, stream);
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  int* table = reinterpret_cast<int*>(ws + l.table);
-  int* lens = reinterpret_cast<int*>(ws + l.lens);
-  int2* dead = reinterpret_cast<int2*>(ws + l.dead);
-  constexpr int per_block = mla::kWindowThreads / 32;
-  mla::mla_window_plan_kernel<<<unsigned((batch + per_block - 1) / per_block), mla::kWindowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      page_table, page_table_stride, page_table_width, kv_lens, mla::ChunkTokens{nullptr, batch, 0}, batch, __builtin_ctz(unsigned(page_size)),
-      window, sink_tokens, l.width, table, lens, dead);
-  MLA_CUDA(cudaGetLastError());
-  return decode_impl(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, table, l.width, lens, batch, heads, sm_scale,
-                     ckv_scale, kpe_scale, l.max_len, 0, NVFP4_MLA_PRECISION_BF16, out, out_f32, lse, workspace, int64_t(l.table), stream, 128,
-                     1, 0, dead, status);
+  return decode_impl(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, page_table, page_table_stride, kv_lens, batch, heads,
+                     sm_scale, ckv_scale, kpe_scale, l.max_len, 0, NVFP4_MLA_PRECISION_BF16, out, out_f32, lse, workspace, int64_t(l.table), stream,
+                     128, 1, 0, nullptr, status, window, sink_tokens, page_table_width);
 }
 
 // ---- decode without caller-provided scratch -----------------------------------------------------------------------

@@ -47,13 +47,44 @@ __host__ __device__ inline WsLayout ws_layout(int n_cta, long long W, int heads_
 // neighbours in the flattened tile order and re-read the same KV range close together in time.
 struct Problem {
   int batch, heads, heads_per_cta, head_groups, splits, chunk, n_cta;
+  int window, sinks, page_shift, pt_width;  // windowed decode (window 0: none; splits 1): see WindowMap; pt_width: columns of the page table
   __host__ __device__ long long items() const { return (long long)batch * splits * head_groups; }
 };
+
+// Sliding-window decode. The query token of a request of n tokens sees the first S tokens and the last W: [0, S) and [n - W, n).
+// Attention does not care about the numbering of the tokens, so the kernels get a shorter request instead of a second range: the
+// first tokens' pages followed by the window's, the number of tokens up to the end of that, and the one interval of it that is not
+// seen (what is left of the last of the first tokens' pages, and of the window's first page before the window begins). Everything
+// that schedules, loads and multiplies then works on visible pages alone; the kernels mask the interval.
+struct WindowMap {
+  int len;             // tokens of the shortened request
+  int first, skipped;  // pages: the first tokens' ones, and how many follow them that are left out
+  int2 dead;           // tokens of the shortened request that are not seen
+  __device__ __forceinline__ int page(int i) const { return i < first ? i : i + skipped; }  // of the request, for page i of the shortened one
+};
+__device__ __forceinline__ WindowMap window_map(int n, int window, int sinks, int page_shift) {
+  const int begin = window > 0 && n > window ? n - window : 0;  // first token of the window
+  WindowMap m;
+  m.first = int(((long long)sinks + (1ll << page_shift) - 1) >> page_shift);
+  m.skipped = (begin >> page_shift) > m.first ? (begin >> page_shift) - m.first : 0;
+  m.len = n - (m.skipped << page_shift);
+  m.dead = begin > sinks ? make_int2(sinks, begin - (m.skipped << page_shift)) : make_int2(0, 0);
+  return m;
+}
+__device__ __forceinline__ WindowMap window_map(const int* kv_lens, const Problem& pb, int b) {
+  const long long most = (long long)pb.pt_width << pb.page_shift;  // a length past the page table is cut at its end
+  const int n = kv_lens[b];
+  return window_map(n < most ? n : int(most), pb.window, pb.sinks, pb.page_shift);
+}
+// tokens of request b that are scheduled
+__device__ __forceinline__ int sched_len(const int* kv_lens, const Problem& pb, int b) {
+  return pb.window > 0 ? window_map(kv_lens, pb, b).len : kv_lens[b];
+}
 
 // 128-token tiles of (request, split) pair bz = b * splits + z: the split covers tokens [z * chunk, (z + 1) * chunk) of the request.
 __device__ __forceinline__ int sched_tiles(const int* kv_lens, const Problem& pb, int bz) {
   const int b = bz / pb.splits, z = bz % pb.splits;
-  long long n = (long long)kv_lens[b] - (long long)z * pb.chunk;
+  long long n = (long long)sched_len(kv_lens, pb, b) - (long long)z * pb.chunk;
   n = n < 0 ? 0 : (n > pb.chunk ? pb.chunk : n);
   return int((n + TILE - 1) / TILE);
 }

@@ -84,10 +84,11 @@ __device__ __forceinline__ bool h16_wait_converted(H16Smem& s, uint32_t tiles) {
   }
   return true;
 }
-__device__ __forceinline__ void h16_prefetch_rows(const DecodeParams& P, const Seg& seg, int t, int cg, int lane) {
+template <bool WINDOW>
+__device__ __forceinline__ void h16_prefetch_rows(const DecodeParams& P, const Seg& seg, const WindowMap& win, int t, int cg, int lane) {
   const int tok = seg.tok0 + t * kH16Tile + kH16Own * cg + lane;
   if (tok >= seg.tok_end) return;
-  const int page = P.page_table[(long long)seg.b * P.pt_stride + (tok >> P.page_shift)];
+  const int pi = tok >> P.page_shift, page = P.page_table[(long long)seg.b * P.pt_stride + (WINDOW ? win.page(pi) : pi)];
   if (uint32_t(page) >= uint32_t(P.num_pages)) return;
   const int in_page = tok & ((1 << P.page_shift) - 1);
   const long long row = ((long long)page << P.page_shift) + in_page;
@@ -99,18 +100,21 @@ __device__ __forceinline__ void h16_prefetch_rows(const DecodeParams& P, const S
     ptx::bulk_prefetch_l2(P.sf + row * 32, run * 32);
   }
 }
+template <bool WINDOW>
 __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams& P, int n_segs, uint32_t& it, int cg) {
   const int lane = ptx::lane_id();
   for (int si = 0; si < n_segs; ++si) {
     const Seg seg = s.segs[si];
     const int nt = h16_tiles(seg);
     if (nt <= 0) continue;
+    WindowMap win;
+    if constexpr (WINDOW) win = seg_window(P, seg.b);
     if (it == 0)
-      for (int t = 1; t < kH16Ahead && t < nt; ++t) h16_prefetch_rows(P, seg, t, cg, lane);
+      for (int t = 1; t < kH16Ahead && t < nt; ++t) h16_prefetch_rows<WINDOW>(P, seg, win, t, cg, lane);
     const int t_next = nt > kH16Ahead ? nt - kH16Ahead : 0;
     for (int t = 0; t < nt; ++t, ++it) {
       if (!__all_sync(~0u, h16_wait_converted(s, it))) return;
-      if (t + kH16Ahead < nt) h16_prefetch_rows(P, seg, t + kH16Ahead, cg, lane);
+      if (t + kH16Ahead < nt) h16_prefetch_rows<WINDOW>(P, seg, win, t + kH16Ahead, cg, lane);
       if (t == t_next)  // the next segment's query rows and first tiles
         for (int sj = si + 1; sj < n_segs; ++sj) {
           const Seg nx = s.segs[sj];
@@ -121,7 +125,9 @@ __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams
           for (int i = lane; i < nr * 9; i += 32)
             ptx::prefetch_l2(i < nr * 8 ? reinterpret_cast<const char*>(P.q_nope + row0 * CKV) + i * 128
                                         : reinterpret_cast<const char*>(P.q_pe + row0 * KPE) + (i - nr * 8) * 128);
-          for (int t2 = 0; t2 < kH16Ahead && t2 < nn; ++t2) h16_prefetch_rows(P, nx, t2, cg, lane);
+          WindowMap nx_win;
+          if constexpr (WINDOW) nx_win = seg_window(P, nx.b);
+          for (int t2 = 0; t2 < kH16Ahead && t2 < nn; ++t2) h16_prefetch_rows<WINDOW>(P, nx, nx_win, t2, cg, lane);
           break;
         }
     }
@@ -159,7 +165,9 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
     const int nt = h16_tiles(seg);
     if (nt <= 0) continue;
     const int* pt = P.page_table + (long long)seg.b * P.pt_stride;
-    const int2 dead = WINDOW ? P.dead[seg.b] : make_int2(0, 0);  // tokens that no row sees: they read as zeros
+    WindowMap win;
+    if constexpr (WINDOW) win = seg_window(P, seg.b);
+    const int2 dead = WINDOW ? win.dead : make_int2(0, 0);  // tokens that no row sees: they read as zeros
     const int first_masked = P.q_len > 1 ? P.kv_lens[seg.b] - (P.q_len - 1) : INT_MAX;  // first token that some row does not see
     uint4 rw[2];
     uint32_t rs[2];
@@ -169,7 +177,10 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
     // No load sits behind a branch (it would be waited for where the branches meet, one trip to memory per load instead of
     // one per tile): tokens past the end look up the last live token's page, dead rows read cache row 0 and are zeroed where
     // their bytes are used, and the fetches past the last tile are issued like the others.
-    auto fetch_id = [&](int tk) { return __ldg(pt + ((tk < seg.tok_end ? tk : seg.tok_end - 1) >> P.page_shift)); };
+    auto fetch_id = [&](int tk) { 
+      const int pi = (tk < seg.tok_end ? tk : seg.tok_end - 1) >> P.page_shift;
+      return __ldg(pt + (WINDOW ? win.page(pi) : pi));
+    };
     auto fetch_rows = [&](int page) {
       const bool live = tok < seg.tok_end, good = uint32_t(page) < uint32_t(P.num_pages);
       // a stale or corrupt id is never dereferenced: the row reads as zeros and the call is flagged
@@ -379,7 +390,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
     // A row sees the tokens up to its own query token: token i of q_len (rows [i, i + 1) * heads / q_len of the request) stops
     // q_len - 1 - i tokens before the request's end.
     int row_end = seg.tok_end;
-    const int2 dead = WINDOW ? P.dead[seg.b] : make_int2(0, 0);
+    const int2 dead = WINDOW ? seg_window(P, seg.b).dead : make_int2(0, 0);
     if (P.q_len > 1) {
       const int i = (r0 + hq) / (P.heads / P.q_len), end = P.kv_lens[seg.b] - (P.q_len - 1 - i);
       row_end = end < row_end ? end : row_end;
@@ -601,7 +612,7 @@ __device__ __forceinline__ void h16_run_role(H16Smem& s, const DecodeParams& P) 
     if (ROLE == kH16Softmax) h16_softmax_role<WINDOW>(s, P, n_segs, it, cg);
     if (ROLE == kH16Convert) h16_convert_role<WINDOW>(s, P, n_segs, it, cg);
     if (ROLE == kH16Qk) h16_qk_role(s, P, n_segs, it, seg_count, cg);
-    if (ROLE == kH16Prefetch) h16_prefetch_role(s, P, n_segs, it, cg);
+    if (ROLE == kH16Prefetch) h16_prefetch_role<WINDOW>(s, P, n_segs, it, cg);
     if (ROLE == kH16Pv) h16_pv_role(s, P, n_segs, it, cg);
     __syncthreads();
     if (s.abort_flag) break;

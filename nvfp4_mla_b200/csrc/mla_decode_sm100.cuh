@@ -76,8 +76,15 @@ struct DecodeParams {
   int2* item_range;  // written by the CTA that holds an item's first tile (read by the combine kernel)
   int2* cta_range_out;
   Seg* segs_out;
-  const int2* dead;  // windowed decode: tokens [x, y) of the request are not seen (kernels with WINDOW only)
+  const int2* dead;  // kernels with WINDOW: tokens [x, y) of the request are not seen; null: as pb's window says
 };
+// the window of request b, in a kernel with WINDOW
+__device__ __forceinline__ WindowMap seg_window(const DecodeParams& P, int b) {
+  if (!P.dead) return window_map(P.kv_lens, P.pb, b);
+  WindowMap m;
+  m.len = 0, m.first = 0, m.skipped = 0, m.dead = P.dead[b];
+  return m;
+}
 
 // ---------------------------------------------------------------------------------------------------------------
 // The schedule, derived by every decode CTA (or CTA pair: `unit`) for itself, so that no schedule kernel runs in
@@ -137,7 +144,7 @@ __device__ __forceinline__ void publish_own_schedule(int* scratch, const DecodeP
       const uint32_t lo = (g0 > Pw ? g0 : Pw) - Pw, hi = (g0 + q < Pw + tw ? g0 + q : Pw + tw) - Pw;
       if (hi > lo) {
         if (lo == 0) P.item_range[w] = make_int2(unit, int((Pw + tw - 1) / q));
-        const int len = P.kv_lens[b];
+        const int len = sched_len(P.kv_lens, P.pb, b);
         const long long end = (long long)(z + 1) * P.pb.chunk;
         g.tok0 = z * P.pb.chunk + int(lo) * TILE, g.ntiles = int(hi - lo), g.tok_end = int(end < len ? end : len);
       }

@@ -100,6 +100,7 @@ constexpr size_t vt_smem_bytes() { return sizeof(VtSmem) + 1024; }
 // ---------------------------------------------------------------------------------------------------------------
 // role: TMA producer (one warp; lane 0 issues, all lanes help with the page ids of small pages)
 // ---------------------------------------------------------------------------------------------------------------
+template <bool WINDOW>
 __device__ __forceinline__ void vt_producer_role(VtSmem& s, const DecodeParams& P, const CUtensorMap* ckv_map, const CUtensorMap* sf_map,
                                                  const CUtensorMap* kpe_map, int n_segs, uint32_t& it) {
   const int lane = ptx::lane_id();
@@ -108,6 +109,9 @@ __device__ __forceinline__ void vt_producer_role(VtSmem& s, const DecodeParams& 
     const Seg seg = s.segs[si];
     if (seg.ntiles <= 0) continue;
     const int* pt = P.page_table + (long long)seg.b * P.pt_stride;
+    WindowMap win;
+    if constexpr (WINDOW) win = seg_window(P, seg.b);
+    auto page_id = [&](int i) { return pt[WINDOW ? win.page(i) : i]; };
     // page ids of a tile's two half tiles and of the two that are prefetched into L2 (three tiles ahead: the ring itself
     // is too shallow to cover HBM latency); read one tile ahead of their use so that nothing ever waits for them
     auto fetch_ids = [&](int tk0, int (&pg)[2], int (&pf)[2]) {
@@ -116,8 +120,8 @@ __device__ __forceinline__ void vt_producer_role(VtSmem& s, const DecodeParams& 
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int tk = tk0 + h * HALF;
-          if (tk < seg.tok_end) pg[h] = pt[tk >> P.page_shift];
-          if (tk + 3 * TILE < seg.tok_end) pf[h] = pt[(tk + 3 * TILE) >> P.page_shift];
+          if (tk < seg.tok_end) pg[h] = page_id(tk >> P.page_shift);
+          if (tk + 3 * TILE < seg.tok_end) pf[h] = page_id((tk + 3 * TILE) >> P.page_shift);
         }
       }
     };
@@ -186,7 +190,7 @@ __device__ __forceinline__ void vt_producer_role(VtSmem& s, const DecodeParams& 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int pi = lane + 32 * k;
-          page[k] = pi < npages ? pt[(tok >> P.page_shift) + pi] : -1;
+          page[k] = pi < npages ? page_id((tok >> P.page_shift) + pi) : -1;
           const bool ok_page = pi < npages && uint32_t(page[k]) < uint32_t(P.num_pages);
           if (pi < npages && !ok_page) atomicExch(P.header, int(kBadPage));
           if (!ok_page) page[k] = -1;
@@ -440,7 +444,7 @@ __device__ __forceinline__ void vt_k_role(VtSmem& s, const DecodeParams& P, int 
     if (!vt_load_query(s, P, seg, quad * 32 + lane, seg_count & 3, lane, quad, dead, it != 0, &s.k_free[(it - 1) & 1], ((it - 1) >> 1) & 1))
       return;
     ++seg_count;
-    const int2 gap = WINDOW ? P.dead[seg.b] : make_int2(0, 0);
+    const int2 gap = WINDOW ? seg_window(P, seg.b).dead : make_int2(0, 0);
     for (int t = 0; t < seg.ntiles; ++t, ++it) {
       if (!vt_k_step<WINDOW>(s, P, seg, gap, t, it, lane, quad)) {
         dead = true;
@@ -654,7 +658,7 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
     if (seg.ntiles <= 0) continue;
     const int par_q = seg_count & 3;
     ++seg_count;
-    const int2 dead = WINDOW ? P.dead[seg.b] : make_int2(0, 0);
+    const int2 dead = WINDOW ? seg_window(P, seg.b).dead : make_int2(0, 0);
     // running maximum and sum per head. The maximum starts at a finite sentinel far below any score rather than at
     // -inf: x - m and m - m' then never meet inf - inf, and no special case is needed anywhere below.
     constexpr float kNoMax = -1e30f;
@@ -828,7 +832,7 @@ __device__ __forceinline__ void vt_run_role(VtSmem& s, const DecodeParams& P, co
     if (ROLE == kVtK) vt_k_role<WINDOW>(s, P, n_segs, it, seg_count);
     if (ROLE == kVtV) vt_v_role(s, P, n_segs, it, (uint32_t(threadIdx.x) >> 7) - 2);
     if (ROLE == kVtQk) vt_qk_role(s, P, n_segs, it);
-    if (ROLE == kVtProducer) vt_producer_role(s, P, ckv_map, sf_map, kpe_map, n_segs, it);
+    if (ROLE == kVtProducer) vt_producer_role<WINDOW>(s, P, ckv_map, sf_map, kpe_map, n_segs, it);
     if (ROLE == kVtPv) vt_pv_role(s, P, n_segs, it);
     __syncthreads();
     if (s.abort_flag) break;

@@ -37,7 +37,7 @@ mla_schedule_kernel(const int* __restrict__ kv_lens, Problem pb, int* header, in
     int t = 0;
     if (bz < BZ) {
       const int b = bz / pb.splits, z = bz % pb.splits;
-      const int len = kv_lens[b];
+      const int len = sched_len(kv_lens, pb, b);
       const long long lo = (long long)z * pb.chunk;
       long long n = (long long)len - lo;
       n = n < 0 ? 0 : (n > pb.chunk ? pb.chunk : n);
@@ -115,7 +115,7 @@ mla_schedule_kernel(const int* __restrict__ kv_lens, Problem pb, int* header, in
     const long long P = (long long)HG * prefix(bz) + (long long)hg * t;
     const int c0 = int(P / q), c1 = int((P + t - 1) / q);
     item_range[w] = make_int2(c0, c1);
-    const int len = kv_lens[b];
+    const int len = sched_len(kv_lens, pb, b);
     const long long end = (long long)(z + 1) * pb.chunk;
     for (int c = c0; c <= c1; ++c) {
       const long long lo = ((long long)c * q > P ? (long long)c * q : P) - P;
