@@ -28,19 +28,21 @@ def _ptr(t):
 
 def _check_cache(ckv, sf, kpe):
     """The reference's check_cache (nvfp4_mla/csrc/mla_decode.cu:970-982), same messages."""
-    if not (ckv.is_cuda and sf.device == ckv.device and kpe.device == ckv.device):
+    at = ckv.get_device()
+    if not (ckv.is_cuda and sf.get_device() == at and kpe.get_device() == at):
         raise RuntimeError("caches must be on the same CUDA device")
     if ckv.dtype != torch.uint8:
         raise RuntimeError("ckv_cache must be uint8 (packed E2M1)")
     if sf.dtype != torch.float8_e4m3fn or kpe.dtype != torch.float8_e4m3fn:
         raise RuntimeError("ckv_sf_cache and kpe_cache must be float8_e4m3fn")
-    if ckv.dim() != 3 or ckv.shape[2] != CKV // 2:
+    shape, sf_shape, kpe_shape = ckv.shape, sf.shape, kpe.shape
+    if len(shape) != 3 or shape[2] != CKV // 2:
         raise RuntimeError("ckv_cache must be [pages, page_size, 256]")
-    if sf.dim() != 3 or sf.shape[2] != CKV // 16:
+    if len(sf_shape) != 3 or sf_shape[2] != CKV // 16:
         raise RuntimeError("ckv_sf_cache must be [pages, page_size, 32]")
-    if kpe.dim() != 3 or kpe.shape[2] != KPE:
+    if len(kpe_shape) != 3 or kpe_shape[2] != KPE:
         raise RuntimeError("kpe_cache must be [pages, page_size, 64]")
-    if sf.shape[:2] != ckv.shape[:2] or kpe.shape[:2] != ckv.shape[:2]:
+    if sf_shape[0] != shape[0] or kpe_shape[0] != shape[0] or sf_shape[1] != shape[1] or kpe_shape[1] != shape[1]:
         raise RuntimeError("ckv_cache, ckv_sf_cache and kpe_cache must have the same [pages, page_size]")
     if not (ckv.is_contiguous() and sf.is_contiguous() and kpe.is_contiguous()):
         raise RuntimeError("caches must be contiguous")
@@ -193,7 +195,8 @@ def _check_page_table(page_table):
 
 def _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale):
     """What the calls below refuse of queries and tables; ``(query tokens, heads, requests, page size, page-table width)``."""
-    if q_nope.dim() != 3 or q_nope.shape[2] != CKV or q_pe.shape != (q_nope.shape[0], q_nope.shape[1], KPE):
+    shape = q_nope.shape
+    if len(shape) != 3 or shape[2] != CKV or q_pe.shape != (shape[0], shape[1], KPE):
         raise RuntimeError("q_nope must be [tokens, heads, 512] and q_pe [tokens, heads, 64]")
     if q_nope.dtype != torch.bfloat16 or q_pe.dtype != torch.bfloat16:
         raise RuntimeError("q must be bfloat16")
@@ -209,7 +212,7 @@ def _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_
     ps = ckv_cache.shape[1]
     if ps & (ps - 1):
         raise RuntimeError("page_size must be a power of two")
-    return q_nope.shape[0], q_nope.shape[1], B, ps, width
+    return shape[0], shape[1], B, ps, width
 
 
 def _check_window(window, sink_tokens):
