@@ -510,7 +510,6 @@ struct ExtendLayout {
 // more memory than there is. 7 million tokens.
 constexpr int64_t kExtTokenBytes = int64_t(8) << 30;
 int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window, int sinks, const DeviceInfo& d, ExtendLayout* l) {
-  MLA_CHECK(batch <= mla::kExtMaxBatch, "at most %d requests, got %d", mla::kExtMaxBatch, batch);
   MLA_CHECK(int64_t(total_q) * heads < (int64_t(1) << 31) - mla::kExtRows, "total_q * heads must be below 2^31");
   const int64_t len = max_kv_len > 1 ? max_kv_len : 1;
   auto blocks_of = [&](int64_t requests) {
@@ -522,7 +521,7 @@ int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window,
     return blocks;
   };
   constexpr int64_t block_bytes = int64_t(mla::kExtBlock) * mla::kExtRow * 2;
-  l->group = batch;
+  l->group = std::min(batch, mla::kExtMaxBatch);
   while (l->group > 1 && blocks_of(std::min(l->group, total_q)) * block_bytes > kExtTokenBytes) l->group = (l->group + 1) / 2;
   const int64_t requests = std::min(l->group, total_q), blocks = blocks_of(requests);  // (at most total_q requests have query tokens)
   const int64_t items = requests + int64_t(total_q) * heads / mla::kExtRows;

@@ -31,7 +31,8 @@ constexpr int kExtRows = 128;   // rows of an item
 constexpr int kExtBlock = 64;   // tokens of a block
 constexpr int kExtTile = 256;   // tokens of a tile
 constexpr int kExtRow = CKV + KPE;
-constexpr int kExtMaxBatch = 8192;
+constexpr int kExtMaxBatch = 2048;  // requests at a time
+constexpr int kExtHeld = 4096;      // items whose tile counts the schedule kernel keeps in shared memory
 constexpr int kExtMaxPairs = 128;
 
 struct ExtItem {
@@ -126,7 +127,8 @@ __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
 }
 
 __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kernel(const ExtProblem E) {
-  __shared__ int item0[kExtMaxBatch + 1];
+  __shared__ int item0[kExtMaxBatch];
+  __shared__ int2 held[kExtHeld];        // {prefix, tiles} of an item
   __shared__ int sums[33];
   __shared__ int cut[kExtMaxPairs + 1];  // tiles of the rest before pair p
   __shared__ int rounds_s;
@@ -195,10 +197,12 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
     if (i < items) {
       m.prefix = total + incl - m.ntiles;
       E.items[i] = m;
+      if (i < kExtHeld) held[i] = make_int2(m.prefix, m.ntiles);
     }
     total += all;
   }
   __syncthreads();
+  auto tiles_of = [&](int i) { return i < kExtHeld ? held[i] : make_int2(E.items[i].prefix, E.items[i].ntiles); };
 
   // ---- rounds of whole items
   const int share = total > 0 ? (total + E.pairs - 1) / E.pairs : 1, most = items / E.pairs;
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
     for (int k = 0; k < rounds; k += kAhead) {
       int n[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) n[j] = k + j < rounds ? E.items[tid + (k + j) * E.pairs].ntiles : 0;
+      for (int j = 0; j < kAhead; ++j) n[j] = k + j < rounds ? tiles_of(tid + (k + j) * E.pairs).y : 0;
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         sum += n[j];
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
   if (tid < E.pairs && rounds < most) load = load_after(rounds, share, fits);
   // ---- the rest: cut at the pairs' remaining shares
   const int rest0 = rounds * E.pairs;                                       // first item of the rest
-  const int base = rest0 < items ? E.items[rest0].prefix : total, rest = total - base;
+  const int base = rest0 < items ? tiles_of(rest0).x : total, rest = total - base;
   int room = tid < E.pairs ? share - load : 0, all;
   const int at = block_scan(room, sums, all) - room;
   if (tid < E.pairs) {
@@ -240,7 +244,8 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
   }
   __syncthreads();
   for (int i = rest0 + tid; i < items; i += kExtSchedThreads) {
-    const int a = E.items[i].prefix - base, z = a + E.items[i].ntiles;
+    const int2 it = tiles_of(i);
+    const int a = it.x - base, z = a + it.y;
     auto holder = [&](int x) {  // last pair whose piece starts at or before tile x (pieces without tiles lie in front of it)
       int lo = 0, hi = E.pairs - 1;
       while (lo < hi) {

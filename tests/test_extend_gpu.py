@@ -257,3 +257,17 @@ def test_what_the_workspace_held_before_does_not_matter(kv_lens, q_lens, window,
     assert call(ws.numel() - 1) != 0 and "workspace" in lib.nvfp4_mla_last_error().decode()
     assert call(ws.numel()) == 0
     assert worst_row(out, reference(c, window, sinks)) <= ROW_TOL and int(status) == 0
+
+
+def test_more_requests_than_are_scheduled_at_once():
+    """2500 requests of one and two new tokens (the schedule takes 2048 at a time)."""
+    n = 2500
+    kv_lens, q_lens = [1 + i % 90 for i in range(n)], [1 + i % 2 for i in range(n)]
+    q_lens = [min(q, k) for q, k in zip(q_lens, kv_lens)]
+    c = chunk(kv_lens, q_lens, 8, 16)
+    out = run(c)
+    for b in (0, 1, 2046, 2047, 2048, 2049, 2499):
+        at = int(c.indptr[b])
+        want = attention64(c.q_nope[at:at + q_lens[b]], c.q_pe[at:at + q_lens[b]], c.cache, c.page_table[b:b + 1], [kv_lens[b]], [q_lens[b]], SM_SCALE, c.ckv_scale, c.kpe_scale)
+        assert worst_row(out[at:at + q_lens[b]], want) <= ROW_TOL
+    assert not out.isnan().any() and mla.workspace_status() == 0
