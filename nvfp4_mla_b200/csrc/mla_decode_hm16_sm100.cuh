@@ -107,7 +107,7 @@ __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams
     const Seg seg = s.segs[si];
     const int nt = h16_tiles(seg);
     if (nt <= 0) continue;
-    WindowMap win;
+    WindowMap win = {};
     if constexpr (WINDOW) win = seg_window(P, seg.b);
     if (it == 0)
       for (int t = 1; t < kH16Ahead && t < nt; ++t) h16_prefetch_rows<WINDOW>(P, seg, win, t, cg, lane);
@@ -125,7 +125,7 @@ __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams
           for (int i = lane; i < nr * 9; i += 32)
             ptx::prefetch_l2(i < nr * 8 ? reinterpret_cast<const char*>(P.q_nope + row0 * CKV) + i * 128
                                         : reinterpret_cast<const char*>(P.q_pe + row0 * KPE) + (i - nr * 8) * 128);
-          WindowMap nx_win;
+          WindowMap nx_win = {};
           if constexpr (WINDOW) nx_win = seg_window(P, nx.b);
           for (int t2 = 0; t2 < kH16Ahead && t2 < nn; ++t2) h16_prefetch_rows<WINDOW>(P, nx, nx_win, t2, cg, lane);
           break;
@@ -165,7 +165,7 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
     const int nt = h16_tiles(seg);
     if (nt <= 0) continue;
     const int* pt = P.page_table + (long long)seg.b * P.pt_stride;
-    WindowMap win;
+    WindowMap win = {};
     if constexpr (WINDOW) win = seg_window(P, seg.b);
     const int2 dead = WINDOW ? win.dead : make_int2(0, 0);  // tokens that no row sees: they read as zeros
     const int first_masked = P.q_len > 1 ? P.kv_lens[seg.b] - (P.q_len - 1) : INT_MAX;  // first token that some row does not see

@@ -109,7 +109,7 @@ __device__ __forceinline__ void vt_producer_role(VtSmem& s, const DecodeParams& 
     const Seg seg = s.segs[si];
     if (seg.ntiles <= 0) continue;
     const int* pt = P.page_table + (long long)seg.b * P.pt_stride;
-    WindowMap win;
+    WindowMap win = {};
     if constexpr (WINDOW) win = seg_window(P, seg.b);
     auto page_id = [&](int i) { return pt[WINDOW ? win.page(i) : i]; };
     // page ids of a tile's two half tiles and of the two that are prefetched into L2 (three tiles ahead: the ring itself

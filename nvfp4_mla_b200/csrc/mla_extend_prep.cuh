@@ -35,7 +35,7 @@ constexpr int kExtMaxBatch = 2048;  // requests at a time
 constexpr int kExtHeld = 4096;      // items whose tile counts the schedule kernel keeps in shared memory
 constexpr int kExtMaxPairs = 128;
 
-struct ExtItem {
+struct alignas(16) ExtItem {  // (read and written in 16-byte words: as ints, 787 items took the schedule kernel 12000 of its 26000 cycles)
   int prefix;      // tiles of the items before
   int ntiles;      // at least 1 (an item that sees nothing has one tile, all masked)
   int block0;      // first workspace block of the request
@@ -44,11 +44,11 @@ struct ExtItem {
   int row0, rows;  // first row in [total_q * heads], number of rows
   int r0;          // first row within the request
   int pos0;        // position of the request's first query token
-  int pad[6];
+  int pad[2];
 };
-static_assert(sizeof(ExtItem) == 64, "ExtItem is a cache line half");
+static_assert(sizeof(ExtItem) == 48, "ExtItem is three 16-byte words");
 
-struct ExtPair {
+struct alignas(16) ExtPair {
   int rounds;              // whole items pair, pair + pairs, ...: this many
   int item, first, count;  // and of the rest: first item, first flattened tile, tiles
   int split, parts;        // item whose first tiles this pair holds and whose last ones another does, or -1; pairs that share it
