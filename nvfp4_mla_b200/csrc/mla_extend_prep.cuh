@@ -1,9 +1,9 @@
 // Chunks of new tokens, everything around the attention kernel (mla_extend_sm100.cuh): the schedule, the FP16 operands, the merge.
 //
 // The rows of a request (query token, head) are cut into tiles of 128, the ITEMS; an item's work is the 64-token BLOCKS of the cache
-// that its rows see, four to a tile of the attention kernel. The items are dealt out whole, item i to CTA pair i % pairs, for as many rounds as leave every pair at or below
-// its even share of the tiles; the tiles of the items that are left are laid end to end and cut so that every pair ends up with its
-// share. Pairs that work at the same time thus work on neighbouring items, which read the same tokens: with one contiguous piece of
+// that its rows see, four to a tile of the attention kernel. An item costs a pair its tiles and kItemCost more (its query, its output).
+// The items are dealt out whole, item i to CTA pair i % pairs, for as many rounds as leave every pair at or below its even share of the
+// cost; the tiles of the items that are left are laid end to end and cut so that every pair ends up with its share. Pairs that work at the same time thus work on neighbouring items, which read the same tokens: with one contiguous piece of
 // the flattened tiles per pair, 24 ragged chunks over 115 MB of FP16 rows read 1.6 GB from HBM (a third of the sectors missed L2) and
 // took 913 us.
 //
@@ -72,6 +72,8 @@ struct ExtProblem {
 };
 
 constexpr int kExtSchedThreads = 1024;
+// Costs in quarters of a tile. Measured, cycles: a tile 5900 to 6200, an item 10000 to 12500 beside its tiles.
+constexpr int kTileCost = 4, kItemCost = 7;
 
 // inclusive scan over the block (every thread takes part); `sums`: 33 ints; the block's sum in `all`
 __device__ __forceinline__ int block_scan(int v, int* sums, int& all) {
@@ -205,10 +207,12 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
   auto tiles_of = [&](int i) { return i < kExtHeld ? held[i] : make_int2(E.items[i].prefix, E.items[i].ntiles); };
 
   // ---- rounds of whole items
-  const int share = total > 0 ? (total + E.pairs - 1) / E.pairs : 1, most = items / E.pairs;
+  const long long cost = (long long)kTileCost * total + (long long)kItemCost * items;
+  const long long share = (cost + E.pairs - 1) / E.pairs;
+  const int most = items / E.pairs;
   constexpr int kAhead = 8;  // loads in flight
-  auto load_after = [&](int rounds, int limit, int& fits) {  // tiles of this pair's first `rounds` items; how many of them stay within `limit`
-    int sum = 0;
+  auto load_after = [&](int rounds, long long limit, int& fits) {  // cost of this pair's first `rounds` items; how many of them stay within `limit`
+    long long sum = 0;
     fits = 0;
     for (int k = 0; k < rounds; k += kAhead) {
       int n[kAhead];
@@ -216,13 +220,14 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
       for (int j = 0; j < kAhead; ++j) n[j] = k + j < rounds ? tiles_of(tid + (k + j) * E.pairs).y : 0;
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        sum += n[j];
+        if (k + j < rounds) sum += kTileCost * n[j] + kItemCost;
         if (k + j < rounds && sum <= limit) fits = k + j + 1;
       }
     }
     return sum;
   };
-  int fits, load = 0;
+  int fits;
+  long long load = 0;
   if (tid < E.pairs) {
     load = load_after(most, share, fits);
     if (fits < most) atomicMin(&rounds_s, fits);
@@ -233,13 +238,30 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
   // ---- the rest: cut at the pairs' remaining shares
   const int rest0 = rounds * E.pairs;                                       // first item of the rest
   const int base = rest0 < items ? tiles_of(rest0).x : total, rest = total - base;
-  int room = tid < E.pairs ? share - load : 0, all;
+  // (a pair's room is below the cost of a round, and that of all pairs below twice the rest's)
+  int room = tid < E.pairs ? int(share - load) : 0, all;
   const int at = block_scan(room, sums, all) - room;
   if (tid < E.pairs) {
-    const int lo = at < rest ? at : rest, hi = at + room < rest ? at + room : rest;
-    cut[tid] = lo;
-    if (tid == E.pairs - 1) cut[E.pairs] = rest;
-    ExtPair o = {rounds, 0, base + lo, hi - lo, -1, 0, {0, 0}};
+    // the tile of the rest at cost `at`: in item i at cost c(i) = kTileCost * tiles before it + kItemCost * items before it
+    int lo = rest0, hi = items - 1;  // last item with c(i) <= at
+    auto c = [&](int i) { return (long long)kTileCost * (tiles_of(i).x - base) + (long long)kItemCost * (i - rest0); };
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (c(mid) <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    int tile = rest;
+    if (lo < items) {
+      const int2 it = tiles_of(lo);
+      const long long in = (at - c(lo) - kItemCost + kTileCost / 2) / kTileCost;  // (nearest)
+      tile = it.x - base + int(in < 0 ? 0 : in < it.y ? in : it.y);
+    }
+    cut[tid] = tid == 0 ? 0 : tile < rest ? tile : rest;
+    if (tid == 0) cut[E.pairs] = rest;
+  }
+  __syncthreads();
+  if (tid < E.pairs) {
+    ExtPair o = {rounds, 0, base + cut[tid], cut[tid + 1] - cut[tid], -1, 0, {0, 0}};
     E.pair[tid] = o;
   }
   __syncthreads();
