@@ -213,7 +213,9 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
   const int lane = threadIdx.x & 31;
   const QuantScales Q(ckv_scale, kpe_scale);
   const float eps_f = float(eps);
-  bool ordinary_gains = true;  // 0 or of ordinary size
+  // Weights: 0 or of ordinary size. A product below fp32's normal numbers (not exact) then stands for a y below 2^-96, whose code is 0
+  // whatever its error, unless the cache's scale is that small as well.
+  bool ordinary_gains = ckv_scale > 0x1p-80f;
   for (int i = threadIdx.x; i < CKV; i += kQuantThreads) {
     const float g = __bfloat162float(weight[i]);
     reinterpret_cast<float*>(&gains[(i & 15) >> 2][i >> 4])[i & 3] = g;

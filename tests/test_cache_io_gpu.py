@@ -76,6 +76,23 @@ def test_values_of_unequal_size_and_separate_rows():
             assert torch.equal(got, exp)
 
 
+def test_products_below_the_range_of_fp32():
+    """Channels whose product with the weight is below fp32's normal numbers, the normalised value and the cache's scale above."""
+    kv_a, weight, cos_sin, b, pos, cache, kv_indices, kv_indptr = rows([200], [0], 64)
+    kv_a *= 2.0 ** -27
+    g = torch.Generator(device="cuda").manual_seed(3)
+    kv_a.view(torch.int16)[:, :256] = torch.randint(1, 64, (200, 256), generator=g, device="cuda").short()  # times 2^-133
+    weight[:256] *= 2.0 ** -15
+    want = tuple(t.clone() for t in cache)
+    ckv, kpe = normed(kv_a, weight, cos_sin, pos, 0.0, True)
+    mla.quantize_append_paged_mla_kv_cache(ckv, kpe, b, pos, *want, kv_indices, kv_indptr, None, 2.0 ** -110, 1.0)
+    mla.norm_rope_append_paged_mla_kv_cache(kv_a[:, :512], kv_a[:, 512:], weight, cos_sin, b, pos, *cache, kv_indices, kv_indptr, eps=0.0,
+                                            ckv_scale=2.0 ** -110)
+    assert want[1].float()[:-1].any()
+    for got, exp in zip(raw(cache), raw(want)):
+        assert torch.equal(got, exp)
+
+
 def test_tokens_outside_the_tables_are_skipped():
     kv_a, weight, cos_sin, b, pos, cache, kv_indices, kv_indptr = rows([40, 3], [0, 0], 16)
     before = [t.clone() for t in raw(cache)]
