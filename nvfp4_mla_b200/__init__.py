@@ -170,7 +170,9 @@ def _status(dev):
     """The device's status word; None while a graph is captured before any call has made it."""
     word = _statuses.get(dev.index)
     if word is None and not torch.cuda.is_current_stream_capturing():
-        word = _statuses[dev.index] = torch.zeros(1, dtype=torch.int32, device=dev)
+        word = torch.zeros(1, dtype=torch.int32, device=dev)
+        torch.cuda.current_stream(dev).synchronize()  # (once per device: a call on another stream may report before the zero is written)
+        word = _statuses.setdefault(dev.index, word)
     return word
 
 
@@ -275,7 +277,8 @@ def extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens
         kv_lens: ``[batch]`` int32, tokens per request WITH the new ones, which are the last and whose rows are in the cache.
         qo_indptr: ``[batch + 1]`` int32, non-decreasing: request ``b`` has the query tokens ``qo_indptr[b] .. qo_indptr[b + 1]``.
         max_kv_len: an upper bound of ``kv_lens``, which with the shapes fixes the launch shape and the workspace. Without it the page
-            table's width is the bound; nothing synchronises either way, and the call can be captured in a CUDA graph.
+            table's width is the bound; nothing synchronises either way, and the call can be captured in a CUDA graph. (The workspace
+            holds up to 1152 bytes per token of the bound and request, at most 8 GB: a bound near the lengths saves memory.)
         window, sink_tokens: with ``window > 0`` a token attends to the last ``window`` tokens up to its own position and to the first
             ``sink_tokens``; pages that no query of the call sees are not looked up.
 
@@ -544,7 +547,8 @@ def norm_rope_append_paged_mla_kv_cache(ckv, kpe, norm_weight, cos_sin, batch_in
     float32 (the 32 cosines of a position, then its sines); a token is rotated by the angles of its ``positions`` entry, in pairs
     ``(2k, 2k + 1)`` (``interleaved``) or ``(k, k + 32)``. The normalised and the rotated row are rounded to bfloat16 once, from
     64-bit arithmetic by way of fp32, and the cache receives the bytes that ``quantize_append_paged_mla_kv_cache`` makes of them;
-    the tables and ``check`` are that call's. A token past the end of ``cos_sin`` counts as outside the tables."""
+    the tables and ``check`` are that call's. A token past the end of ``cos_sin`` counts as outside the tables. A place in the cache may be
+    named once per call."""
     strides = _check_norm_append(ckv, kpe, norm_weight, cos_sin, batch_indices, positions, ckv_cache, ckv_sf_cache, kpe_cache, kv_indices, kv_indptr, eps,
                                  ckv_scale, kpe_scale)
     status = torch.zeros(1, dtype=torch.int32, device=ckv_cache.device) if check else None
