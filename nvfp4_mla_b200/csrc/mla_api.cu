@@ -175,9 +175,8 @@ int device_info(DeviceInfo** out) {
       return clusters < d.sm_count / 2 ? clusters : d.sm_count / 2;
     };
     d.hm_pairs = resident_pairs(decode_entry(NVFP4_MLA_PRECISION_FP8, 128), mla::kHmThreads, decode_smem(NVFP4_MLA_PRECISION_FP8, 128));
-    static_assert(mla::kExtMaxPairs >= 74, "more pairs than the chunk schedule has room for");
     d.ext_pairs = resident_pairs(reinterpret_cast<const void*>(mla::mla_extend_kernel), mla::kExtThreads, mla::ext_smem_bytes());
-    if (d.ext_pairs > mla::kExtMaxPairs) d.ext_pairs = mla::kExtMaxPairs;
+    if (d.ext_pairs > mla::kExtMaxPairs) d.ext_pairs = mla::kExtMaxPairs;  // (74 on 148 SMs)
     if (getenv("NVFP4_MLA_DEBUG"))
       fprintf(stderr, "nvfp4_mla_b200: device %d: %d SMs, %d resident CTA pairs for the 128-head kernel, %d for chunk attention\n", dev, d.sm_count,
               d.hm_pairs, d.ext_pairs);
@@ -330,8 +329,7 @@ int64_t nvfp4_mla_decode_workspace_bytes(int batch, int heads, int num_splits) {
 // The decode call proper; `heads` counts the rows of all q_len query tokens of a request, `hpc_limit` caps the heads per CTA
 // (see heads_per_cta), which are chosen for requests of `expected_kv_len` tokens (0: of the bound max_kv_len). `dead`: the tokens of
 // each request that are not seen (kernels with WINDOW, 16-bit mode), or null; `window`: a sliding window, the page table's width with it;
-// `status`: where the kernels report, or null for the
-// workspace's first word.
+// `status`: where the kernels report, or null for the workspace's first word.
 static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
                        const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table,
                        int64_t page_table_stride, const int32_t* kv_lens, int batch, int heads, float sm_scale, float ckv_scale,

@@ -177,7 +177,7 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
     // No load sits behind a branch (it would be waited for where the branches meet, one trip to memory per load instead of
     // one per tile): tokens past the end look up the last live token's page, dead rows read cache row 0 and are zeroed where
     // their bytes are used, and the fetches past the last tile are issued like the others.
-    auto fetch_id = [&](int tk) { 
+    auto fetch_id = [&](int tk) {
       const int pi = (tk < seg.tok_end ? tk : seg.tok_end - 1) >> P.page_shift;
       return __ldg(pt + (WINDOW ? win.page(pi) : pi));
     };

@@ -2,10 +2,11 @@
 //
 // The rows of a request (query token, head) are cut into tiles of 128, the ITEMS; an item's work is the 64-token BLOCKS of the cache
 // that its rows see, four to a tile of the attention kernel. An item costs a pair its tiles and kItemCost more (its query, its output).
-// The items are dealt out whole, item i to CTA pair i % pairs, for as many rounds as leave every pair at or below its even share of the
-// cost; the tiles of the items that are left are laid end to end and cut so that every pair ends up with its share. Pairs that work at the same time thus work on neighbouring items, which read the same tokens: with one contiguous piece of
-// the flattened tiles per pair, 24 ragged chunks over 115 MB of FP16 rows read 1.6 GB from HBM (a third of the sectors missed L2) and
-// took 913 us.
+// The items are dealt out whole, item i to CTA pair i % pairs, for as many rounds as leave every pair at or below its even share of
+// the cost; the tiles of the items that are left are laid end to end and cut so that every pair ends up with its share. Pairs that
+// work at the same time thus work on neighbouring items, which read the same tokens. 24 ragged chunks of 16 heads (1 to 400 query
+// tokens behind 0 to 8000 others, 115 MB of FP16 rows): 885 us; with shares of tiles alone 900; with one contiguous piece of the
+// flattened tiles per pair 913 and 1.6 GB read from HBM (a third of the sectors missed L2).
 //
 // Window: the tokens that some query of the request sees are [0, S) and everything from the first query's window on. The cache is
 // read into a numbering of blocks that has no gap: the first `sink_blocks` blocks, then the blocks from the window's on, `shift` tokens
@@ -75,29 +76,31 @@ constexpr int kExtSchedThreads = 1024;
 // Costs in quarters of a tile. Measured, cycles: a tile 5900 to 6200, an item 10000 to 12500 beside its tiles.
 constexpr int kTileCost = 4, kItemCost = 7;
 
-// inclusive scan over the block (every thread takes part); `sums`: 33 ints; the block's sum in `all`
-__device__ __forceinline__ int block_scan(int v, int* sums, int& all) {
+// inclusive scan over the block (every thread takes part); `sums`: 32 of them; the block's sum in `all`
+template <class T>
+__device__ __forceinline__ T block_scan(T v, long long* held, T& all) {
+  T* sums = reinterpret_cast<T*>(held);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(~0u, v, o);
+    const T u = __shfl_up_sync(~0u, v, o);
     if (lane >= o) v += u;
   }
   __syncthreads();
   if (lane == 31) sums[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    int w = sums[lane];
+    T w = sums[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(~0u, w, o);
+      const T u = __shfl_up_sync(~0u, w, o);
       if (lane >= o) w += u;
     }
     sums[lane] = w;
   }
   __syncthreads();
   all = sums[31];
-  return v + (warp ? sums[warp - 1] : 0);
+  return v + (warp ? sums[warp - 1] : T(0));
 }
 
 struct ExtRequest {
@@ -131,7 +134,7 @@ __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
 __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kernel(const ExtProblem E) {
   __shared__ int item0[kExtMaxBatch];
   __shared__ int2 held[kExtHeld];        // {prefix, tiles} of an item
-  __shared__ int sums[33];
+  __shared__ long long sums[32];
   __shared__ int cut[kExtMaxPairs + 1];  // tiles of the rest before pair p
   __shared__ int rounds_s;
   static_assert(kExtSchedThreads == 1024, "block_scan takes 32 warps");
@@ -238,9 +241,9 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
   // ---- the rest: cut at the pairs' remaining shares
   const int rest0 = rounds * E.pairs;                                       // first item of the rest
   const int base = rest0 < items ? tiles_of(rest0).x : total, rest = total - base;
-  // (a pair's room is below the cost of a round, and that of all pairs below twice the rest's)
-  int room = tid < E.pairs ? int(share - load) : 0, all;
-  const int at = block_scan(room, sums, all) - room;
+  const long long room = tid < E.pairs ? share - load : 0;
+  long long all;
+  const long long at = block_scan(room, sums, all) - room;
   if (tid < E.pairs) {
     // the tile of the rest at cost `at`: in item i at cost c(i) = kTileCost * tiles before it + kItemCost * items before it
     int lo = rest0, hi = items - 1;  // last item with c(i) <= at
