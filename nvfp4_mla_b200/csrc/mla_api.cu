@@ -500,7 +500,7 @@ namespace {
 constexpr int kExtendSlice = 512;  // query tokens at a time in the first form (the partial results of a slice take 2 KB per head and token)
 
 struct ExtendLayout {
-  size_t counts, req_block0, req_map, items, pair, q_scale, lse_part, o_part, q16, kv16, total;
+  size_t items, pair, q_scale, lse_part, o_part, q16, kv16, total;
   int group;  // requests at a time
   int pairs, max_items, max_blocks;
 };
@@ -532,7 +532,6 @@ int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window,
     off = mla::align_up(off + bytes, 256);
     return at;
   };
-  l->counts = take(64), l->req_block0 = take(size_t(l->group + 1) * 4), l->req_map = take(size_t(l->group) * 16);
   l->items = take(size_t(items) * sizeof(mla::ExtItem)), l->pair = take(size_t(l->pairs) * sizeof(mla::ExtPair));
   l->q_scale = take(size_t(items) * mla::kExtRows * 4);
   l->lse_part = take(size_t(l->pairs) * 2 * mla::kExtRows * 4), l->o_part = take(size_t(l->pairs) * 2 * mla::kExtRows * mla::CKV * 4);
@@ -593,9 +592,7 @@ int extend_shared(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache
   mla::ExtProblem E;
   E.total_q = total_q, E.heads = heads, E.max_kv_len = max_kv_len;
   E.window = window, E.sinks = sink_tokens, E.pairs = l.pairs, E.max_items = l.max_items, E.max_blocks = l.max_blocks;
-  E.req_block0 = reinterpret_cast<int*>(ws + l.req_block0);
-  E.req_map = reinterpret_cast<int4*>(ws + l.req_map), E.items = reinterpret_cast<mla::ExtItem*>(ws + l.items);
-  E.pair = reinterpret_cast<mla::ExtPair*>(ws + l.pair), E.counts = reinterpret_cast<int*>(ws + l.counts), E.status = status;
+  E.items = reinterpret_cast<mla::ExtItem*>(ws + l.items), E.pair = reinterpret_cast<mla::ExtPair*>(ws + l.pair), E.status = status;
   mla::ExtOperands O;
   O.q_nope = static_cast<const __nv_bfloat16*>(q_nope), O.q_pe = static_cast<const __nv_bfloat16*>(q_pe), O.ckv = ckv_cache, O.sf = ckv_sf_cache;
   O.kpe = kpe_cache, O.pt_stride = page_table_stride, O.pt_width = page_table_width;

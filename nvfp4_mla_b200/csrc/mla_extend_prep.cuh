@@ -33,7 +33,7 @@ constexpr int kExtBlock = 64;   // tokens of a block
 constexpr int kExtTile = 256;   // tokens of a tile
 constexpr int kExtRow = CKV + KPE;
 constexpr int kExtMaxBatch = 2048;  // requests at a time
-constexpr int kExtHeld = 4096;      // items whose tile counts the schedule kernel keeps in shared memory
+constexpr int kExtHeld = 3584;      // items whose tile counts the schedule kernel keeps in shared memory
 constexpr int kExtMaxPairs = 128;
 
 struct alignas(16) ExtItem {  // (read and written in 16-byte words: as ints, 787 items took the schedule kernel 12000 of its 26000 cycles)
@@ -64,11 +64,8 @@ struct ExtProblem {
   int max_items, max_blocks;
   int first_q;      // without an indptr: index of the first request's query token
   int edges;        // 1: the rows in front of the first request's are this call's to fill with zeros, 2: those behind the last one's
-  int* req_block0;  // [batch + 1] workspace blocks before request b
-  int4* req_map;    // [batch] {shift, first tokens' blocks, tokens in the blocks (with the shift taken out), first token of the window}
   ExtItem* items;   // [max_items]
   ExtPair* pair;    // [pairs]
-  int* counts;      // [0] items, [1] workspace blocks
   int* status;
 };
 
@@ -76,8 +73,8 @@ constexpr int kExtSchedThreads = 1024;
 // Costs in quarters of a tile. Measured, cycles: a tile 5900 to 6200, an item 10000 to 12500 beside its tiles.
 constexpr int kTileCost = 4, kItemCost = 7;
 
-// inclusive scan over the block (every thread takes part); `sums`: 32 of them; the block's sum in `all`
-template <class T>
+// inclusive scan over a block of WARPS warps (every thread takes part); `sums`: 32 of them; the block's sum in `all`
+template <int WARPS, class T>
 __device__ __forceinline__ T block_scan(T v, long long* held, T& all) {
   T* sums = reinterpret_cast<T*>(held);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -90,7 +87,7 @@ __device__ __forceinline__ T block_scan(T v, long long* held, T& all) {
   if (lane == 31) sums[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    T w = sums[lane];
+    T w = lane < WARPS ? sums[lane] : T(0);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const T u = __shfl_up_sync(~0u, w, o);
@@ -131,41 +128,51 @@ __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
   return r;
 }
 
-__global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kernel(const ExtProblem E) {
-  __shared__ int item0[kExtMaxBatch];
-  __shared__ int2 held[kExtHeld];        // {prefix, tiles} of an item
-  __shared__ long long sums[32];
-  __shared__ int cut[kExtMaxPairs + 1];  // tiles of the rest before pair p
-  __shared__ int rounds_s;
-  static_assert(kExtSchedThreads == 1024, "block_scan takes 32 warps");
-  ptx::grid_launch_dependents();
+// Where the requests' items and workspace blocks begin. The schedule and every block of the operands' kernel work this out for
+// themselves, so that neither waits for the other (32 windowed single tokens of 128 heads: 66.7 us one after the other, 61.6 so).
+struct ExtTables {
+  int item0[kExtMaxBatch], block0[kExtMaxBatch];  // items and blocks of the requests before
+  long long sums[32];
+  int items, blocks;
+};
+template <int THREADS>
+__device__ __forceinline__ void ext_tables(const ExtProblem& E, ExtTables& s) {
   const int tid = threadIdx.x;
   int items = 0, blocks = 0;
-  ExtRequest r = {};
-  for (int b0 = 0; b0 < E.batch; b0 += kExtSchedThreads) {
+  for (int b0 = 0; b0 < E.batch; b0 += THREADS) {
     const int b = b0 + tid;
     int mine = 0, all;
-    r = {};
+    ExtRequest r = {};
     if (b < E.batch) {
       r = ext_request(E, b);
       mine = int(((long long)r.q * E.heads + kExtRows - 1) / kExtRows);
     }
-    const int ii = items + block_scan(mine, sums, all) - mine;
+    const int ii = items + block_scan<THREADS / 32>(mine, s.sums, all) - mine;
     items += all;
-    const int ib = blocks + block_scan(r.blocks, sums, all) - r.blocks;
+    const int ib = blocks + block_scan<THREADS / 32>(r.blocks, s.sums, all) - r.blocks;
     blocks += all;
-    if (b < E.batch) {
-      item0[b] = ii, E.req_block0[b] = ib;
-      E.req_map[b] = make_int4(r.shift, r.sink_blocks, r.n - r.shift, r.begin);
-    }
+    if (b < E.batch) s.item0[b] = ii, s.block0[b] = ib;
   }
   // (a query index that runs backwards could ask for more than there is room for)
   if (items > E.max_items || blocks > E.max_blocks) {
     if (tid == 0 && E.status) atomicExch(E.status, int(kBadSchedule));
     items = 0, blocks = 0;
   }
-  if (tid == 0) E.req_block0[E.batch] = blocks, E.counts[0] = items, E.counts[1] = blocks, rounds_s = items / E.pairs;
+  if (tid == 0) s.items = items, s.blocks = blocks;
   __syncthreads();
+}
+
+__global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kernel(const ExtProblem E) {
+  __shared__ ExtTables tab;
+  __shared__ int2 held[kExtHeld];        // {prefix, tiles} of an item; static shared memory is 48 KB, the tables take 16
+  __shared__ int cut[kExtMaxPairs + 1];  // tiles of the rest before pair p
+  __shared__ int rounds_s;
+  ptx::grid_launch_dependents();
+  const int tid = threadIdx.x;
+  constexpr int kWarps = kExtSchedThreads / 32;
+  ext_tables<kExtSchedThreads>(E, tab);
+  const int items = tab.items;
+  if (tid == 0) rounds_s = items / E.pairs;
 
   // ---- items
   int total = 0;
@@ -176,14 +183,14 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
       int lo = 0, hi = E.batch - 1;  // last b with item0[b] <= i
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (item0[mid] <= i) lo = mid;
+        if (tab.item0[mid] <= i) lo = mid;
         else hi = mid - 1;
       }
-      r = ext_request(E, lo);
-      m.r0 = (i - item0[lo]) * kExtRows;
+      const ExtRequest r = ext_request(E, lo);
+      m.r0 = (i - tab.item0[lo]) * kExtRows;
       const long long rows = (long long)r.q * E.heads - m.r0;
       m.rows = int(rows < kExtRows ? rows : kExtRows);
-      m.row0 = r.q0 * E.heads + m.r0, m.pos0 = r.pos0, m.shift = r.shift, m.block0 = E.req_block0[lo];
+      m.row0 = r.q0 * E.heads + m.r0, m.pos0 = r.pos0, m.shift = r.shift, m.block0 = tab.block0[lo];
       const int first = r.pos0 + m.r0 / E.heads, last = r.pos0 + (m.r0 + m.rows - 1) / E.heads;  // positions of its query tokens
       const int end = last + 1 < r.n ? last + 1 : r.n;                                           // tokens before it are seen
       int e = (end - r.shift + kExtBlock - 1) / kExtBlock;                                       // blocks up to there
@@ -198,7 +205,7 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
       if (m.ntiles < 1) m.ntiles = 1, m.skip = 0;
     }
     int all;
-    const int incl = block_scan(m.ntiles, sums, all);
+    const int incl = block_scan<kWarps>(m.ntiles, tab.sums, all);
     if (i < items) {
       m.prefix = total + incl - m.ntiles;
       E.items[i] = m;
@@ -243,7 +250,7 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
   const int base = rest0 < items ? tiles_of(rest0).x : total, rest = total - base;
   const long long room = tid < E.pairs ? share - load : 0;
   long long all;
-  const long long at = block_scan(room, sums, all) - room;
+  const long long at = block_scan<kWarps>(room, tab.sums, all) - room;
   if (tid < E.pairs) {
     // the tile of the rest at cost `at`: in item i at cost c(i) = kTileCost * tiles before it + kItemCost * items before it
     int lo = rest0, hi = items - 1;  // last item with c(i) <= at
@@ -311,7 +318,7 @@ constexpr int kExtPrepThreads = 256;
 constexpr int kExtQRows = 32;   // rows of a unit
 
 // last b in [0, n) with a[b] <= x (a is non-decreasing, a[0] <= x), by the whole warp: 32 probes at a time
-__device__ __forceinline__ int warp_upper(const int* __restrict__ a, int n, int x) {
+__device__ __forceinline__ int warp_upper(const int* a, int n, int x) {
   const int lane = threadIdx.x & 31;
   int lo = 0;
   while (n > 1) {
@@ -323,18 +330,18 @@ __device__ __forceinline__ int warp_upper(const int* __restrict__ a, int n, int 
   return lo;
 }
 
-__device__ __forceinline__ void ext_convert_tokens(const ExtProblem& E, const ExtOperands& O, int unit) {
+__device__ __forceinline__ void ext_convert_tokens(const ExtProblem& E, const ExtOperands& O, const ExtTables& tab, int unit) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kPer = kExtBlock / (kExtPrepThreads / 32);  // tokens of a warp
   const int t0 = unit * kExtBlock + kPer * warp;
-  const int lo = warp_upper(E.req_block0, E.batch, unit);
-  const int4 map = E.req_map[lo];
-  const int v = t0 - E.req_block0[lo] * kExtBlock + lane;  // this lane's token among the request's
+  const int lo = warp_upper(tab.block0, E.batch, unit);
+  const ExtRequest r = ext_request(E, lo);
+  const int v = t0 - tab.block0[lo] * kExtBlock + lane;  // this lane's token among the request's
   int src = -1;                                          // its cache row; -1: zeros
-  if (lane < kPer && v < map.z && unit < E.counts[1]) {
-    const int tok = v < map.y * kExtBlock ? v : v + map.x;
+  if (lane < kPer && v < r.n - r.shift && unit < tab.blocks) {
+    const int tok = v < r.sink_blocks * kExtBlock ? v : v + r.shift;
     // (tokens between the first ones and the window belong to blocks that are read, but their pages may be gone)
-    if (tok < E.sinks || tok >= map.w) {
+    if (tok < E.sinks || tok >= r.begin) {
       const int pi = tok >> O.page_shift;
       const int page = pi < O.pt_width ? O.page_table[(long long)lo * O.pt_stride + pi] : -1;
       if (page >= 0 && page < O.num_pages) src = (page << O.page_shift) + (tok & ((1 << O.page_shift) - 1));
@@ -375,18 +382,20 @@ __device__ __forceinline__ void ext_convert_tokens(const ExtProblem& E, const Ex
   }
 }
 
-__device__ __forceinline__ void ext_convert_rows(const ExtProblem& E, const ExtOperands& O, int unit) {
+__device__ __forceinline__ void ext_convert_rows(const ExtProblem& E, const ExtOperands& O, const ExtTables& tab, int unit) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int item = unit / (kExtRows / kExtQRows);
   constexpr int U = kExtQRows / (kExtPrepThreads / 32);  // rows of a warp
   const int r0 = (unit % (kExtRows / kExtQRows)) * kExtQRows + U * warp;
-  const int row0 = E.items[item].row0, rows = E.items[item].rows;
+  const int b = warp_upper(tab.item0, E.batch, item), first = (item - tab.item0[b]) * kExtRows;  // of the request's rows
+  const ExtRequest r = ext_request(E, b);
+  const long long row0 = (long long)r.q0 * E.heads + first, rows = (long long)r.q * E.heads - first;  // (of which the item has up to 128)
   const float ratio = O.kpe_scale / O.ckv_scale;  // rope scores in units of the latent ones
   uint4 w0[U], w1[U];
   uint32_t rp[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long at = (long long)row0 + (r0 + u < rows ? r0 + u : rows - 1);  // (dead rows repeat the last live one and are not written out)
+    const long long at = row0 + (r0 + u < rows ? r0 + u : rows - 1);  // (dead rows repeat the last live one and are not written out)
     const uint4* src = reinterpret_cast<const uint4*>(O.q_nope + at * CKV);
     w0[u] = __ldg(src + lane), w1[u] = __ldg(src + 32 + lane);  // channels 8 lane .. of both halves of the row
     rp[u] = __ldg(reinterpret_cast<const uint32_t*>(O.q_pe + at * KPE) + lane);
@@ -419,9 +428,11 @@ __device__ __forceinline__ void ext_convert_rows(const ExtProblem& E, const ExtO
   }
 }
 
+// Starts while the schedule is made and ends after it: the attention kernel, which waits for this grid, has waited for both.
 __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const ExtProblem E, const ExtOperands O) {
-  ptx::grid_dependency_wait();
+  __shared__ ExtTables tab;
   ptx::grid_launch_dependents();
+  ext_tables<kExtPrepThreads>(E, tab);
   const int a = ext_first(E, 0), first = a < 0 ? 0 : a < E.total_q ? a : E.total_q;
   const int z = ext_first(E, E.batch), last = z < first ? first : z < E.total_q ? z : E.total_q;
   const long long front = E.edges & 1 ? (long long)first * E.heads : 0, none = front + (E.edges & 2 ? (long long)(E.total_q - last) * E.heads : 0);
@@ -430,11 +441,12 @@ __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const 
     O.out[row * (CKV / 8) + (threadIdx.x & 63)] = make_uint4(0, 0, 0, 0);
   }
   // (the last tile reads up to three blocks behind the last one, with weight 0: zeros)
-  const int tokens = E.counts[1] + 3 < E.max_blocks ? E.counts[1] + 3 : E.max_blocks, units = tokens + E.counts[0] * (kExtRows / kExtQRows);
+  const int tokens = tab.blocks + 3 < E.max_blocks ? tab.blocks + 3 : E.max_blocks, units = tokens + tab.items * (kExtRows / kExtQRows);
   for (int i = blockIdx.x; i < units; i += gridDim.x) {
-    if (i < tokens) ext_convert_tokens(E, O, i);
-    else ext_convert_rows(E, O, i - tokens);
+    if (i < tokens) ext_convert_tokens(E, O, tab, i);
+    else ext_convert_rows(E, O, tab, i - tokens);
   }
+  ptx::grid_dependency_wait();
 }
 
 // ---------------------------------------------------------------------------------------------------------------
