@@ -11,7 +11,14 @@
 // does. As the pair shares B, each CTA loads half of it; K is split by tokens and V by channels, so a token row crosses into
 // shared memory twice (its K part in one CTA, halves of its V part in both): 278 KB per tile and CTA.
 //
-// What bounds it: the tensor pipe needs 36 * 64 + 32 * 64 = 4352 cycles per tile.
+// What bounds it: the tensor pipe needs 36 * 64 + 32 * 64 = 4352 cycles per tile, shared memory 5690 (728 KB at 128 bytes per cycle: A and
+// B of the products 408, the loads 278, P 32; measured 5900 to 6200), and in calls of more than a few hundred us the 1 kW power
+// limit holds the clock at 1.57 to 1.65 GHz. 1024 query tokens of 128 heads behind 15360 others: 3.56 ms, 1.27 PFLOP/s, 0.93 of what the
+// library's BF16 product sustains; 4 chunks of 512 of 16 heads behind 7680: 418 us of the call's 484, tensor pipe 73 % busy (ncu),
+// 76 MB from HBM, 10.7 TB/s from L2. The end of an item costs a pair 10000 to 12500 cycles (output, next query, pipeline filling).
+// Stalls that were taken out without the time changing, which is how the power limit shows: a thread of its own for the query's
+// loads, output by four more warps, output straight from registers, the query converted in here. M = 256 per pair (two thirds of the
+// shared-memory traffic per row) would need all of tensor memory for O.
 //
 // Tensor memory: O: 0..255 | S: 256..511 (two buffers of 128).
 // Shared memory: Q 72 KB | P 32 KB | ring of seven 16 KB units (K: 128 tokens x 64 channels; V: 64 tokens x 128 channels).

@@ -58,11 +58,12 @@ __device__ __forceinline__ uint32_t e2m1_code(float y) {
 constexpr float kQuantDown = 1.f - 0x1p-21f, kQuantUp = 1.f + 0x1p-21f;
 struct QuantScales {
   float ckv_scale, kpe_scale, six_dn, six_up, kpe_dn, kpe_up;
-  bool fast_sf, fast_kpe;
+  bool fast_sf, fast_kpe, short_ckv;
   __device__ __forceinline__ QuantScales(float ckv, float kpe) : ckv_scale(ckv), kpe_scale(kpe) {
     auto ordinary = [](float d) { return d > 0x1p-100f && d < 0x1p100f; };
     const float six = __fmul_rn(6.0f, ckv), r_six = __frcp_rn(six), r_kpe = __frcp_rn(kpe);
     fast_sf = ordinary(six), fast_kpe = ordinary(kpe);
+    short_ckv = (__float_as_uint(ckv) & 0xFFFFu) == 0u;
     const bool kpe_pow2 = (__float_as_uint(kpe) & 0x007FFFFFu) == 0u;
     six_dn = r_six * kQuantDown, six_up = r_six * kQuantUp;
     kpe_dn = kpe_pow2 ? r_kpe : r_kpe * kQuantDown, kpe_up = kpe_pow2 ? r_kpe : r_kpe * kQuantUp;
@@ -84,7 +85,25 @@ __device__ __forceinline__ QuantBlock quantize_block(const float (&x)[16], const
   const float sf = __fmul_rn(e4m3_value(uint8_t(sf8)), Q.ckv_scale);
   uint32_t lo = 0, hi = 0;
   if (sf > 0.f) {
-    const float r = __frcp_rn(sf), rd = r * kQuantDown, ru = r * kQuantUp;
+    const float r = __frcp_rn(sf);
+    // A value is this close to a boundary T (mantissa 1, 1.25, 1.5 or 1.75) only where T * sf is that close to a BF16 number, which the
+    // scale alone decides: x * r and fl(x / sf) round alike unless |x - T sf| <= 2^-22 T sf, five units in the last place of
+    // fl(T sf). With eight units of room one block in a thousand is left, unless the cache's scale has few bits.
+    if (!Q.short_ckv) {
+      const float t1 = sf * 1.25f, t2 = sf * 1.5f, t3 = sf * 1.75f;
+      uint32_t nearest = __viaddmin_u16x2(__byte_perm(__float_as_uint(sf), __float_as_uint(t1), 0x5410), 0x00080008u, 0xFFFFFFFFu);
+      nearest = __viaddmin_u16x2(__byte_perm(__float_as_uint(t2), __float_as_uint(t3), 0x5410), 0x00080008u, nearest);
+      if ((nearest & 0xFFFFu) > 16u && nearest >> 16 > 16u && sf > 0x1p-100f && sf < 0x1p100f) {
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          const float2 p = ptx::mul_f32x2(make_float2(x[j], x[j + 1]), make_float2(r, r));
+          y[j] = p.x, y[j + 1] = p.y;
+        }
+        return {e2m1x8(reinterpret_cast<const float(&)[8]>(y[0])), e2m1x8(reinterpret_cast<const float(&)[8]>(y[8])), sf8};
+      }
+    }
+    const float rd = r * kQuantDown, ru = r * kQuantUp;
     float yd[16], yu[16];
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
@@ -181,8 +200,8 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 //   then the writer's own steps (above): the bytes are those of mla_quantize_append_kernel on the BF16 rows.
 // A code of the cache changes by a whole step where a value crosses a rounding border, so the BF16 values themselves are exact. They
 // are computed in fp32 with an error bound, and a value that close to a BF16 border is computed again in 64 bits:
-//   latent: the squares are exact in fp32 (eight bits times eight), their sum passes nine rounding additions (four levels of a tree in
-//           a lane, five shuffles): within 9 * 2^-24 of itself; eps and its addition (2 * 2^-24 of the mean, half of it in the root),
+//   latent: the squares are exact in fp32 (eight bits times eight), their sum passes ten rounding additions (five in a lane, five
+//           shuffles): within 10 * 2^-24 of itself; eps and its addition (2 * 2^-24 of the mean, half of it in the root),
 //           the reciprocal root (two units) and the product (x w is exact) make y off by at most 11 units in its last place. One
 //           value in 2600 is that close to a border, one token in five has such a value.
 //   rope  : a cos - b sin as fma(a, cos, -p) - fma(b, sin, -p) with p = b sin rounded, which is within two units of the defined number.
@@ -224,7 +243,17 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
   ordinary_gains = __syncthreads_and(ordinary_gains);
   const long long warp0 = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   const long long stride = (long long)gridDim.x * (kQuantThreads / 32);
-  for (long long t = warp0; t < nnz; t += stride) {
+  // A lane looks up the place of one of the warp's next 32 tokens: one walk through the page tables for all of them.
+  int places = -1, at = 0;
+  int k = 0;
+  for (long long t = warp0; t < nnz; t += stride, ++k) {
+    if ((k & 31) == 0) {
+      const long long mine = t + lane * stride;
+      if (mine < nnz) {
+        at = positions[mine];
+        places = at < max_pos ? cache_row(batch_indices[mine], at, int(num_pages), page_shift, kv_indices, kv_indptr, batch) : -1;
+      }
+    }
     const uint4* src = reinterpret_cast<const uint4*>(ckv + t * ckv_stride + 16 * lane);
     const uint4 w0 = __ldcs(src), w1 = __ldcs(src + 1);
     const __nv_bfloat16* rp = kpe + t * kpe_stride;
@@ -232,20 +261,15 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
     if constexpr (INTERLEAVED) rope = __ldcs(reinterpret_cast<const uint32_t*>(rp) + lane);
     else rope = uint32_t(__ldcs(reinterpret_cast<const uint16_t*>(rp) + lane)) | uint32_t(__ldcs(reinterpret_cast<const uint16_t*>(rp) + 32 + lane)) << 16;
     const float a = __uint_as_float(rope << 16), b = __uint_as_float(rope & 0xFFFF0000u);
-    const int pos = positions[t], request = batch_indices[t];
-    // (the slot is needed at the end only: the arithmetic does not wait for the walk through the page tables)
-    const long long row = pos < max_pos ? cache_row(request, pos, int(num_pages), page_shift, kv_indices, kv_indptr, batch) : -1;
+    const int pos = __shfl_sync(~0u, at, k & 31);
     const bool rotated = uint32_t(pos) < uint32_t(max_pos);
     const float cs = rotated ? __ldg(cos_sin + (long long)pos * KPE + lane) : 0.f, sn = rotated ? __ldg(cos_sin + (long long)pos * KPE + 32 + lane) : 0.f;
     const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
     auto two = [](uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); };
-    float2 sq[8];
+    float2 sq[2];  // two chains of four
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sq[j] = ptx::mul_f32x2(two(w[j]), two(w[j]));
-#pragma unroll
-    for (int n = 4; n; n >>= 1)
-#pragma unroll
-      for (int j = 0; j < n; ++j) sq[j] = ptx::add_f32x2(sq[j], sq[j + n]);
+    for (int j = 0; j < 8; ++j) sq[j & 1] = j < 2 ? ptx::mul_f32x2(two(w[j]), two(w[j])) : ptx::fma_f32x2(two(w[j]), two(w[j]), sq[j & 1]);
+    sq[0] = ptx::add_f32x2(sq[0], sq[1]);
     float sum = __fadd_rn(sq[0].x, sq[0].y);
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(~0u, sum, o));
@@ -293,6 +317,7 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
       const uint32_t v = reinterpret_cast<const uint32_t*>(&held[j >> 3][threadIdx.x])[j >> 1 & 3];
       return __uint_as_float(j & 1 ? v & 0xFFFF0000u : v << 16);
     });
+    const long long row = __shfl_sync(~0u, places, k & 31);
     if (row < 0) {
       if (lane == 0 && status) *status = 1;
       continue;
