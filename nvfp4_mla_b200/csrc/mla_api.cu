@@ -943,7 +943,7 @@ int nvfp4_mla_norm_rope_append(const void* ckv, int64_t ckv_stride, const void* 
   if (device_info(&d)) return 1;
   const long long warps_per_block = mla::kQuantThreads / 32;
   long long blocks = (nnz + warps_per_block - 1) / warps_per_block;
-  const long long cap = (long long)d->sm_count * 8;  // grid-stride beyond 8 CTAs per SM, twice what is resident (4: 151 us, 8: 150, 32: 155)
+  const long long cap = (long long)d->sm_count * 4;  // what is resident: every CTA makes its tables once
   if (blocks > cap) blocks = cap;
   const auto kernel = interleaved ? mla::mla_norm_rope_append_kernel<true> : mla::mla_norm_rope_append_kernel<false>;
   kernel<<<unsigned(blocks), mla::kQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(

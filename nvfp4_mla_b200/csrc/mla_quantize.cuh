@@ -14,9 +14,9 @@
 // power-of-two rope scale needs no enclosure, its products are exact.
 //
 // 1152 bytes in, 352 bytes out per token, bound by instruction issue and the latency of the walk through the page tables (194 warp
-// instructions per token, 56 % of the issue slots): 274880 tokens in 82 us (63 at the measured copy bandwidth); 100 with one
-// instruction per product instead of two products per instruction and 64-bit rows.
-// Thirty-two tokens per warp with one walk through the page tables for all of them was slower (246.7 us).
+// instructions per token, 56 % of the issue slots): 274880 tokens in 82 us (63 at the measured copy bandwidth; 110 with a power of two as
+// ckv_scale, where more values tie); 100 with one instruction per product instead
+// of two products per instruction and 64-bit rows. Thirty-two tokens per warp with one walk through the page tables for all of them was slower (246.7 us).
 // One warp per token per trip; lane l owns scale block l
 // (channels 16l .. 16l+15: two 16-byte loads, one 8-byte store, the warp writes the token's 256 packed bytes as one
 // contiguous run) and rope channels 2l, 2l+1.
@@ -58,51 +58,81 @@ __device__ __forceinline__ uint32_t e2m1_code(float y) {
 constexpr float kQuantDown = 1.f - 0x1p-21f, kQuantUp = 1.f + 0x1p-21f;
 struct QuantScales {
   float ckv_scale, kpe_scale, six_dn, six_up, kpe_dn, kpe_up;
-  bool fast_sf, fast_kpe, short_ckv;
+  bool fast_sf, fast_kpe;
   __device__ __forceinline__ QuantScales(float ckv, float kpe) : ckv_scale(ckv), kpe_scale(kpe) {
     auto ordinary = [](float d) { return d > 0x1p-100f && d < 0x1p100f; };
     const float six = __fmul_rn(6.0f, ckv), r_six = __frcp_rn(six), r_kpe = __frcp_rn(kpe);
     fast_sf = ordinary(six), fast_kpe = ordinary(kpe);
-    short_ckv = (__float_as_uint(ckv) & 0xFFFFu) == 0u;
     const bool kpe_pow2 = (__float_as_uint(kpe) & 0x007FFFFFu) == 0u;
     six_dn = r_six * kQuantDown, six_up = r_six * kQuantUp;
     kpe_dn = kpe_pow2 ? r_kpe : r_kpe * kQuantDown, kpe_up = kpe_pow2 ? r_kpe : r_kpe * kQuantUp;
   }
 };
 
-// Codes and scale byte of one block of 16 latent values; `value(j)` gives value j again.
+// A factor f for the block scale `sf8` with which every BF16 value x has code(fl(x f)) = code(fl(x / sf)), or 0 if none is found.
+// Both quotients round alike unless x / sf is within 2^-20 of a boundary; a boundary is m 2^k with m = 1, 1.25, 1.5 or 1.75, so only the
+// BF16 number x_m next to m sf can be that close (and its products with powers of two, which behave like it), and the scale alone
+// says whether it is: fl(m sf) is then within 16 units in its last place of a BF16 number. For these m (none for most scales, one or
+// two for amax / (6 * 448) of a BF16 amax, all four where the cache's scale is a power of two) f has to put x_m on the side of m,
+// or on m itself, that the division does; f is the reciprocal or one of the two numbers on either side of it, within 3 * 2^-23 of 1 / sf.
+__device__ __forceinline__ float quant_factor(uint32_t sf8, float ckv_scale) {
+  const float sf = __fmul_rn(e4m3_value(uint8_t(sf8)), ckv_scale);
+  if (!(sf > 0x1p-100f && sf < 0x1p100f)) return 0.f;
+  const uint32_t r = __float_as_uint(__frcp_rn(sf));
+  float x[4];   // x_m, or m itself over ...
+  float q[4];   // ... and its quotient
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t t = __float_as_uint(__fmul_rn(sf, 1.f + 0.25f * i)) + 16u;
+    x[i] = (t & 0xFFFFu) <= 32u ? __uint_as_float(t & 0xFFFF0000u) : 0.f;
+    q[i] = __fdiv_rn(x[i], sf);
+  }
+#pragma unroll
+  for (int j = 0; j < 5; ++j) {
+    const float f = __uint_as_float(r + (j & 1 ? -((j + 1) >> 1) : j >> 1));
+    bool good = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float m = 1.f + 0.25f * i, p = __fmul_rn(x[i], f);
+      good &= (p < m) == (q[i] < m) && (p > m) == (q[i] > m);
+    }
+    if (good) return f;
+  }
+  return 0.f;
+}
+constexpr int kQuantFactors = 128;
+__device__ __forceinline__ void quant_factors(float (&factors)[kQuantFactors], float ckv_scale) {  // (the caller synchronises)
+  if (threadIdx.x < kQuantFactors) factors[threadIdx.x] = quant_factor(threadIdx.x, ckv_scale);
+}
+
+// Codes and scale byte of one block of 16 latent values; `value(j)` gives value j again. With FACTORS one product per value settles its code.
 struct QuantBlock {
   uint32_t lo, hi, sf8;
 };
-template <class Value>
-__device__ __forceinline__ QuantBlock quantize_block(const float (&x)[16], const QuantScales& Q, Value value) {
+template <bool FACTORS, class Value>
+__device__ __forceinline__ QuantBlock quantize_block(const float (&x)[16], const QuantScales& Q, const float* factors, Value value) {
   float amax = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) amax = ptx::max3(amax, fabsf(x[2 * j]), fabsf(x[2 * j + 1]));
   const uint32_t sf2 = f32x2_to_e4m3x2_sat(amax * Q.six_dn, amax * Q.six_up);
   uint32_t sf8 = sf2 & 0xFFu;
   if (!Q.fast_sf || sf8 != sf2 >> 8) sf8 = f32x2_to_e4m3x2_sat(__fdiv_rn(__fdiv_rn(amax, 6.0f), Q.ckv_scale), 0.f) & 0xFFu;
+  if constexpr (FACTORS) {
+    const float f = factors[sf8 & 127u];
+    if (f != 0.f) {
+      float y[16];
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        const float2 p = ptx::mul_f32x2(make_float2(x[j], x[j + 1]), make_float2(f, f));
+        y[j] = p.x, y[j + 1] = p.y;
+      }
+      return {e2m1x8(reinterpret_cast<const float(&)[8]>(y[0])), e2m1x8(reinterpret_cast<const float(&)[8]>(y[8])), sf8};
+    }
+  }
   const float sf = __fmul_rn(e4m3_value(uint8_t(sf8)), Q.ckv_scale);
   uint32_t lo = 0, hi = 0;
   if (sf > 0.f) {
     const float r = __frcp_rn(sf);
-    // A value is this close to a boundary T (mantissa 1, 1.25, 1.5 or 1.75) only where T * sf is that close to a BF16 number, which the
-    // scale alone decides: x * r and fl(x / sf) round alike unless |x - T sf| <= 2^-22 T sf, five units in the last place of
-    // fl(T sf). With eight units of room one block in a thousand is left, unless the cache's scale has few bits.
-    if (!Q.short_ckv) {
-      const float t1 = sf * 1.25f, t2 = sf * 1.5f, t3 = sf * 1.75f;
-      uint32_t nearest = __viaddmin_u16x2(__byte_perm(__float_as_uint(sf), __float_as_uint(t1), 0x5410), 0x00080008u, 0xFFFFFFFFu);
-      nearest = __viaddmin_u16x2(__byte_perm(__float_as_uint(t2), __float_as_uint(t3), 0x5410), 0x00080008u, nearest);
-      if ((nearest & 0xFFFFu) > 16u && nearest >> 16 > 16u && sf > 0x1p-100f && sf < 0x1p100f) {
-        float y[16];
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const float2 p = ptx::mul_f32x2(make_float2(x[j], x[j + 1]), make_float2(r, r));
-          y[j] = p.x, y[j + 1] = p.y;
-        }
-        return {e2m1x8(reinterpret_cast<const float(&)[8]>(y[0])), e2m1x8(reinterpret_cast<const float(&)[8]>(y[8])), sf8};
-      }
-    }
     const float rd = r * kQuantDown, ru = r * kQuantUp;
     float yd[16], yu[16];
 #pragma unroll
@@ -181,7 +211,7 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
     // (a value that has to be settled is read again from memory: the registers cannot be indexed)
-    const QuantBlock q = quantize_block(x, Q, [&](int j) { return __bfloat162float(ckv[t * CKV + 16 * lane + j]); });
+    const QuantBlock q = quantize_block<false>(x, Q, nullptr, [&](int j) { return __bfloat162float(ckv[t * CKV + 16 * lane + j]); });
     *reinterpret_cast<uint2*>(ckv_cache + row * (CKV / 2) + 8 * lane) = make_uint2(q.lo, q.hi);
     sf_cache[row * (CKV / 16) + lane] = uint8_t(q.sf8);
     // ---- rope channels 2 lane, 2 lane + 1
@@ -207,17 +237,13 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 //   rope  : a cos - b sin as fma(a, cos, -p) - fma(b, sin, -p) with p = b sin rounded, which is within two units of the defined number.
 //
 // One warp per token per trip, lane l = scale block l, as above; a lane's normalised BF16 values sit in shared memory for the few that
-// have to be settled, the weights there too. 1512 bytes per token, bound by the latency of a warp's chain of steps (414 warp
-// instructions per token, 65 % of the issue slots): 274880 tokens in 150 us (63 at the measured copy bandwidth; the writer above 82).
-// With the norm in 64 bits throughout it took 345 us, one instruction per value and step 273; fetching the next token's row
-// ahead gained nothing at the registers it took (149), and 24 or 40 warps per SM instead of 32 made it 182 and 176.
+// have to be settled, the weights and the factors of the 128 block scales there too. A lane looks up the place of one of the warp's next
+// 32 tokens, so that the walk through the page tables is paid for once in 32 trips. 1512 bytes per token, bound by instruction issue and
+// the latency of a warp's chain of steps (352 warp instructions per token, 67 % of the issue slots): 274880 tokens in 129 us with
+// ckv_scale = 6.5 / (6 * 448) (63 at the measured copy bandwidth), 172 with a power of two, where a third of the block scales has no
+// factor. Before: 166 and 188 with the enclosing products of the writer above and a walk per token; 345 with the norm in 64 bits
+// throughout. Rows fetched ahead into shared memory (134), 40 warps per SM (171) and two CTAs per resident one (129.5) gained nothing.
 // ---------------------------------------------------------------------------------------------------------------
-// whether the fp32 number y, off by at most `units` in its last place, may round to another BF16 number than what it stands for: its low
-// half is within `units` of 0x8000
-__device__ __forceinline__ bool near_bf16_border(float y, uint32_t units) {
-  return ((__float_as_uint(y) - 0x8000u + units) & 0xFFFFu) <= 2 * units;
-}
-
 template <bool INTERLEAVED>
 __global__ void __launch_bounds__(kQuantThreads, 4)
 mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv_stride, const __nv_bfloat16* __restrict__ kpe,
@@ -229,6 +255,7 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
                             float kpe_scale, int* status) {
   __shared__ uint4 held[2][kQuantThreads];  // a lane's 16 normalised values
   __shared__ float4 gains[4][32];           // the weights: lane l's 16
+  __shared__ float factors[kQuantFactors];
   const int lane = threadIdx.x & 31;
   const QuantScales Q(ckv_scale, kpe_scale);
   const float eps_f = float(eps);
@@ -240,14 +267,15 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
     reinterpret_cast<float*>(&gains[(i & 15) >> 2][i >> 4])[i & 3] = g;
     ordinary_gains &= g == 0.f || (fabsf(g) > 0x1p-20f && fabsf(g) < 0x1p20f);
   }
+  quant_factors(factors, ckv_scale);
   ordinary_gains = __syncthreads_and(ordinary_gains);
   const long long warp0 = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   const long long stride = (long long)gridDim.x * (kQuantThreads / 32);
   // A lane looks up the place of one of the warp's next 32 tokens: one walk through the page tables for all of them.
   int places = -1, at = 0;
-  int k = 0;
-  for (long long t = warp0; t < nnz; t += stride, ++k) {
-    if ((k & 31) == 0) {
+  int trip = 0;
+  for (long long t = warp0; t < nnz; t += stride, ++trip) {
+    if ((trip & 31) == 0) {
       const long long mine = t + lane * stride;
       if (mine < nnz) {
         at = positions[mine];
@@ -261,7 +289,7 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
     if constexpr (INTERLEAVED) rope = __ldcs(reinterpret_cast<const uint32_t*>(rp) + lane);
     else rope = uint32_t(__ldcs(reinterpret_cast<const uint16_t*>(rp) + lane)) | uint32_t(__ldcs(reinterpret_cast<const uint16_t*>(rp) + 32 + lane)) << 16;
     const float a = __uint_as_float(rope << 16), b = __uint_as_float(rope & 0xFFFF0000u);
-    const int pos = __shfl_sync(~0u, at, k & 31);
+    const int pos = __shfl_sync(~0u, at, trip & 31);
     const bool rotated = uint32_t(pos) < uint32_t(max_pos);
     const float cs = rotated ? __ldg(cos_sin + (long long)pos * KPE + lane) : 0.f, sn = rotated ? __ldg(cos_sin + (long long)pos * KPE + 32 + lane) : 0.f;
     const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
@@ -313,11 +341,11 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
     float x[16];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[2 * j] = two(held_[j]).x, x[2 * j + 1] = two(held_[j]).y;
-    const QuantBlock q = quantize_block(x, Q, [&](int j) {
+    const QuantBlock q = quantize_block<true>(x, Q, factors, [&](int j) {
       const uint32_t v = reinterpret_cast<const uint32_t*>(&held[j >> 3][threadIdx.x])[j >> 1 & 3];
       return __uint_as_float(j & 1 ? v & 0xFFFF0000u : v << 16);
     });
-    const long long row = __shfl_sync(~0u, places, k & 31);
+    const long long row = __shfl_sync(~0u, places, trip & 31);
     if (row < 0) {
       if (lane == 0 && status) *status = 1;
       continue;
@@ -326,8 +354,10 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
     sf_cache[row * (CKV / 16) + lane] = uint8_t(q.sf8);
     const float p0 = __fmul_rn(b, sn), p1 = __fmul_rn(a, sn);
     float x0 = __fsub_rn(__fmaf_rn(a, cs, -p0), __fmaf_rn(b, sn, -p0)), x1 = __fadd_rn(__fmaf_rn(b, cs, p1), __fmaf_rn(a, sn, -p1));
-    const bool tiny = fabsf(x0) < 0x1p-60f || fabsf(x1) < 0x1p-60f;  // (the products' errors may be below fp32's range)
-    if (near_bf16_border(x0, 3) || near_bf16_border(x1, 3) || tiny || !(fabsf(x0) < 0x1p100f && fabsf(x1) < 0x1p100f)) {
+    // (very small: the products' errors may be below fp32's range; very large or NaN: something may have overflowed)
+    const bool odd = fminf(fabsf(x0), fabsf(x1)) < 0x1p-60f || !(fabsf(x0) + fabsf(x1) < 0x1p100f);
+    const uint32_t border = __viaddmin_u16x2(__byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x5410), 0x80038003u, 0xFFFFFFFFu);
+    if ((border & 0xFFFFu) <= 6u || border >> 16 <= 6u || odd) {
       const double da = double(a), db = double(b), dc = double(cs), ds = double(sn);
       x0 = float(fma(da, dc, -(db * ds))), x1 = float(fma(db, dc, da * ds));
     }

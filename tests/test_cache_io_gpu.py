@@ -76,6 +76,21 @@ def test_values_of_unequal_size_and_separate_rows():
             assert torch.equal(got, exp)
 
 
+@pytest.mark.parametrize("scale", [1.0, 0.25, 6.5 / 2688, 1 / 448, 3.140625 / 2688, 0.0031, 1e-37, 3e38])
+def test_codes_at_every_block_scale(scale):
+    """Scales of the cache that make ties everywhere, somewhere and nowhere; rows of sizes that reach every block scale; more tokens than
+    a warp looks up at a time."""
+    kv_a, weight, cos_sin, b, pos, cache, kv_indices, kv_indptr = rows([160000, 3], [0, 5], 64)
+    weight[:] = (torch.arange(512, device="cuda") // 16 - 16).float().exp2().bfloat16()  # block j of a row is scaled by 2^(j - 16)
+    want = tuple(t.clone() for t in cache)
+    ckv, kpe = normed(kv_a, weight, cos_sin, pos, 1e-6, True)
+    mla.quantize_append_paged_mla_kv_cache(ckv, kpe, b, pos, *want, kv_indices, kv_indptr, None, scale, 0.02)
+    mla.norm_rope_append_paged_mla_kv_cache(kv_a[:, :512], kv_a[:, 512:], weight, cos_sin, b, pos, *cache, kv_indices, kv_indptr, ckv_scale=scale,
+                                            kpe_scale=0.02, check=True)
+    for got, exp in zip(raw(cache), raw(want)):
+        assert torch.equal(got, exp)
+
+
 def test_products_below_the_range_of_fp32():
     """Channels whose product with the weight is below fp32's normal numbers, the normalised value and the cache's scale above."""
     kv_a, weight, cos_sin, b, pos, cache, kv_indices, kv_indptr = rows([200], [0], 64)
