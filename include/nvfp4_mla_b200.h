@@ -123,14 +123,16 @@ NVFP4_MLA_API int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, 
  * position; with window > 0 to the last `window` of these, itself among them, and to the first `sink_tokens`.
  *
  *   q_nope, q_pe  [total_q, heads, 512] and [total_q, heads, 64] bfloat16;  out [total_q, heads, 512] bfloat16
- *   qo_indptr     [batch + 1] int32, non-decreasing, read on the device; NULL: one query token per request (total_q = batch). Query tokens of no request (before qo_indptr[0], at or
- *                 behind qo_indptr[batch]) and tokens in front of a request's first (more new tokens than kv_lens) give zeros
+ *   qo_indptr     [batch + 1] int32, non-decreasing, read on the device; NULL: one query token per request (total_q = batch). Query
+ *                 tokens of no request (before qo_indptr[0], at or behind qo_indptr[batch]) and tokens in front of a request's first
+ *                 (more new tokens than kv_lens) give zeros
  *   window        0: none
  *   others        as in nvfp4_mla_decode_window; 16-bit arithmetic; any number of heads
  *
- * Where it is estimated to be faster (nvfp4_mla_extend_shares: 1, 0: not, -1: error; in the main chunks of more than a few tokens), all
- * rows of a request share one pass over its cache, which is dequantised once into the workspace: 1152 bytes per visible token, of which there are at most batch * max_kv_len (and with a window at most
- * batch * (window + sink_tokens + 256) + total_q), and as many requests at a time as keep this below 8 GB.
+ * Where it is estimated to be faster (nvfp4_mla_extend_shares: 1, 0: not, -1: error; in the main chunks of more than a few tokens),
+ * all rows of a request share one pass over its cache, which is dequantised once into the workspace: 1152 bytes per visible token,
+ * of which there are at most batch * max_kv_len (and with a window at most batch * (window + sink_tokens + 256) + total_q), and as
+ * many requests at a time as keep this below 8 GB.
  * (No counterpart in the reference, which decodes one query token per request.) */
 NVFP4_MLA_API int nvfp4_mla_extend_shares(int batch, int total_q, int heads, int max_kv_len, int window, int sink_tokens);
 NVFP4_MLA_API int64_t nvfp4_mla_extend_workspace_bytes(int batch, int total_q, int heads, int page_size, int page_table_width, int max_kv_len,

@@ -239,7 +239,7 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 // One warp per token per trip, lane l = scale block l, as above; a lane's normalised BF16 values sit in shared memory for the few that
 // have to be settled, the weights and the factors of the 128 block scales there too. A lane looks up the place of one of the warp's next
 // 32 tokens, so that the walk through the page tables is paid for once in 32 trips. 1512 bytes per token, bound by instruction issue and
-// the latency of a warp's chain of steps (352 warp instructions per token, 67 % of the issue slots): 274880 tokens in 129 us with
+// the latency of a warp's chain of steps (348 warp instructions per token, 67 % of the issue slots): 274880 tokens in 129 us with
 // ckv_scale = 6.5 / (6 * 448) (63 at the measured copy bandwidth), 172 with a power of two, where a third of the block scales has no
 // factor. Before: 166 and 188 with the enclosing products of the writer above and a walk per token; 345 with the norm in 64 bits
 // throughout. Rows fetched ahead into shared memory (134), 40 warps per SM (171) and two CTAs per resident one (129.5) gained nothing.
