@@ -271,3 +271,61 @@ def test_more_requests_than_are_scheduled_at_once():
         want = attention64(c.q_nope[at:at + q_lens[b]], c.q_pe[at:at + q_lens[b]], c.cache, c.page_table[b:b + 1], [kv_lens[b]], [q_lens[b]], SM_SCALE, c.ckv_scale, c.kpe_scale)
         assert worst_row(out[at:at + q_lens[b]], want) <= ROW_TOL
     assert not out.isnan().any() and mla.workspace_status() == 0
+
+
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1), (2 ** 31 - 1, 0), (30, 5000)])
+@pytest.mark.parametrize("q_lens", [[2, 1, 3], [200, 1, 130]])
+def test_windows_and_first_tokens_beyond_every_length(q_lens, window, sinks):
+    c = chunk([700, 64, 150], q_lens, 16, 64)
+    assert worst_row(run(c, window=window, sink_tokens=sinks, max_kv_len=None), reference(c, window, sinks)) <= ROW_TOL
+    last = c.indptr[1:].long() - 1
+    out = mla.decode_window(c.q_nope[last].contiguous(), c.q_pe[last].contiguous(), *c.cache, c.page_table, c.kv_lens, SM_SCALE, window, sinks,
+                            c.ckv_scale, c.kpe_scale)
+    assert worst_row(out, reference(c, window, sinks)[last]) <= ROW_TOL
+    assert mla.workspace_status() == 0
+
+
+@pytest.mark.parametrize("heads", [16, 64])
+def test_single_tokens_of_more_requests_than_a_slice_takes(heads):
+    """1100 requests of one new token, and padding behind them."""
+    kv_lens = [1 + 7 * i % 2000 for i in range(1100)]
+    c = chunk(kv_lens, [1] * 1100, heads, 16, pad=30)
+    for kw in (dict(), dict(window=150, sink_tokens=20)):
+        out = run(c, **kw)
+        assert worst_row(out[:-30], reference(c, kw.get("window", 0), kw.get("sink_tokens", 0))) <= ROW_TOL and (out[-30:] == 0).all()
+    assert mla.workspace_status() == 0
+
+
+def test_window_decode_captured_and_replayed_beside_another_stream():
+    """A graph of two windowed decodes that share its pool, replayed with other lengths and pages while the call runs on another stream."""
+    c = chunk([3000, 900, 64, 1], [1] * 4, 16, 64)
+    d = chunk([500] * 4, [1] * 4, 64, 64, seed=7)
+    kv_lens = c.kv_lens.clone()
+
+    def call(x, lens, window, sinks):
+        return mla.decode_window(x.q_nope, x.q_pe, *x.cache, x.page_table, lens, SM_SCALE, window, sinks, x.ckv_scale, x.kpe_scale)
+
+    call(c, kv_lens, 100, 4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first, second = call(c, kv_lens, 100, 4), call(c, kv_lens, 1000, 0)
+    other = torch.cuda.Stream()
+    for lens in ([3000, 900, 64, 1], [17, 0, 30, 1], [2999, 101, 5, 0]):
+        c.lens = lens
+        kv_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(other):
+            beside = [call(d, d.kv_lens, 200, 9) for _ in range(3)]
+        torch.cuda.synchronize()
+        c.q_lens = [min(n, 1) for n in lens]
+        live = [i for i, n in enumerate(lens) if n]
+        for out, window, sinks in ((first, 100, 4), (second, 1000, 0)):
+            want = attention64(c.q_nope[live], c.q_pe[live], c.cache, c.page_table[live], [lens[i] for i in live], [1] * len(live), SM_SCALE, c.ckv_scale,
+                               c.kpe_scale, window, sinks)
+            assert worst_row(out[live], want) <= ROW_TOL
+            assert all((out[i] == 0).all() for i, n in enumerate(lens) if not n)
+        for out in beside:
+            assert worst_row(out, reference(d, 200, 9)) <= ROW_TOL
+    assert mla.workspace_status() == 0
