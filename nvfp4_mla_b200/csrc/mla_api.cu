@@ -22,7 +22,6 @@
 #include "mla_gather.cuh"
 #include "mla_quantize.cuh"
 #include "mla_schedule.cuh"
-#include "mla_window.cuh"
 
 namespace {
 
@@ -108,14 +107,20 @@ int schedule_units(const DeviceInfo& d, int precision, int hpc) {
 }
 int ctas_per_unit(int hpc) { return runs_on_pairs(hpc) ? 2 : 1; }
 // the kernels that take tensor maps (all but the 16-bit heads-as-M kernel)
-DecodeKernel decode_kernel(int precision, int hpc, bool window = false) {
+DecodeKernel decode_kernel(int precision, int hpc, int map = mla::kMapNone) {
   if (precision == NVFP4_MLA_PRECISION_FP8)
     return hpc == 128  ? mla::mla_decode_hm_kernel<kRawSlotsHm>
            : hpc == 32 ? mla::mla_decode_kernel<32, kRawSlots8, true>
                        : mla::mla_decode_kernel<16, kRawSlots8, true>;
-  return window ? mla::mla_decode_vt_kernel<true> : mla::mla_decode_vt_kernel<false>;
+  return map == mla::kMapChunk    ? mla::mla_decode_vt_kernel<mla::kMapChunk>
+         : map == mla::kMapWindow ? mla::mla_decode_vt_kernel<mla::kMapWindow>
+                                  : mla::mla_decode_vt_kernel<mla::kMapNone>;
 }
-auto hm16_kernel(bool window) { return window ? mla::mla_decode_hm16_kernel<true> : mla::mla_decode_hm16_kernel<false>; }
+auto hm16_kernel(int map) {
+  return map == mla::kMapChunk    ? mla::mla_decode_hm16_kernel<mla::kMapChunk>
+         : map == mla::kMapWindow ? mla::mla_decode_hm16_kernel<mla::kMapWindow>
+                                  : mla::mla_decode_hm16_kernel<mla::kMapNone>;
+}
 unsigned decode_threads(int precision, int hpc) {
   if (precision == NVFP4_MLA_PRECISION_FP8) return hpc == 128 ? mla::kHmThreads : mla::kDecodeThreads;
   return hpc > 16 ? mla::kH16Threads : mla::kVtThreads;
@@ -127,9 +132,9 @@ size_t decode_smem(int precision, int hpc) {
                        : mla::decode_smem_bytes<16, kRawSlots8, true>();
   return hpc > 16 ? mla::h16_smem_bytes() : mla::vt_smem_bytes();
 }
-const void* decode_entry(int precision, int hpc, bool window = false) {
-  if (precision != NVFP4_MLA_PRECISION_FP8 && hpc > 16) return reinterpret_cast<const void*>(hm16_kernel(window));
-  return reinterpret_cast<const void*>(decode_kernel(precision, hpc, window));
+const void* decode_entry(int precision, int hpc, int map = mla::kMapNone) {
+  if (precision != NVFP4_MLA_PRECISION_FP8 && hpc > 16) return reinterpret_cast<const void*>(hm16_kernel(map));
+  return reinterpret_cast<const void*>(decode_kernel(precision, hpc, map));
 }
 static_assert(mla::h16_smem_bytes() <= 232448, "16-bit heads-as-M kernel exceeds the shared memory a CTA can opt in to");
 static_assert(mla::hm_smem_bytes<kRawSlotsHm>() <= 232448, "heads-as-M kernel exceeds the shared memory a CTA can opt in to");
@@ -154,8 +159,9 @@ int device_info(DeviceInfo** out) {
         MLA_CUDA(cudaFuncSetAttribute(decode_entry(prec, hpc), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       int(decode_smem(prec, hpc))));
     for (int hpc : {16, 128})
-      MLA_CUDA(cudaFuncSetAttribute(decode_entry(NVFP4_MLA_PRECISION_BF16, hpc, true), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    int(decode_smem(NVFP4_MLA_PRECISION_BF16, hpc))));
+      for (int map : {mla::kMapWindow, mla::kMapChunk})
+        MLA_CUDA(cudaFuncSetAttribute(decode_entry(NVFP4_MLA_PRECISION_BF16, hpc, map), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      int(decode_smem(NVFP4_MLA_PRECISION_BF16, hpc))));
     MLA_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(mla::mla_extend_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   int(mla::ext_smem_bytes())));
     // clusters of two need both SMs in one GPC: ask how many can be resident rather than assuming sm_count / 2
@@ -265,7 +271,7 @@ int problem_of(int batch, int heads, int max_kv_len, int num_splits, int n_cta, 
   const long long chunk = ((len + splits - 1) / splits + mla::TILE - 1) / mla::TILE * mla::TILE;
   pb->batch = batch, pb->heads = heads, pb->heads_per_cta = hpc, pb->head_groups = (heads + hpc - 1) / hpc;
   pb->splits = splits, pb->chunk = int(chunk), pb->n_cta = n_cta;
-  pb->window = 0, pb->sinks = 0, pb->page_shift = 0, pb->pt_width = 0;
+  pb->map = mla::kMapNone, pb->window = 0, pb->sinks = 0, pb->page_shift = 0, pb->pt_width = 0, pb->requests = 0, pb->q_first = 0, pb->q_indptr = nullptr;
   MLA_CHECK((long long)batch * splits <= mla::kSchedMaxBZ, "batch * num_splits = %lld exceeds %d", (long long)batch * splits,
             mla::kSchedMaxBZ);
   MLA_CHECK(splits + n_cta <= 512, "num_splits %d too large (at most %d)", splits, 512 - n_cta);
@@ -327,22 +333,24 @@ int64_t nvfp4_mla_decode_workspace_bytes(int batch, int heads, int num_splits) {
 }
 
 // The decode call proper; `heads` counts the rows of all q_len query tokens of a request, `hpc_limit` caps the heads per CTA
-// (see heads_per_cta), which are chosen for requests of `expected_kv_len` tokens (0: of the bound max_kv_len). `dead`: the tokens of
-// each request that are not seen (kernels with WINDOW, 16-bit mode), or null; `window`: a sliding window, the page table's width with it;
-// `status`: where the kernels report, or null for the workspace's first word.
+// (see heads_per_cta), which are chosen for requests of `expected_kv_len` tokens (0: of the bound max_kv_len). `window`: a sliding
+// window; `q_indptr`: the batch's entries are query tokens from q_first on of `requests` requests (Problem, mla_common.cuh); both in the
+// 16-bit mode and with the page table's width. `status`: where the kernels report, or null for the workspace's first word.
 static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache,
                        const uint8_t* kpe_cache, int64_t num_pages, int page_size, const int32_t* page_table,
                        int64_t page_table_stride, const int32_t* kv_lens, int batch, int heads, float sm_scale, float ckv_scale,
                        float kpe_scale, int max_kv_len, int num_splits, int precision, void* out, float* out_f32, float* lse,
                        void* workspace, int64_t workspace_bytes, void* stream, int hpc_limit, int q_len = 1, int expected_kv_len = 0,
-                       const int2* dead = nullptr, int* status = nullptr, int window = 0, int sinks = 0, int pt_width = 0) {
+                       int* status = nullptr, int window = 0, int sinks = 0, int pt_width = 0, const int* q_indptr = nullptr, int requests = 0,
+                       int q_first = 0) {
   g_error[0] = 0;
+  const int map = q_indptr ? mla::kMapChunk : window > 0 ? mla::kMapWindow : mla::kMapNone;
   MLA_CHECK(precision == NVFP4_MLA_PRECISION_BF16 || precision == NVFP4_MLA_PRECISION_FP8,
             "precision must be 0 (bf16) or 1 (fp8), got %d", precision);
   MLA_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0, "page_size must be a power of two, got %d", page_size);
   MLA_CHECK(num_pages > 0 && num_pages * page_size < (int64_t(1) << 31), "num_pages * page_size must be in [1, 2^31)");
   MLA_CHECK(ckv_scale > 0.f && kpe_scale > 0.f, "ckv_scale and kpe_scale must be positive");
-  MLA_CHECK(q_nope && q_pe && ckv_cache && ckv_sf_cache && kpe_cache && (page_table || (window > 0 && pt_width == 0)) && kv_lens && workspace,
+  MLA_CHECK(q_nope && q_pe && ckv_cache && ckv_sf_cache && kpe_cache && (page_table || (map != mla::kMapNone && pt_width == 0)) && kv_lens && workspace,
             "null pointer argument");
   MLA_CHECK(out || out_f32 || lse, "at least one of out, out_f32 and lse must be given");
   MLA_CHECK(aligned(q_nope, 16) && aligned(q_pe, 16) && aligned(ckv_cache, 16) && aligned(ckv_sf_cache, 16) &&
@@ -355,8 +363,10 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   const int hpc = heads_per_cta(heads, precision, *d, hpc_limit, batch, expected_kv_len > 0 ? expected_kv_len : max_kv_len);
   if (problem_of(batch, heads, max_kv_len, num_splits, schedule_units(*d, precision, hpc), hpc, &pb)) return 1;
   if (batch == 0) return 0;
-  if (window > 0) pb.window = window, pb.sinks = sinks, pb.page_shift = __builtin_ctz(unsigned(page_size)), pb.pt_width = pt_width;
-  const bool windowed = dead || window > 0;
+  if (map != mla::kMapNone) {
+    pb.map = map, pb.window = window, pb.sinks = sinks, pb.page_shift = __builtin_ctz(unsigned(page_size)), pb.pt_width = pt_width;
+    pb.requests = requests, pb.q_first = q_first, pb.q_indptr = q_indptr;
+  }
   const mla::WsLayout L = mla::ws_layout(pb.n_cta, pb.items(), pb.heads_per_cta);
   MLA_CHECK(workspace_bytes >= int64_t(L.total), "workspace too small: %lld bytes given, %lld needed", (long long)workspace_bytes,
             (long long)L.total);
@@ -395,15 +405,15 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   P.sm_scale_log2 = sm_scale * 1.4426950408889634f, P.ckv_scale = ckv_scale, P.kpe_scale = kpe_scale;
   P.cta_range = cta_range, P.segs = segs, P.lse_part = lse_part, P.o_part = o_part, P.header = header;
   P.kv_lens = kv_lens, P.pb = pb, P.inline_sched = inline_sched ? 1 : 0, P.item_range = item_range;
-  P.cta_range_out = cta_range, P.segs_out = segs, P.dead = dead;
+  P.cta_range_out = cta_range, P.segs_out = segs;
   if (status) P.header = status;
   Profile* prof = g_profile && g_profile->used < int(g_profile->start.size()) ? g_profile : nullptr;
   if (prof) MLA_CUDA(cudaEventRecord(prof->start[prof->used], st));
   const dim3 grid(pb.n_cta * ctas_per_unit(hpc)), block(decode_threads(precision, hpc));
   if (hm16)
-    MLA_CUDA(launch_dependent(hm16_kernel(windowed), grid, block, decode_smem(precision, hpc), st, P));
+    MLA_CUDA(launch_dependent(hm16_kernel(map), grid, block, decode_smem(precision, hpc), st, P));
   else
-    MLA_CUDA(launch_dependent_cluster(decode_kernel(precision, hpc, windowed), grid, block, decode_smem(precision, hpc), st,
+    MLA_CUDA(launch_dependent_cluster(decode_kernel(precision, hpc, map), grid, block, decode_smem(precision, hpc), st,
                                       unsigned(ctas_per_unit(hpc)), ckv_map, sf_map, kpe_map, P));
   if (prof) MLA_CUDA(cudaEventRecord(prof->stop[prof->used++], st));
 
@@ -464,12 +474,10 @@ int nvfp4_mla_decode_multi(const void* q_nope, const void* q_pe, const uint8_t* 
 }
 
 // ---- a few query tokens as requests ------------------------------------------------------------------------------------
-// Workspace: the decode call's | page tables of the visible pages | lengths | unseen intervals
 namespace {
 struct WindowLayout {
-  size_t decode, table, lens, dead, total;
-  int width;     // pages of a request that can be visible
-  int max_len;   // bound of the lengths in them
+  size_t total;  // the decode call's workspace
+  int max_len;   // bound of the tokens in the pages of a request that can be visible
 };
 int window_layout(int batch, int heads, int page_size, int page_table_width, int max_kv_len, int window, int sinks, WindowLayout* l) {
   MLA_CHECK(batch >= 0, "batch must be non-negative");
@@ -481,14 +489,9 @@ int window_layout(int batch, int heads, int page_size, int page_table_width, int
   // the first tokens' pages, the window's (one more than its tokens fill: it need not start on a page), and the one between
   // where the two meet
   const int64_t pages = window == 0 ? page_table_width : (int64_t(sinks) + page_size - 1) / page_size + (int64_t(window) + page_size - 1) / page_size + 2;
-  l->width = int(pages < page_table_width ? pages : page_table_width);
-  const int64_t len = int64_t(l->width) * page_size;
-  l->max_len = int(len < max_kv_len ? len : max_kv_len);
-  l->decode = 0;
-  l->table = mla::align_up(size_t(bytes), 256);
-  l->lens = mla::align_up(l->table + size_t(batch) * l->width * 4, 256);
-  l->dead = mla::align_up(l->lens + size_t(batch) * 4, 256);
-  l->total = mla::align_up(l->dead + size_t(batch) * 8, 256);
+  const int64_t len = std::min<int64_t>(pages, page_table_width) * page_size;
+  l->max_len = int(std::min<int64_t>(len, max_kv_len));
+  l->total = mla::align_up(size_t(bytes), 256);
   return 0;
 }
 }  // namespace
@@ -625,21 +628,13 @@ int extend_by_token(const void* q_nope, const void* q_pe, const uint8_t* ckv_cac
                     int64_t num_pages, int page_size, const int32_t* page_table, int64_t page_table_stride, int page_table_width,
                     const int32_t* kv_lens, const int32_t* qo_indptr, int batch, int total_q, int heads, float sm_scale, float ckv_scale,
                     float kpe_scale, int window, int sink_tokens, void* out, uint8_t* ws, const WindowLayout& l, int32_t* status, void* stream) {
-  int* table = reinterpret_cast<int*>(ws + l.table);
-  int* lens = reinterpret_cast<int*>(ws + l.lens);
-  int2* dead = reinterpret_cast<int2*>(ws + l.dead);
-  constexpr int per_block = mla::kWindowThreads / 32;
   for (int i = 0; i < total_q; i += kExtendSlice) {
     const int n = total_q - i < kExtendSlice ? total_q - i : kExtendSlice;
-    mla::mla_window_plan_kernel<<<unsigned((n + per_block - 1) / per_block), mla::kWindowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        page_table, page_table_stride, page_table_width, kv_lens, mla::ChunkTokens{qo_indptr, batch, i}, n, __builtin_ctz(unsigned(page_size)),
-        window, sink_tokens, l.width, table, lens, dead);
-    MLA_CUDA(cudaGetLastError());
     const size_t row = size_t(i) * heads;
     if (decode_impl(static_cast<const uint16_t*>(q_nope) + row * mla::CKV, static_cast<const uint16_t*>(q_pe) + row * mla::KPE, ckv_cache,
-                    ckv_sf_cache, kpe_cache, num_pages, page_size, table, l.width, lens, n, heads, sm_scale, ckv_scale, kpe_scale, l.max_len, 0,
-                    NVFP4_MLA_PRECISION_BF16, static_cast<uint16_t*>(out) + row * mla::CKV, nullptr, nullptr, ws, int64_t(l.table), stream,
-                    128, 1, 0, dead, status))
+                    ckv_sf_cache, kpe_cache, num_pages, page_size, page_table, page_table_stride, kv_lens, n, heads, sm_scale, ckv_scale, kpe_scale,
+                    l.max_len, 0, NVFP4_MLA_PRECISION_BF16, static_cast<uint16_t*>(out) + row * mla::CKV, nullptr, nullptr, ws, int64_t(l.total),
+                    stream, 128, 1, 0, status, window, sink_tokens, page_table_width, qo_indptr, batch, i))
       return 1;
   }
   return 0;
@@ -750,8 +745,8 @@ int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, const uint8_t*
                             kv_lens, nullptr, batch, batch, heads, sm_scale, ckv_scale, kpe_scale, max_kv_len, window, sink_tokens, out, workspace,
                             workspace_bytes, status, stream);
   return decode_impl(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, num_pages, page_size, page_table, page_table_stride, kv_lens, batch, heads,
-                     sm_scale, ckv_scale, kpe_scale, l.max_len, 0, NVFP4_MLA_PRECISION_BF16, out, out_f32, lse, workspace, int64_t(l.table), stream,
-                     128, 1, 0, nullptr, status, window, sink_tokens, page_table_width);
+                     sm_scale, ckv_scale, kpe_scale, l.max_len, 0, NVFP4_MLA_PRECISION_BF16, out, out_f32, lse, workspace, int64_t(l.total), stream,
+                     128, 1, 0, status, window, sink_tokens, page_table_width);
 }
 
 // ---- decode without caller-provided scratch -----------------------------------------------------------------------

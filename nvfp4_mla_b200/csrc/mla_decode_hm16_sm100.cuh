@@ -84,11 +84,11 @@ __device__ __forceinline__ bool h16_wait_converted(H16Smem& s, uint32_t tiles) {
   }
   return true;
 }
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ void h16_prefetch_rows(const DecodeParams& P, const Seg& seg, const WindowMap& win, int t, int cg, int lane) {
   const int tok = seg.tok0 + t * kH16Tile + kH16Own * cg + lane;
   if (tok >= seg.tok_end) return;
-  const int pi = tok >> P.page_shift, page = P.page_table[(long long)seg.b * P.pt_stride + (WINDOW ? win.page(pi) : pi)];
+  const int pi = tok >> P.page_shift, page = P.page_table[(long long)(MAP == kMapChunk ? win.request : seg.b) * P.pt_stride + (MAP ? win.page(pi) : pi)];
   if (uint32_t(page) >= uint32_t(P.num_pages)) return;
   const int in_page = tok & ((1 << P.page_shift) - 1);
   const long long row = ((long long)page << P.page_shift) + in_page;
@@ -100,7 +100,7 @@ __device__ __forceinline__ void h16_prefetch_rows(const DecodeParams& P, const S
     ptx::bulk_prefetch_l2(P.sf + row * 32, run * 32);
   }
 }
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams& P, int n_segs, uint32_t& it, int cg) {
   const int lane = ptx::lane_id();
   for (int si = 0; si < n_segs; ++si) {
@@ -108,13 +108,13 @@ __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams
     const int nt = h16_tiles(seg);
     if (nt <= 0) continue;
     WindowMap win = {};
-    if constexpr (WINDOW) win = seg_window(P, seg.b);
+    if constexpr (MAP != kMapNone) win = seg_window<MAP>(P, seg.b);
     if (it == 0)
-      for (int t = 1; t < kH16Ahead && t < nt; ++t) h16_prefetch_rows<WINDOW>(P, seg, win, t, cg, lane);
+      for (int t = 1; t < kH16Ahead && t < nt; ++t) h16_prefetch_rows<MAP>(P, seg, win, t, cg, lane);
     const int t_next = nt > kH16Ahead ? nt - kH16Ahead : 0;
     for (int t = 0; t < nt; ++t, ++it) {
       if (!__all_sync(~0u, h16_wait_converted(s, it))) return;
-      if (t + kH16Ahead < nt) h16_prefetch_rows<WINDOW>(P, seg, win, t + kH16Ahead, cg, lane);
+      if (t + kH16Ahead < nt) h16_prefetch_rows<MAP>(P, seg, win, t + kH16Ahead, cg, lane);
       if (t == t_next)  // the next segment's query rows and first tiles
         for (int sj = si + 1; sj < n_segs; ++sj) {
           const Seg nx = s.segs[sj];
@@ -126,8 +126,8 @@ __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams
             ptx::prefetch_l2(i < nr * 8 ? reinterpret_cast<const char*>(P.q_nope + row0 * CKV) + i * 128
                                         : reinterpret_cast<const char*>(P.q_pe + row0 * KPE) + (i - nr * 8) * 128);
           WindowMap nx_win = {};
-          if constexpr (WINDOW) nx_win = seg_window(P, nx.b);
-          for (int t2 = 0; t2 < kH16Ahead && t2 < nn; ++t2) h16_prefetch_rows<WINDOW>(P, nx, nx_win, t2, cg, lane);
+          if constexpr (MAP != kMapNone) nx_win = seg_window<MAP>(P, nx.b);
+          for (int t2 = 0; t2 < kH16Ahead && t2 < nn; ++t2) h16_prefetch_rows<MAP>(P, nx, nx_win, t2, cg, lane);
           break;
         }
     }
@@ -144,7 +144,7 @@ __device__ __forceinline__ void h16_prefetch_role(H16Smem& s, const DecodeParams
 // there the block becomes 0, and the token's rope part, which only enters scores, NaN. The loads of tile t + 1 are issued as soon as tile t's bytes have
 // been converted, the page ids of tile t + 2 behind them.
 // ---------------------------------------------------------------------------------------------------------------
-template <bool part_a, bool WINDOW>  // whether the warp's panel belongs to part A
+template <bool part_a, int MAP>  // whether the warp's panel belongs to part A
 __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams& P, int n_segs, uint32_t& it) {
   const int lane = ptx::lane_id();
   const int cw = (threadIdx.x >> 5) - 8, w = cw & 7, v = cw >> 3, hh = lane & 1;
@@ -166,8 +166,9 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
     if (nt <= 0) continue;
     const int* pt = P.page_table + (long long)seg.b * P.pt_stride;
     WindowMap win = {};
-    if constexpr (WINDOW) win = seg_window(P, seg.b);
-    const int2 dead = WINDOW ? win.dead : make_int2(0, 0);  // tokens that no row sees: they read as zeros
+    if constexpr (MAP != kMapNone) win = seg_window<MAP>(P, seg.b);
+    if constexpr (MAP == kMapChunk) pt = P.page_table + (long long)win.request * P.pt_stride;
+    const int2 dead = MAP ? win.dead : make_int2(0, 0);  // tokens that no row sees: they read as zeros
     const int first_masked = P.q_len > 1 ? P.kv_lens[seg.b] - (P.q_len - 1) : INT_MAX;  // first token that some row does not see
     uint4 rw[2];
     uint32_t rs[2];
@@ -179,13 +180,13 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
     // their bytes are used, and the fetches past the last tile are issued like the others.
     auto fetch_id = [&](int tk) {
       const int pi = (tk < seg.tok_end ? tk : seg.tok_end - 1) >> P.page_shift;
-      return __ldg(pt + (WINDOW ? win.page(pi) : pi));
+      return __ldg(pt + (MAP ? win.page(pi) : pi));
     };
     auto fetch_rows = [&](int page) {
       const bool live = tok < seg.tok_end, good = uint32_t(page) < uint32_t(P.num_pages);
       // a stale or corrupt id is never dereferenced: the row reads as zeros and the call is flagged
       if (live && !good) atomicExch(P.header, int(kBadPage));
-      const bool seen = live && (!WINDOW || tok < dead.x || tok >= dead.y);
+      const bool seen = live && (!MAP || tok < dead.x || tok >= dead.y);
       const int row = seen && good ? (page << P.page_shift) + (tok & ((1 << P.page_shift) - 1)) : -1;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -265,10 +266,10 @@ __device__ __forceinline__ void h16_convert_warps(H16Smem& s, const DecodeParams
   }
 }
 
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ void h16_convert_role(H16Smem& s, const DecodeParams& P, int n_segs, uint32_t& it, int cg) {
-  if (int(((threadIdx.x >> 5) - 8) >> 2 & 1) != cg) h16_convert_warps<true, WINDOW>(s, P, n_segs, it);
-  else h16_convert_warps<false, WINDOW>(s, P, n_segs, it);
+  if (int(((threadIdx.x >> 5) - 8) >> 2 & 1) != cg) h16_convert_warps<true, MAP>(s, P, n_segs, it);
+  else h16_convert_warps<false, MAP>(s, P, n_segs, it);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -359,7 +360,7 @@ __device__ __forceinline__ void h16_pv_role(H16Smem& s, const DecodeParams& P, i
 // same in both, so the pair votes at a named barrier once per tile and, only when some row outgrows its max by 2^8,
 // exchanges the maxima through shared memory. A quadrant without live rows only keeps the barriers going.
 // ---------------------------------------------------------------------------------------------------------------
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams& P, int n_segs, uint32_t& it, int cg) {
   const int lane = ptx::lane_id(), warp = threadIdx.x >> 5;
   const int quad = warp & 3, half = warp >> 2;
@@ -390,7 +391,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
     // A row sees the tokens up to its own query token: token i of q_len (rows [i, i + 1) * heads / q_len of the request) stops
     // q_len - 1 - i tokens before the request's end.
     int row_end = seg.tok_end;
-    const int2 dead = WINDOW ? seg_window(P, seg.b).dead : make_int2(0, 0);
+    const int2 dead = MAP ? seg_window<MAP>(P, seg.b).dead : make_int2(0, 0);
     if (P.q_len > 1) {
       const int i = (r0 + hq) / (P.heads / P.q_len), end = P.kv_lens[seg.b] - (P.q_len - 1 - i);
       row_end = end < row_end ? end : row_end;
@@ -489,7 +490,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
 #pragma unroll
         for (int j = 0; j < 32; ++j) sr[j] = (ok && j < nvalid) ? sr[j] : 0xFF800000u;
       }
-      if constexpr (WINDOW) {  // the gap between the first tokens and the window
+      if constexpr (MAP != kMapNone) {  // the gap between the first tokens and the window
         const int at = seg.tok0 + t * kH16Tile + 32 * half, d0 = dead.x - at, d1 = dead.y - at;
         if (d0 < 32 && d1 > 0) {
 #pragma unroll
@@ -585,7 +586,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
           *reinterpret_cast<float4*>(orow + 4 * i * CKV + c0) = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
       }
     }
-    if (cg == 0 && half == 0 && h < live_rows) P.lse_part[slot * P.heads_per_cta + h] = (WINDOW ? lt != 0.f : lt > 0.f) ? m + log2f(lt) : -INFINITY;
+    if (cg == 0 && half == 0 && h < live_rows) P.lse_part[slot * P.heads_per_cta + h] = (MAP ? lt != 0.f : lt > 0.f) ? m + log2f(lt) : -INFINITY;
     ptx::tc_fence_before_sync();
     ptx::bar_sync(pair_bar, 64);  // s.xl and s.xch are reused by the next segment
   }
@@ -596,7 +597,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
 // ---------------------------------------------------------------------------------------------------------------
 enum H16Role { kH16Softmax, kH16Convert, kH16Qk, kH16Prefetch, kH16Pv, kH16Idle };
 
-template <int ROLE, bool WINDOW>
+template <int ROLE, int MAP>
 __device__ __forceinline__ void h16_run_role(H16Smem& s, const DecodeParams& P) {
   const int pair = blockIdx.x >> 1, cg = blockIdx.x & 1;
   const int2 range = P.cta_range[pair];
@@ -609,17 +610,17 @@ __device__ __forceinline__ void h16_run_role(H16Smem& s, const DecodeParams& P) 
       s.segs[threadIdx.x] = g;
     }
     __syncthreads();
-    if (ROLE == kH16Softmax) h16_softmax_role<WINDOW>(s, P, n_segs, it, cg);
-    if (ROLE == kH16Convert) h16_convert_role<WINDOW>(s, P, n_segs, it, cg);
+    if (ROLE == kH16Softmax) h16_softmax_role<MAP>(s, P, n_segs, it, cg);
+    if (ROLE == kH16Convert) h16_convert_role<MAP>(s, P, n_segs, it, cg);
     if (ROLE == kH16Qk) h16_qk_role(s, P, n_segs, it, seg_count, cg);
-    if (ROLE == kH16Prefetch) h16_prefetch_role<WINDOW>(s, P, n_segs, it, cg);
+    if (ROLE == kH16Prefetch) h16_prefetch_role<MAP>(s, P, n_segs, it, cg);
     if (ROLE == kH16Pv) h16_pv_role(s, P, n_segs, it, cg);
     __syncthreads();
     if (s.abort_flag) break;
   }
 }
 
-template <bool WINDOW>
+template <int MAP>
 __global__ void __launch_bounds__(kH16Threads, 1) mla_decode_hm16_kernel(const DecodeParams P) {
   extern __shared__ uint8_t smem_raw[];
   H16Smem& s = *reinterpret_cast<H16Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -646,23 +647,23 @@ __global__ void __launch_bounds__(kH16Threads, 1) mla_decode_hm16_kernel(const D
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();  // after the wait: the combine kernel reads a schedule kernel's output as soon as it starts
   // the query panels are free until the softmax warps write them
-  if (P.inline_sched) publish_own_schedule<kH16Threads>(reinterpret_cast<int*>(s.q[0]), P, blockIdx.x >> 1);
+  if (P.inline_sched) publish_own_schedule<kH16Threads, MAP>(reinterpret_cast<int*>(s.q[0]), P, blockIdx.x >> 1);
 
   // register budgets, warp group by warp group; the pool is the launch allocation, 28 warps x 72
   constexpr int kLaunchRegs = 72, kSoftmaxRegs = 96, kConvertRegs = 64, kIssueRegs = 48;
   static_assert(8 * kSoftmaxRegs + 16 * kConvertRegs + 4 * kIssueRegs <= 28 * kLaunchRegs, "register budgets exceed the CTA's allocation");
   if (warp < 8) {
     ptx::reg_alloc<kSoftmaxRegs>();
-    h16_run_role<kH16Softmax, WINDOW>(s, P);
+    h16_run_role<kH16Softmax, MAP>(s, P);
   } else if (warp < 24) {
     ptx::reg_dealloc<kConvertRegs>();
-    h16_run_role<kH16Convert, WINDOW>(s, P);
+    h16_run_role<kH16Convert, MAP>(s, P);
   } else {
     ptx::reg_dealloc<kIssueRegs>();
-    if (warp == 24) h16_run_role<kH16Qk, WINDOW>(s, P);
-    else if (warp == 25) h16_run_role<kH16Prefetch, WINDOW>(s, P);
-    else if (warp == 26) h16_run_role<kH16Pv, WINDOW>(s, P);
-    else h16_run_role<kH16Idle, WINDOW>(s, P);
+    if (warp == 24) h16_run_role<kH16Qk, MAP>(s, P);
+    else if (warp == 25) h16_run_role<kH16Prefetch, MAP>(s, P);
+    else if (warp == 26) h16_run_role<kH16Pv, MAP>(s, P);
+    else h16_run_role<kH16Idle, MAP>(s, P);
   }
 
   ptx::tc_fence_before_sync();

@@ -100,7 +100,7 @@ constexpr size_t vt_smem_bytes() { return sizeof(VtSmem) + 1024; }
 // ---------------------------------------------------------------------------------------------------------------
 // role: TMA producer (one warp; lane 0 issues, all lanes help with the page ids of small pages)
 // ---------------------------------------------------------------------------------------------------------------
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ void vt_producer_role(VtSmem& s, const DecodeParams& P, const CUtensorMap* ckv_map, const CUtensorMap* sf_map,
                                                  const CUtensorMap* kpe_map, int n_segs, uint32_t& it) {
   const int lane = ptx::lane_id();
@@ -110,8 +110,9 @@ __device__ __forceinline__ void vt_producer_role(VtSmem& s, const DecodeParams& 
     if (seg.ntiles <= 0) continue;
     const int* pt = P.page_table + (long long)seg.b * P.pt_stride;
     WindowMap win = {};
-    if constexpr (WINDOW) win = seg_window(P, seg.b);
-    auto page_id = [&](int i) { return pt[WINDOW ? win.page(i) : i]; };
+    if constexpr (MAP != kMapNone) win = seg_window<MAP>(P, seg.b);
+    if constexpr (MAP == kMapChunk) pt = P.page_table + (long long)win.request * P.pt_stride;
+    auto page_id = [&](int i) { return pt[MAP ? win.page(i) : i]; };
     // page ids of a tile's two half tiles and of the two that are prefetched into L2 (three tiles ahead: the ring itself
     // is too shallow to cover HBM latency); read one tile ahead of their use so that nothing ever waits for them
     auto fetch_ids = [&](int tk0, int (&pg)[2], int (&pf)[2]) {
@@ -343,15 +344,15 @@ __device__ __forceinline__ bool vt_load_query(VtSmem& s, const DecodeParams& P, 
   return true;
 }
 
-// Whether token `tok` of the segment's request is seen: before its end and, with WINDOW, outside the gap between the first tokens
+// Whether token `tok` of the segment's request is seen: before its end and, with a MAP, outside the gap between the first tokens
 // and the window.
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ bool vt_sees(const Seg& seg, int2 dead, int tok) {
-  return tok < seg.tok_end && (!WINDOW || tok < dead.x || tok >= dead.y);
+  return tok < seg.tok_end && (!MAP || tok < dead.x || tok >= dead.y);
 }
 
 // One tile of a K thread. Returns false if a wait gave up.
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ bool vt_k_step(VtSmem& s, const DecodeParams& P, const Seg& seg, int2 dead, int t, uint32_t it, int lane, int quad) {
   const int r = quad * 32 + lane;
   const uint32_t tm_lane = s.tmem_base + (uint32_t(quad * 32) << 16);
@@ -359,7 +360,7 @@ __device__ __forceinline__ bool vt_k_step(VtSmem& s, const DecodeParams& P, cons
   const uint32_t raw = ptx::smem_u32(s.raw[slot]);
   const uint32_t buf = it & 1;
   if (!__all_sync(~0u, ptx::mbar_wait(&s.raw_full[slot], (it / kVtRawSlots) & 1, &s.abort_flag))) return false;
-  const bool valid = vt_sees<WINDOW>(seg, dead, seg.tok0 + t * TILE + r);
+  const bool valid = vt_sees<MAP>(seg, dead, seg.tok0 + t * TILE + r);
   // tests of the barriers needed further down, issued before the work that precedes them
   const uint32_t pr_kfree = ptx::mbar_probe(&s.k_free[buf], ((it >> 1) & 1) ^ 1), pr_rope = ptx::mbar_probe(&s.rope_free, (it & 1) ^ 1);
 
@@ -431,7 +432,7 @@ __device__ __forceinline__ bool vt_k_step(VtSmem& s, const DecodeParams& P, cons
 // A warp whose wait gave up does not leave at once: the 128 K threads meet at a named barrier at the start of every
 // segment, so it carries on (skipping the work) to the next such barrier, where the failure is OR-reduced and all
 // four warps leave together.
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ void vt_k_role(VtSmem& s, const DecodeParams& P, int n_segs, uint32_t& it, uint32_t& seg_count) {
   const int lane = ptx::lane_id();
   const int quad = (threadIdx.x >> 5) & 3;
@@ -444,9 +445,9 @@ __device__ __forceinline__ void vt_k_role(VtSmem& s, const DecodeParams& P, int 
     if (!vt_load_query(s, P, seg, quad * 32 + lane, seg_count & 3, lane, quad, dead, it != 0, &s.k_free[(it - 1) & 1], ((it - 1) >> 1) & 1))
       return;
     ++seg_count;
-    const int2 gap = WINDOW ? seg_window(P, seg.b).dead : make_int2(0, 0);
+    const int2 gap = MAP ? seg_window<MAP>(P, seg.b).dead : make_int2(0, 0);
     for (int t = 0; t < seg.ntiles; ++t, ++it) {
-      if (!vt_k_step<WINDOW>(s, P, seg, gap, t, it, lane, quad)) {
+      if (!vt_k_step<MAP>(s, P, seg, gap, t, it, lane, quad)) {
         dead = true;
         break;
       }
@@ -642,7 +643,7 @@ __device__ __forceinline__ void vt_pv_role(VtSmem& s, const DecodeParams& P, int
 // ---------------------------------------------------------------------------------------------------------------
 // role: softmax + epilogue (4 warps; thread r = token row of S^T and channel-pair row of O^T)
 // ---------------------------------------------------------------------------------------------------------------
-template <bool WINDOW>
+template <int MAP>
 __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P, int n_segs, uint32_t& it, uint32_t& seg_count) {
   constexpr int N = 16;
   const int lane = ptx::lane_id(), warp = threadIdx.x >> 5;
@@ -658,7 +659,7 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
     if (seg.ntiles <= 0) continue;
     const int par_q = seg_count & 3;
     ++seg_count;
-    const int2 dead = WINDOW ? seg_window(P, seg.b).dead : make_int2(0, 0);
+    const int2 dead = MAP ? seg_window<MAP>(P, seg.b).dead : make_int2(0, 0);
     // running maximum and sum per head. The maximum starts at a finite sentinel far below any score rather than at
     // -inf: x - m and m - m' then never meet inf - inf, and no special case is needed anywhere below.
     constexpr float kNoMax = -1e30f;
@@ -681,7 +682,7 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
         }
       }
       if (ok) {
-        const bool valid = vt_sees<WINDOW>(seg, dead, seg.tok0 + t * TILE + r);
+        const bool valid = vt_sees<MAP>(seg, dead, seg.tok0 + t * TILE + r);
         uint32_t sv[32];  // columns [0, 16): even terms + rope, [16, 32): odd terms
         ptx::tmem_ld32(tm_lane + VtCols::s(buf), sv);
         ptx::tmem_wait_ld();
@@ -801,8 +802,8 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
 #pragma unroll
       for (int h = 0; h < N; ++h)
         if (h == r) l = lsum[h], mm = m[h];
-      // (with WINDOW a sum of NaN is carried on: a row that sees a NaN block scale is NaN)
-      P.lse_part[slot * N + r] = (WINDOW ? l != 0.f : l > 0.f) ? mm + log2f(l) : -INFINITY;
+      // (with a MAP a sum of NaN is carried on: a row that sees a NaN block scale is NaN)
+      P.lse_part[slot * N + r] = (MAP ? l != 0.f : l > 0.f) ? mm + log2f(l) : -INFINITY;
     }
     ptx::tc_fence_before_sync();
     ptx::bar_sync(1, 128);  // s.red is reused by the next segment
@@ -815,7 +816,7 @@ __device__ __forceinline__ void vt_softmax_role(VtSmem& s, const DecodeParams& P
 // ---------------------------------------------------------------------------------------------------------------
 enum VtRole { kVtSoftmax, kVtK, kVtV, kVtQk, kVtProducer, kVtPv, kVtIdle };
 
-template <int ROLE, bool WINDOW>
+template <int ROLE, int MAP>
 __device__ __forceinline__ void vt_run_role(VtSmem& s, const DecodeParams& P, const CUtensorMap* ckv_map, const CUtensorMap* sf_map,
                                             const CUtensorMap* kpe_map) {
   const int2 range = P.cta_range[blockIdx.x];
@@ -828,18 +829,18 @@ __device__ __forceinline__ void vt_run_role(VtSmem& s, const DecodeParams& P, co
       s.segs[threadIdx.x] = g;
     }
     __syncthreads();
-    if (ROLE == kVtSoftmax) vt_softmax_role<WINDOW>(s, P, n_segs, it, seg_count);
-    if (ROLE == kVtK) vt_k_role<WINDOW>(s, P, n_segs, it, seg_count);
+    if (ROLE == kVtSoftmax) vt_softmax_role<MAP>(s, P, n_segs, it, seg_count);
+    if (ROLE == kVtK) vt_k_role<MAP>(s, P, n_segs, it, seg_count);
     if (ROLE == kVtV) vt_v_role(s, P, n_segs, it, (uint32_t(threadIdx.x) >> 7) - 2);
     if (ROLE == kVtQk) vt_qk_role(s, P, n_segs, it);
-    if (ROLE == kVtProducer) vt_producer_role<WINDOW>(s, P, ckv_map, sf_map, kpe_map, n_segs, it);
+    if (ROLE == kVtProducer) vt_producer_role<MAP>(s, P, ckv_map, sf_map, kpe_map, n_segs, it);
     if (ROLE == kVtPv) vt_pv_role(s, P, n_segs, it);
     __syncthreads();
     if (s.abort_flag) break;
   }
 }
 
-template <bool WINDOW>
+template <int MAP>
 __global__ void __launch_bounds__(kVtThreads, 1)
 mla_decode_vt_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__ CUtensorMap sf_map,
                      const __grid_constant__ CUtensorMap kpe_map, const DecodeParams P) {
@@ -871,7 +872,7 @@ mla_decode_vt_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_c
   ptx::grid_dependency_wait();  // whatever precedes the call in the stream (the lengths' producer, the schedule kernel, the
                                 // previous call's use of the workspace) is settled
   ptx::grid_launch_dependents();
-  if (P.inline_sched) publish_own_schedule<kVtThreads>(reinterpret_cast<int*>(s.raw[0]), P, blockIdx.x);  // raw[0] is free until the first load
+  if (P.inline_sched) publish_own_schedule<kVtThreads, MAP>(reinterpret_cast<int*>(s.raw[0]), P, blockIdx.x);  // raw[0] is free until the first load
 
   // Register budgets per warp group (setmaxnreg); the pool is the launch allocation, 20 warps x 96, and the V warps keep
   // what they were launched with.
@@ -879,18 +880,18 @@ mla_decode_vt_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_c
   static_assert(4 * kSoftmaxRegs + 4 * kKRegs + 8 * kVRegs + 4 * kMiscRegs <= 20 * 96, "register budgets exceed the CTA's allocation");
   if (warp < 4) {
     ptx::reg_alloc<kSoftmaxRegs>();
-    vt_run_role<kVtSoftmax, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
+    vt_run_role<kVtSoftmax, MAP>(s, P, &ckv_map, &sf_map, &kpe_map);
   } else if (warp < 8) {
     ptx::reg_alloc<kKRegs>();
-    vt_run_role<kVtK, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
+    vt_run_role<kVtK, MAP>(s, P, &ckv_map, &sf_map, &kpe_map);
   } else if (warp < 16) {
-    vt_run_role<kVtV, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
+    vt_run_role<kVtV, MAP>(s, P, &ckv_map, &sf_map, &kpe_map);
   } else {
     ptx::reg_dealloc<kMiscRegs>();
-    if (warp == 16) vt_run_role<kVtQk, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
-    else if (warp == 17) vt_run_role<kVtProducer, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
-    else if (warp == 18) vt_run_role<kVtPv, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
-    else vt_run_role<kVtIdle, WINDOW>(s, P, &ckv_map, &sf_map, &kpe_map);
+    if (warp == 16) vt_run_role<kVtQk, MAP>(s, P, &ckv_map, &sf_map, &kpe_map);
+    else if (warp == 17) vt_run_role<kVtProducer, MAP>(s, P, &ckv_map, &sf_map, &kpe_map);
+    else if (warp == 18) vt_run_role<kVtPv, MAP>(s, P, &ckv_map, &sf_map, &kpe_map);
+    else vt_run_role<kVtIdle, MAP>(s, P, &ckv_map, &sf_map, &kpe_map);
   }
 
   ptx::tc_fence_before_sync();

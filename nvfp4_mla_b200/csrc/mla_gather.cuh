@@ -17,17 +17,6 @@ namespace mla {
 constexpr int kGatherThreads = 256;
 constexpr int kGatherRows = 4;  // rows of a warp (two trips); two where there are too few to give every SM its warps
 
-// the request whose rows [indptr[b], indptr[b + 1]) hold row i (indptr[0] <= i < indptr[batch]); empty requests hold none
-__device__ __forceinline__ int request_of_row(const int* __restrict__ indptr, int batch, int i) {
-  int lo = 0, hi = batch - 1;  // last b with indptr[b] <= i
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(indptr + mid) <= i) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
-
 // status: optional device word, set to 1 if a row's token lies outside the page table or on a page outside the cache (its output is 0)
 template <typename T>
 __global__ void __launch_bounds__(kGatherThreads)

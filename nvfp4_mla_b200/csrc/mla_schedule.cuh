@@ -249,7 +249,7 @@ mla_combine_sched_kernel(Problem pb, const int2* __restrict__ item_range, const 
       if (z < pb.splits) w = ((long long)b * pb.splits + z) * pb.head_groups + hg;
       if (kv_lens) {
         // the two loads are independent (a stale range is read and dropped): one memory latency, not two in a row
-        const int t = z < pb.splits ? sched_tiles(kv_lens, pb, b * pb.splits + z) : 0;
+        const int t = z < pb.splits ? sched_tiles(sched_len(kv_lens, pb, b), pb, b * pb.splits + z) : 0;
         ptx::grid_dependency_wait();  // item_range is the decode kernel's output here
         const int2 r = z < pb.splits ? item_range[w] : make_int2(0, -1);
         if (t > 0) c0 = r.x, c1 = r.y;
