@@ -562,9 +562,10 @@ int make_half_map(const void* base, int64_t rows, CUtensorMap* map) {
 // to 16000 tokens).
 //   by token: those of the decode kernels (wants_hm16), every query token a request
 //   shared  : 21 + 0.3 per thousand dequantised tokens + 4.2 per 256-token tile of the fullest pair + 0.2 per thousand rows
-// Measured (by token / shared), heads, requests, query tokens, tokens: 16,1,1,1000: 20 / 26; 16,64,1,4000: 61 / 180; 16,4,8,16000: 78 / 73;
-// 16,64,8,1000: 114 / 59; 32,16,4,4000: 84 / 59; 64,16,8,4000: 240 / 108; 128,16,1,4000: 61 / 59; 128,16,1,16000: 134 / 177;
-// 128,64,1,200: 47 / 30; 128,64,4,4000: 508 / 331.
+// Measured (by token / shared), heads, requests, query tokens, tokens: 16,1,1,1000: 18 / 22; 16,64,1,4000: 61 / 173; 16,4,8,16000: 78 / 57;
+// 16,64,8,1000: 127 / 64; 32,16,4,4000: 88 / 56; 64,16,8,4000: 251 / 103; 128,16,1,4000: 65 / 57; 128,16,1,16000: 135 / 170;
+// 128,64,1,200: 54 / 27; 128,64,4,4000: 545 / 327. Over the 158 sizes the form that is taken costs 0.9 % more than the better one; the
+// constants are those of calls among others on the host, where a launch is 2 us and the second form has two more.
 bool extend_shares(int batch, int total_q, int heads, int max_kv_len, int window, int sinks, const DeviceInfo& d) {
   if (d.ext_pairs < 2 || batch <= 0 || total_q <= 0) return false;
   if (heads % 16 != 0) return true;

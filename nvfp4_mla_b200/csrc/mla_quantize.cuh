@@ -69,15 +69,16 @@ struct QuantScales {
   }
 };
 
-// A factor f for the block scale `sf8` with which every BF16 value x has code(fl(x f)) = code(fl(x / sf)), or 0 if none is found.
+// A factor f for the block scale `sf8` with which every BF16 value x has code(fl(x f)) = code(fl(x / sf)); where there is none, the
+// reciprocal f and a second term g with which fl(x f + fl(x g)) has the code; {0, 0} if that is none either.
 // Both quotients round alike unless x / sf is within 2^-20 of a boundary; a boundary is m 2^k with m = 1, 1.25, 1.5 or 1.75, so only the
 // BF16 number x_m next to m sf can be that close (and its products with powers of two, which behave like it), and the scale alone
 // says whether it is: fl(m sf) is then within 16 units in its last place of a BF16 number. For these m (none for most scales, one or
 // two for amax / (6 * 448) of a BF16 amax, all four where the cache's scale is a power of two) f has to put x_m on the side of m,
 // or on m itself, that the division does; f is the reciprocal or one of the two numbers on either side of it, within 3 * 2^-23 of 1 / sf.
-__device__ __forceinline__ float quant_factor(uint32_t sf8, float ckv_scale) {
+__device__ __forceinline__ float2 quant_factor(uint32_t sf8, float ckv_scale) {
   const float sf = __fmul_rn(e4m3_value(uint8_t(sf8)), ckv_scale);
-  if (!(sf > 0x1p-100f && sf < 0x1p100f)) return 0.f;
+  if (!(sf > 0x1p-100f && sf < 0x1p100f)) return make_float2(0.f, 0.f);
   const uint32_t r = __float_as_uint(__frcp_rn(sf));
   float x[4];   // x_m, or m itself over ...
   float q[4];   // ... and its quotient
@@ -96,13 +97,30 @@ __device__ __forceinline__ float quant_factor(uint32_t sf8, float ckv_scale) {
       const float m = 1.f + 0.25f * i, p = __fmul_rn(x[i], f);
       good &= (p < m) == (q[i] < m) && (p > m) == (q[i] > m);
     }
-    if (good) return f;
+    if (good) return make_float2(f, 0.f);
   }
-  return 0.f;
+  const float f = __uint_as_float(r), g = __fmul_rn(__fmaf_rn(-sf, f, 1.f), f);
+  bool good = sf8 != 0x7Eu;  // (the largest scale's block may hold infinities)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float m = 1.f + 0.25f * i, p = __fmaf_rn(x[i], f, __fmul_rn(x[i], g));
+    good &= (p < m) == (q[i] < m) && (p > m) == (q[i] > m);
+  }
+  return good ? make_float2(f, g) : make_float2(0.f, 0.f);
 }
 constexpr int kQuantFactors = 128;
-__device__ __forceinline__ void quant_factors(float (&factors)[kQuantFactors], float ckv_scale) {  // (the caller synchronises)
-  if (threadIdx.x < kQuantFactors) factors[threadIdx.x] = quant_factor(threadIdx.x, ckv_scale);
+struct QuantFactors {
+  float f[kQuantFactors], g[kQuantFactors];
+};
+// by the block, synchronises; whether some block scale needs its second term (then all products take both, 0 for the others)
+__device__ __forceinline__ bool quant_factors(QuantFactors& s, float ckv_scale) {  // by the block; synchronises
+  const bool mine = threadIdx.x < kQuantFactors;
+  const float2 f = mine ? quant_factor(threadIdx.x, ckv_scale) : make_float2(0.f, 0.f);
+  const bool second = __syncthreads_or(f.y != 0.f);
+  // (0 * inf: where second terms are taken, a block that may hold infinities has no factor)
+  if (mine) s.f[threadIdx.x] = second && threadIdx.x == 0x7Eu ? 0.f : f.x, s.g[threadIdx.x] = f.y;
+  __syncthreads();
+  return second;
 }
 
 // Codes and scale byte of one block of 16 latent values; `value(j)` gives value j again. With FACTORS one product per value settles its code.
@@ -110,7 +128,7 @@ struct QuantBlock {
   uint32_t lo, hi, sf8;
 };
 template <bool FACTORS, class Value>
-__device__ __forceinline__ QuantBlock quantize_block(const float (&x)[16], const QuantScales& Q, const float* factors, Value value) {
+__device__ __forceinline__ QuantBlock quantize_block(const float (&x)[16], const QuantScales& Q, const QuantFactors* factors, bool second, Value value) {
   float amax = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) amax = ptx::max3(amax, fabsf(x[2 * j]), fabsf(x[2 * j + 1]));
@@ -118,13 +136,21 @@ __device__ __forceinline__ QuantBlock quantize_block(const float (&x)[16], const
   uint32_t sf8 = sf2 & 0xFFu;
   if (!Q.fast_sf || sf8 != sf2 >> 8) sf8 = f32x2_to_e4m3x2_sat(__fdiv_rn(__fdiv_rn(amax, 6.0f), Q.ckv_scale), 0.f) & 0xFFu;
   if constexpr (FACTORS) {
-    const float f = factors[sf8 & 127u];
+    const float f = factors->f[sf8 & 127u];
     if (f != 0.f) {
       float y[16];
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {
         const float2 p = ptx::mul_f32x2(make_float2(x[j], x[j + 1]), make_float2(f, f));
         y[j] = p.x, y[j + 1] = p.y;
+      }
+      if (second) {
+        const float g = factors->g[sf8 & 127u];
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          const float2 v = make_float2(x[j], x[j + 1]), p = ptx::fma_f32x2(v, make_float2(f, f), ptx::mul_f32x2(v, make_float2(g, g)));
+          y[j] = p.x, y[j + 1] = p.y;
+        }
       }
       return {e2m1x8(reinterpret_cast<const float(&)[8]>(y[0])), e2m1x8(reinterpret_cast<const float(&)[8]>(y[8])), sf8};
     }
@@ -211,7 +237,7 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
     // (a value that has to be settled is read again from memory: the registers cannot be indexed)
-    const QuantBlock q = quantize_block<false>(x, Q, nullptr, [&](int j) { return __bfloat162float(ckv[t * CKV + 16 * lane + j]); });
+    const QuantBlock q = quantize_block<false>(x, Q, nullptr, false, [&](int j) { return __bfloat162float(ckv[t * CKV + 16 * lane + j]); });
     *reinterpret_cast<uint2*>(ckv_cache + row * (CKV / 2) + 8 * lane) = make_uint2(q.lo, q.hi);
     sf_cache[row * (CKV / 16) + lane] = uint8_t(q.sf8);
     // ---- rope channels 2 lane, 2 lane + 1
@@ -239,9 +265,9 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 // One warp per token per trip, lane l = scale block l, as above; a lane's normalised BF16 values sit in shared memory for the few that
 // have to be settled, the weights and the factors of the 128 block scales there too. A lane looks up the place of one of the warp's next
 // 32 tokens, so that the walk through the page tables is paid for once in 32 trips. 1512 bytes per token, bound by instruction issue and
-// the latency of a warp's chain of steps (348 warp instructions per token, 67 % of the issue slots): 274880 tokens in 129 us with
-// ckv_scale = 6.5 / (6 * 448) (63 at the measured copy bandwidth), 172 with a power of two, where a third of the block scales has no
-// factor. Before: 166 and 188 with the enclosing products of the writer above and a walk per token; 345 with the norm in 64 bits
+// the latency of a warp's chain of steps (348 warp instructions per token, 67 % of the issue slots): 274880 tokens in 128 us with
+// ckv_scale = 6.5 / (6 * 448) (63 at the measured copy bandwidth), 137 with a power of two, where a third of the block scales needs a
+// second term (172 with the enclosing products for these). Before: 166 and 188 with the enclosing products of the writer above and a walk per token; 345 with the norm in 64 bits
 // throughout. Rows fetched ahead into shared memory (134), 40 warps per SM (171) and two CTAs per resident one (129.5) gained nothing.
 // ---------------------------------------------------------------------------------------------------------------
 template <bool INTERLEAVED>
@@ -255,7 +281,7 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
                             float kpe_scale, int* status) {
   __shared__ uint4 held[2][kQuantThreads];  // a lane's 16 normalised values
   __shared__ float4 gains[4][32];           // the weights: lane l's 16
-  __shared__ float factors[kQuantFactors];
+  __shared__ QuantFactors factors;
   const int lane = threadIdx.x & 31;
   const QuantScales Q(ckv_scale, kpe_scale);
   const float eps_f = float(eps);
@@ -267,7 +293,7 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
     reinterpret_cast<float*>(&gains[(i & 15) >> 2][i >> 4])[i & 3] = g;
     ordinary_gains &= g == 0.f || (fabsf(g) > 0x1p-20f && fabsf(g) < 0x1p20f);
   }
-  quant_factors(factors, ckv_scale);
+  const bool second = quant_factors(factors, ckv_scale);
   ordinary_gains = __syncthreads_and(ordinary_gains);
   const long long warp0 = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   const long long stride = (long long)gridDim.x * (kQuantThreads / 32);
@@ -341,7 +367,7 @@ mla_norm_rope_append_kernel(const __nv_bfloat16* __restrict__ ckv, long long ckv
     float x[16];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[2 * j] = two(held_[j]).x, x[2 * j + 1] = two(held_[j]).y;
-    const QuantBlock q = quantize_block<true>(x, Q, factors, [&](int j) {
+    const QuantBlock q = quantize_block<true>(x, Q, &factors, second, [&](int j) {
       const uint32_t v = reinterpret_cast<const uint32_t*>(&held[j >> 3][threadIdx.x])[j >> 1 & 3];
       return __uint_as_float(j & 1 ? v & 0xFFFF0000u : v << 16);
     });
