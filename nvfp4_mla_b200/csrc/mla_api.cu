@@ -614,9 +614,8 @@ int extend_shared(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache
     E.edges = (b == 0 ? 1 : 0) | (b + l.group >= batch ? 2 : 0);
     O.page_table = page_table + b * page_table_stride;
     P.E = E;
-    mla::mla_extend_schedule_kernel<<<1, mla::kExtSchedThreads, 0, st>>>(E);
+    mla::mla_extend_prep_kernel<<<unsigned(units < resident ? units : resident) + 1, mla::kExtPrepThreads, 0, st>>>(E, O);
     MLA_CUDA(cudaGetLastError());
-    MLA_CUDA(launch_dependent(mla::mla_extend_prep_kernel, dim3(unsigned(units < resident ? units : resident)), dim3(mla::kExtPrepThreads), 0, st, E, O));
     MLA_CUDA(launch_dependent_cluster(mla::mla_extend_kernel, dim3(unsigned(2 * l.pairs)), dim3(mla::kExtThreads), mla::ext_smem_bytes(), st, 2u,
                                       kv_map, q_map, P));
     MLA_CUDA(launch_dependent(mla::mla_extend_combine_kernel, dim3(unsigned(l.pairs), mla::kExtRows / 4), dim3(128), 0, st, E,

@@ -33,10 +33,10 @@ constexpr int kExtBlock = 64;   // tokens of a block
 constexpr int kExtTile = 256;   // tokens of a tile
 constexpr int kExtRow = CKV + KPE;
 constexpr int kExtMaxBatch = 2048;  // requests at a time
-constexpr int kExtHeld = 3584;      // items whose tile counts the schedule kernel keeps in shared memory
+constexpr int kExtHeld = 1024;      // items whose tile counts the schedule keeps in shared memory
 constexpr int kExtMaxPairs = 128;
 
-struct alignas(16) ExtItem {  // (read and written in 16-byte words: as ints, 787 items took the schedule kernel 12000 of its 26000 cycles)
+struct alignas(16) ExtItem {  // (read and written in 16-byte words: as ints, 787 items took the schedule 12000 of its 26000 cycles)
   int prefix;      // tiles of the items before
   int ntiles;      // at least 1 (an item that sees nothing has one tile, all masked)
   int block0;      // first workspace block of the request
@@ -69,7 +69,7 @@ struct ExtProblem {
   int* status;
 };
 
-constexpr int kExtSchedThreads = 1024;
+constexpr int kExtPrepThreads = 256;
 // Costs in quarters of a tile. Measured, cycles: a tile 5900 to 6200, an item 10000 to 12500 beside its tiles.
 constexpr int kTileCost = 4, kItemCost = 7;
 
@@ -128,15 +128,16 @@ __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
   return r;
 }
 
-// Where the requests' items and workspace blocks begin. The schedule and every block of the operands' kernel work this out for
-// themselves, so that neither waits for the other (32 windowed single tokens of 128 heads: 66.7 us one after the other, 61.6 so).
+// Where the requests' items and workspace blocks begin. Every CTA of the call's first kernel works this out for itself: the first one
+// makes the schedule, the others convert operands meanwhile (32 windowed single tokens of 128 heads: 66.7 us one after the other, 61.3 so; 24 to
+// 33 us of small calls 1 to 2 less than with a launch of its own for the schedule).
 struct ExtTables {
   int item0[kExtMaxBatch], block0[kExtMaxBatch];  // items and blocks of the requests before
   long long sums[32];
   int items, blocks;
 };
-template <int THREADS>
 __device__ __forceinline__ void ext_tables(const ExtProblem& E, ExtTables& s) {
+  constexpr int THREADS = kExtPrepThreads;
   const int tid = threadIdx.x;
   int items = 0, blocks = 0;
   for (int b0 = 0; b0 < E.batch; b0 += THREADS) {
@@ -162,21 +163,19 @@ __device__ __forceinline__ void ext_tables(const ExtProblem& E, ExtTables& s) {
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kernel(const ExtProblem E) {
-  __shared__ ExtTables tab;
-  __shared__ int2 held[kExtHeld];        // {prefix, tiles} of an item; static shared memory is 48 KB, the tables take 16
+__device__ __forceinline__ void ext_schedule(const ExtProblem& E, ExtTables& tab) {
+  __shared__ int2 held[kExtHeld];        // {prefix, tiles} of an item
   __shared__ int cut[kExtMaxPairs + 1];  // tiles of the rest before pair p
   __shared__ int rounds_s;
-  ptx::grid_launch_dependents();
   const int tid = threadIdx.x;
-  constexpr int kWarps = kExtSchedThreads / 32;
-  ext_tables<kExtSchedThreads>(E, tab);
+  constexpr int kWarps = kExtPrepThreads / 32;
+  static_assert(kExtMaxPairs <= kExtPrepThreads, "a thread per pair");
   const int items = tab.items;
   if (tid == 0) rounds_s = items / E.pairs;
 
   // ---- items
   int total = 0;
-  for (int i0 = 0; i0 < items; i0 += kExtSchedThreads) {
+  for (int i0 = 0; i0 < items; i0 += kExtPrepThreads) {
     const int i = i0 + tid;
     ExtItem m = {};
     if (i < items) {
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(kExtSchedThreads, 1) mla_extend_schedule_kerne
     E.pair[tid] = o;
   }
   __syncthreads();
-  for (int i = rest0 + tid; i < items; i += kExtSchedThreads) {
+  for (int i = rest0 + tid; i < items; i += kExtPrepThreads) {
     const int2 it = tiles_of(i);
     const int a = it.x - base, z = a + it.y;
     auto holder = [&](int x) {  // last pair whose piece starts at or before tile x (pieces without tiles lie in front of it)
@@ -314,7 +313,6 @@ struct ExtOperands {
   uint4* out;       // [total_q * heads][512] BF16
 };
 
-constexpr int kExtPrepThreads = 256;
 constexpr int kExtQRows = 32;   // rows of a unit
 
 // last b in [0, n) with a[b] <= x (a is non-decreasing, a[0] <= x), by the whole warp: 32 probes at a time
@@ -428,25 +426,29 @@ __device__ __forceinline__ void ext_convert_rows(const ExtProblem& E, const ExtO
   }
 }
 
-// Starts while the schedule is made and ends after it: the attention kernel, which waits for this grid, has waited for both.
+// The first CTA makes the schedule, the others the operands.
 __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const ExtProblem E, const ExtOperands O) {
   __shared__ ExtTables tab;
   ptx::grid_launch_dependents();
-  ext_tables<kExtPrepThreads>(E, tab);
+  ext_tables(E, tab);
+  if (blockIdx.x == 0) {
+    ext_schedule(E, tab);
+    return;
+  }
+  const int cta = int(blockIdx.x) - 1, ctas = int(gridDim.x) - 1;
   const int a = ext_first(E, 0), first = a < 0 ? 0 : a < E.total_q ? a : E.total_q;
   const int z = ext_first(E, E.batch), last = z < first ? first : z < E.total_q ? z : E.total_q;
   const long long front = E.edges & 1 ? (long long)first * E.heads : 0, none = front + (E.edges & 2 ? (long long)(E.total_q - last) * E.heads : 0);
-  for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < none; i += (long long)gridDim.x * 4) {
+  for (long long i = (long long)cta * 4 + (threadIdx.x >> 6); i < none; i += (long long)ctas * 4) {
     const long long row = i < front ? i : i - front + (long long)last * E.heads;
     O.out[row * (CKV / 8) + (threadIdx.x & 63)] = make_uint4(0, 0, 0, 0);
   }
   // (the last tile reads up to three blocks behind the last one, with weight 0: zeros)
   const int tokens = tab.blocks + 3 < E.max_blocks ? tab.blocks + 3 : E.max_blocks, units = tokens + tab.items * (kExtRows / kExtQRows);
-  for (int i = blockIdx.x; i < units; i += gridDim.x) {
+  for (int i = cta; i < units; i += ctas) {
     if (i < tokens) ext_convert_tokens(E, O, tab, i);
     else ext_convert_rows(E, O, tab, i - tokens);
   }
-  ptx::grid_dependency_wait();
 }
 
 // ---------------------------------------------------------------------------------------------------------------
