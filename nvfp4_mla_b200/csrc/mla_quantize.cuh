@@ -70,7 +70,8 @@ struct QuantScales {
 };
 
 // A factor f for the block scale `sf8` with which every BF16 value x has code(fl(x f)) = code(fl(x / sf)); where there is none, the
-// reciprocal f and a second term g with which fl(x f + fl(x g)) has the code; {0, 0} if that is none either.
+// reciprocal f, rounded down, and a second term g >= 0 with which fl(x f + fl(x g)) has the code; {0, 0} if that is none either. (With g < 0
+// the two products of x = -0 would have opposite signs and their sum would be +0, another code than -0 / sf.)
 // Both quotients round alike unless x / sf is within 2^-20 of a boundary; a boundary is m 2^k with m = 1, 1.25, 1.5 or 1.75, so only the
 // BF16 number x_m next to m sf can be that close (and its products with powers of two, which behave like it), and the scale alone
 // says whether it is: fl(m sf) is then within 16 units in its last place of a BF16 number. For these m (none for most scales, one or
@@ -99,7 +100,7 @@ __device__ __forceinline__ float2 quant_factor(uint32_t sf8, float ckv_scale) {
     }
     if (good) return make_float2(f, 0.f);
   }
-  const float f = __uint_as_float(r), g = __fmul_rn(__fmaf_rn(-sf, f, 1.f), f);
+  const float f = __uint_as_float(__fmaf_rn(-sf, __uint_as_float(r), 1.f) < 0.f ? r - 1 : r), g = __fmul_rn(__fmaf_rn(-sf, f, 1.f), f);
   bool good = sf8 != 0x7Eu;  // (the largest scale's block may hold infinities)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
