@@ -108,7 +108,8 @@ NVFP4_MLA_API int nvfp4_mla_decode_multi(const void* q_nope, const void* q_pe, c
  *                     workspace's first word receives them
  *   workspace         at least nvfp4_mla_decode_window_workspace_bytes() bytes, 256-byte aligned; nothing in it is kept between calls
  *
- * What is read and multiplied is the visible tokens, in whole pages. With many heads the call takes the form of nvfp4_mla_extend where
+ * A query row (request, head) with an element that is not finite gives NaN where it sees a token (nvfp4_mla_decode takes such elements as
+ * 0). What is read and multiplied is the visible tokens, in whole pages. With many heads the call takes the form of nvfp4_mla_extend where
  * that is estimated to be faster and only `out` is asked for. (No counterpart in the reference.) */
 NVFP4_MLA_API int64_t nvfp4_mla_decode_window_workspace_bytes(int batch, int heads, int page_size, int page_table_width, int max_kv_len,
                                                               int window, int sink_tokens);
@@ -127,7 +128,7 @@ NVFP4_MLA_API int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, 
  *                 tokens of no request (before qo_indptr[0], at or behind qo_indptr[batch]) and tokens in front of a request's first
  *                 (more new tokens than kv_lens) give zeros
  *   window        0: none
- *   others        as in nvfp4_mla_decode_window; 16-bit arithmetic; any number of heads
+ *   others        as in nvfp4_mla_decode_window, query rows that are not finite among them; 16-bit arithmetic; any number of heads
  *
  * Where it is estimated to be faster (nvfp4_mla_extend_shares: 1, 0: not, -1: error; in the main chunks of more than a few tokens),
  * all rows of a request share one pass over its cache, which is dequantised once into the workspace: 1152 bytes per visible token,

@@ -232,8 +232,8 @@ def decode_window(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, 
     Arguments as for ``decode``, 16-bit arithmetic. Pages without a visible token are not looked up, so that they can go back to the
     pool and their page-table entries may hold anything; the rows of ``page_table`` may be a slice of a wider one. What the call
     reads grows with ``window + sink_tokens``, not with the length. ``max_kv_len`` bounds ``kv_lens`` as in ``decode``; without it the
-    page table's width does, and nothing synchronises either way. Returns ``[batch, heads, 512]`` bfloat16; ``workspace_status``
-    reports bad pages."""
+    page table's width does, and nothing synchronises either way. Returns ``[batch, heads, 512]`` bfloat16; a query row that is not finite
+    gives NaN (``decode`` takes such elements as 0). ``workspace_status`` reports bad pages."""
     window, sink_tokens = _check_window(window, sink_tokens)
     _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)
     N, H, B, ps, width = _check_queries(q_nope, q_pe, ckv_cache, page_table, kv_lens, ckv_scale, kpe_scale)
@@ -283,8 +283,8 @@ def extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens
             ``sink_tokens``; pages that no query of the call sees are not looked up.
 
     The caches, scales and ``sm_scale`` are those of ``decode``; 16-bit arithmetic. Returns ``[total_q, heads, 512]`` bfloat16. Query tokens of
-    no request (at or behind ``qo_indptr[-1]``: a padded batch) and tokens that see nothing give zeros. ``workspace_status`` reports
-    bad pages.
+    no request (at or behind ``qo_indptr[-1]``: a padded batch) and tokens that see nothing give zeros, any other query row that is not
+    finite gives NaN. ``workspace_status`` reports bad pages.
     """
     window, sink_tokens = _check_window(window, sink_tokens) if window else (0, _check_window(1, sink_tokens)[1])
     _check_cache(ckv_cache, ckv_sf_cache, kpe_cache)

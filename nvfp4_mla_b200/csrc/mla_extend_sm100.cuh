@@ -233,10 +233,10 @@ __device__ __forceinline__ void ext_softmax_role(ExtSmem& s, const ExtParams& P,
   uint32_t g = 0;
   while (walk.next(m, t0, t1)) {
     const int r = 64 * int(rank) + h;  // row of the item
-    const float qa = P.q_scale[(long long)walk.item * kExtRows + r];
     // the row sees tokens [begin, end) and [0, sinks)
     const int pos = m.pos0 + (m.r0 + (r < m.rows ? r : m.rows - 1)) / P.E.heads;
     const int end = pos + 1;
+    const float qa = end > 0 ? P.q_scale[(long long)walk.item * kExtRows + r] : 1.f;  // (a row that sees nothing is 0 even if its query is not finite)
     const int begin = P.E.window > 0 && end > P.E.window ? end - P.E.window : 0, sinks = P.E.window > 0 ? P.E.sinks : 0;
     float mx_run = -INFINITY, l = 0.f;  // the maximum is the same in the row's four threads; l is this thread's share of the sum
     for (int t = t0; t < t1; ++t, ++g) {
