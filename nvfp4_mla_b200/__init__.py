@@ -394,7 +394,7 @@ def combine_records_signalled(record_ptrs, flag_ptrs, rank, epoch, rows, device,
 
 def combine(o_part, lse_part, out_dtype=torch.bfloat16, return_lse=False):
     """Log-sum-exp merge of partial results: ``o_part [parts, ..., 512]`` float32 (each normalised by its own softmax
-    sum) and ``lse_part [parts, ...]`` float32 in log2 units. Returns ``[..., 512]`` in ``out_dtype`` (bfloat16 or
+    sum) and ``lse_part [parts, ...]`` float32 in log2 units (-inf: an empty part; NaN: the row and its lse are NaN). Returns ``[..., 512]`` in ``out_dtype`` (bfloat16 or
     float32), and the merged lse with ``return_lse``."""
     if o_part.dtype != torch.float32 or lse_part.dtype != torch.float32:
         raise RuntimeError("o_part and lse_part must be float32")

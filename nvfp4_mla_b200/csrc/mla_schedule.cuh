@@ -219,7 +219,7 @@ __device__ __forceinline__ void merge_row(int n_parts, LseOf lse_of, OOf o_of, l
   if (out_bf16)
     reinterpret_cast<uint2*>(out_bf16)[row * (CKV / 4) + t] = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
   if (out_f32) reinterpret_cast<float4*>(out_f32)[row * (CKV / 4) + t] = acc;
-  if (lse_out && t == 0) lse_out[row] = den > 0.f ? M + log2f(den) : -INFINITY;
+  if (lse_out && t == 0) lse_out[row] = den == 0.f ? -INFINITY : M + log2f(den);  // (NaN stays NaN: no later merge takes the row for an empty one)
 }
 
 // Partials addressed through the schedule (what the decode kernel wrote).
