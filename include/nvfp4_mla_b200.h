@@ -184,7 +184,7 @@ NVFP4_MLA_API int nvfp4_mla_decode_static_status(void* stream);
 
 /* Synchronises `stream` and returns the status word of a decode workspace: 0 = every kernel ran to completion,
  * 1 = a bounded wait inside the decode kernel gave up (results invalid), 2 = batch * num_splits too large for the
- * schedule kernel, 3 = a page id inside a request's live range lies outside [0, num_pages) (it was not dereferenced:
+ * schedule kernel, or a query index of nvfp4_mla_extend that asks for more rows or tokens than its sizes allow (zeros), 3 = a page id inside a request's live range lies outside [0, num_pages) (it was not dereferenced:
  * pages of 64 tokens or more read as zeros, smaller pages keep whatever the staging buffer held; results invalid);
  * negative = CUDA error (see nvfp4_mla_last_error). No counterpart in the reference, whose kernels
  * have no bounded waits. */

@@ -604,7 +604,8 @@ def gather_paged_mla_kv_cache(ckv_cache, ckv_sf_cache, kpe_cache, page_table, in
 
 def workspace_status(device=None, clear=False):
     """Synchronises and returns the worst device-side status of the decode workspaces of ``device`` (0 = fine,
-    1 = a bounded wait inside the decode kernel gave up, 2 = schedule capacity exceeded, 3 = a page id inside a request's
+    1 = a bounded wait inside the decode kernel gave up, 2 = schedule capacity exceeded (or a ``qo_indptr`` that asks for more than there is room
+    for), 3 = a page id inside a request's
     live range lies outside the cache; the id was not dereferenced). The status word is sticky; ``clear=True`` zeroes
     it after reading. For tests and debugging."""
     lib = _lib.load()

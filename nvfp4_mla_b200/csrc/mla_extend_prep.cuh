@@ -105,6 +105,7 @@ struct ExtRequest {
 };
 // index of request b's first query token; without an indptr every request has one
 __device__ __forceinline__ int ext_first(const ExtProblem& E, int b) { return E.indptr ? E.indptr[b] : E.first_q + b; }
+__device__ __forceinline__ int ext_blocks(int tokens) { return tokens > 0 ? (tokens - 1) / kExtBlock + 1 : 0; }
 __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
   ExtRequest r;
   const int a = ext_first(E, b), z = ext_first(E, b + 1);
@@ -112,7 +113,7 @@ __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
   r.q0 = lo, r.q = hi > lo ? hi - lo : 0;
   const int n = E.kv_lens[b];
   r.n = n < 0 ? 0 : n < E.max_kv_len ? n : E.max_kv_len;
-  r.pos0 = r.n - (z - a) + (lo - a);
+  r.pos0 = r.q ? r.n - (z - lo) : 0;  // (z > lo >= 0)
   r.shift = 0, r.sink_blocks = 0, r.begin = 0;
   if (E.window > 0) {
     const long long s = ((long long)E.sinks + kExtBlock - 1) / kExtBlock;
@@ -120,9 +121,9 @@ __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
     r.begin = begin > 0 ? int(begin) : 0;
     const long long t = r.begin / kExtBlock;
     if (t > s) r.shift = int(t - s) * kExtBlock;
-    r.sink_blocks = int(s < (r.n + kExtBlock - 1) / kExtBlock ? s : (r.n + kExtBlock - 1) / kExtBlock);
+    r.sink_blocks = int(s < ext_blocks(r.n) ? s : ext_blocks(r.n));
   }
-  r.blocks = (r.n - r.shift + kExtBlock - 1) / kExtBlock;
+  r.blocks = ext_blocks(r.n - r.shift);
   if (r.blocks < 1) r.blocks = 1;
   if (r.q == 0) r.blocks = 0;
   return r;
@@ -135,31 +136,32 @@ struct ExtTables {
   int item0[kExtMaxBatch], block0[kExtMaxBatch];  // items and blocks of the requests before
   long long sums[32];
   int items, blocks;
+  bool failed;  // there is no room for what the query index asks for: no items, and zeros in the output
 };
 __device__ __forceinline__ void ext_tables(const ExtProblem& E, ExtTables& s) {
   constexpr int THREADS = kExtPrepThreads;
   const int tid = threadIdx.x;
+  // A query index that runs backwards or past total_q could ask for more than there is room for. A request has less than 2^26 of
+  // either, so that a round's 256 requests may add up to 2^34: sums of 64 bits, and no further round after one without room.
   int items = 0, blocks = 0;
+  bool failed = false;
   for (int b0 = 0; b0 < E.batch; b0 += THREADS) {
     const int b = b0 + tid;
-    int mine = 0, all;
+    long long mine = 0, all_items, all_blocks;
     ExtRequest r = {};
     if (b < E.batch) {
       r = ext_request(E, b);
-      mine = int(((long long)r.q * E.heads + kExtRows - 1) / kExtRows);
+      mine = ((long long)r.q * E.heads + kExtRows - 1) / kExtRows;
     }
-    const int ii = items + block_scan<THREADS / 32>(mine, s.sums, all) - mine;
-    items += all;
-    const int ib = blocks + block_scan<THREADS / 32>(r.blocks, s.sums, all) - r.blocks;
-    blocks += all;
-    if (b < E.batch) s.item0[b] = ii, s.block0[b] = ib;
+    const long long ii = items + block_scan<THREADS / 32>(mine, s.sums, all_items) - mine;
+    const long long ib = blocks + block_scan<THREADS / 32>((long long)r.blocks, s.sums, all_blocks) - r.blocks;
+    failed = items + all_items > E.max_items || blocks + all_blocks > E.max_blocks;
+    if (failed) break;
+    items += int(all_items), blocks += int(all_blocks);
+    if (b < E.batch) s.item0[b] = int(ii), s.block0[b] = int(ib);
   }
-  // (a query index that runs backwards could ask for more than there is room for)
-  if (items > E.max_items || blocks > E.max_blocks) {
-    if (tid == 0 && E.status) atomicExch(E.status, int(kBadSchedule));
-    items = 0, blocks = 0;
-  }
-  if (tid == 0) s.items = items, s.blocks = blocks;
+  if (failed && tid == 0 && E.status) atomicExch(E.status, int(kBadSchedule));
+  if (tid == 0) s.items = failed ? 0 : items, s.blocks = failed ? 0 : blocks, s.failed = failed;
   __syncthreads();
 }
 
@@ -192,7 +194,7 @@ __device__ __forceinline__ void ext_schedule(const ExtProblem& E, ExtTables& tab
       m.row0 = r.q0 * E.heads + m.r0, m.pos0 = r.pos0, m.shift = r.shift, m.block0 = tab.block0[lo];
       const int first = r.pos0 + m.r0 / E.heads, last = r.pos0 + (m.r0 + m.rows - 1) / E.heads;  // positions of its query tokens
       const int end = last + 1 < r.n ? last + 1 : r.n;                                           // tokens before it are seen
-      int e = (end - r.shift + kExtBlock - 1) / kExtBlock;                                       // blocks up to there
+      int e = ext_blocks(end - r.shift);                                                         // blocks up to there
       if (E.window > 0) {
         const long long begin = (long long)first - E.window + 1 - r.shift;
         const int t = begin > 0 ? int(begin / kExtBlock) : 0;
@@ -438,11 +440,14 @@ __global__ void __launch_bounds__(kExtPrepThreads) mla_extend_prep_kernel(const 
   const int cta = int(blockIdx.x) - 1, ctas = int(gridDim.x) - 1;
   const int a = ext_first(E, 0), first = a < 0 ? 0 : a < E.total_q ? a : E.total_q;
   const int z = ext_first(E, E.batch), last = z < first ? first : z < E.total_q ? z : E.total_q;
-  const long long front = E.edges & 1 ? (long long)first * E.heads : 0, none = front + (E.edges & 2 ? (long long)(E.total_q - last) * E.heads : 0);
+  // query tokens [a0, a1) and [b0, b1) get zeros: those of no request, or all of the call's requests where they find no room
+  const int a0 = E.edges & 1 ? 0 : first, a1 = tab.failed ? last : first, b0 = last, b1 = E.edges & 2 ? E.total_q : last;
+  const long long front = (long long)(a1 - a0) * E.heads, none = front + (long long)(b1 - b0) * E.heads;
   for (long long i = (long long)cta * 4 + (threadIdx.x >> 6); i < none; i += (long long)ctas * 4) {
-    const long long row = i < front ? i : i - front + (long long)last * E.heads;
+    const long long row = i < front ? i + (long long)a0 * E.heads : i - front + (long long)b0 * E.heads;
     O.out[row * (CKV / 8) + (threadIdx.x & 63)] = make_uint4(0, 0, 0, 0);
   }
+  if (tab.failed) return;
   // (the last tile reads up to three blocks behind the last one, with weight 0: zeros)
   const int tokens = tab.blocks + 3 < E.max_blocks ? tab.blocks + 3 : E.max_blocks, units = tokens + tab.items * (kExtRows / kExtQRows);
   for (int i = cta; i < units; i += ctas) {
