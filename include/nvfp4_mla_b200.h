@@ -105,8 +105,8 @@ NVFP4_MLA_API int nvfp4_mla_decode_multi(const void* q_nope, const void* q_pe, c
  *   page_table_width  columns of page_table that hold page ids. Pages that hold no visible token are not looked up: their entries
  *                     may hold anything (a serving engine has returned them to its pool)
  *   status            optional device int: receives the codes of nvfp4_mla_workspace_status (the caller zeroes it); NULL: the
- *                     workspace's first word receives them
- *   workspace         at least nvfp4_mla_decode_window_workspace_bytes() bytes, 256-byte aligned; nothing in it is kept between calls
+ *                     workspace's first word receives them (the caller zeroes that)
+ *   workspace         at least nvfp4_mla_decode_window_workspace_bytes() bytes, 256-byte aligned; nothing else in it is kept between calls
  *
  * A query row (request, head) with an element that is not finite gives NaN where it sees a token (nvfp4_mla_decode takes such elements as
  * 0). What is read and multiplied is the visible tokens, in whole pages. With many heads the call takes the form of nvfp4_mla_extend where
@@ -189,6 +189,13 @@ NVFP4_MLA_API int nvfp4_mla_decode_static_status(void* stream);
  * negative = CUDA error (see nvfp4_mla_last_error). No counterpart in the reference, whose kernels
  * have no bounded waits. */
 NVFP4_MLA_API int nvfp4_mla_workspace_status(const void* workspace, void* stream);
+
+/* A status word of the library's own, for callers of nvfp4_mla_extend and nvfp4_mla_decode_window that have none to hand over: its address
+ * on the current device (no allocation; may be asked for during stream capture once the device's set-up has run). It is zero when the
+ * library is loaded and sticky. nvfp4_mla_status_word_read synchronises `stream`, returns it (same codes as
+ * nvfp4_mla_workspace_status, negative = CUDA error) and with clear != 0 zeroes it. (No counterpart in the reference.) */
+NVFP4_MLA_API int nvfp4_mla_status_word(int32_t** word);
+NVFP4_MLA_API int nvfp4_mla_status_word_read(int clear, void* stream);
 
 /* Measurement aid: between nvfp4_mla_profile_begin(capacity) and nvfp4_mla_profile_end, every nvfp4_mla_decode call
  * made by this thread (up to `capacity` of them) brackets its main decode kernel, and only that kernel, with a pair

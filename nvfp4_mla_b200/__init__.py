@@ -4,6 +4,7 @@ Drop-in for the reference project's ``nvfp4_mla`` package (nvfp4_mla/__init__.py
 ``dequantize`` signatures, defaults, exception types and messages. The work is done by hand-written CUDA kernels in
 ``libnvfp4_mla_b200.so`` behind a C ABI (``include/nvfp4_mla_b200.h``); torch only owns the memory and the stream.
 """
+import ctypes
 import functools
 import operator
 
@@ -163,17 +164,17 @@ def decode(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens
                    kpe_scale, max_kv_len, num_splits, _PRECISIONS[precision], True, False)[0]
 
 
-_statuses = {}  # device index -> int32 word that the kernels of the calls below report to, sticky
+_statuses = {}  # device index -> address of the word that the kernels of the calls below report to, sticky
 
 
 def _status(dev):
-    """The device's status word; None while a graph is captured before any call has made it."""
-    word = _statuses.get(dev.index)
-    if word is None and not torch.cuda.is_current_stream_capturing():
-        word = torch.zeros(1, dtype=torch.int32, device=dev)
-        torch.cuda.current_stream(dev).synchronize()  # (once per device: a call on another stream may report before the zero is written)
-        word = _statuses.setdefault(dev.index, word)
-    return word
+    """Address of the library's status word on the current device ``dev`` (nothing is allocated: a graph may be captured before any call)."""
+    at = _statuses.get(dev.index)
+    if at is None:
+        word = ctypes.c_void_p()
+        _lib.check(_lib.load().nvfp4_mla_status_word(ctypes.byref(word)))
+        at = _statuses[dev.index] = word.value
+    return at
 
 
 @functools.lru_cache(maxsize=4096)
@@ -251,7 +252,7 @@ def decode_window(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, 
         _lib.check(_lib.load().nvfp4_mla_decode_window(
             q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), ckv_cache.shape[0], ps,
             page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), B, H, float(sm_scale), float(ckv_scale), float(kpe_scale),
-            max_kv_len, window, sink_tokens, out.data_ptr(), None, None, ws.data_ptr(), ws.numel(), _ptr(_status(dev)),
+            max_kv_len, window, sink_tokens, out.data_ptr(), None, None, ws.data_ptr(), ws.numel(), _status(dev),
             _raw_stream(dev)))
         return out
 
@@ -304,7 +305,7 @@ def extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens
             q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), ckv_sf_cache.data_ptr(), kpe_cache.data_ptr(), ckv_cache.shape[0], ps,
             page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), qo_indptr.data_ptr(), B, N, H, float(sm_scale),
             float(ckv_scale), float(kpe_scale), max_kv_len, window, sink_tokens, out.data_ptr(), ws.data_ptr(), ws.numel(),
-            _ptr(_status(dev)), _raw_stream(dev)))
+            _status(dev), _raw_stream(dev)))
         return out
 
     return _on_device(dev, launch)
@@ -350,7 +351,6 @@ def combine_records(record_ptrs, rows, device, out_dtype=torch.bfloat16):
     part (at most 16): the partial results of the GPUs of a sequence-sharded decode, read where their owners wrote them
     (addresses of peers' symmetric-memory buffers included). The caller orders the call after the owners' writes.
     Returns ``[rows, 512]`` in ``out_dtype`` on ``device``."""
-    import ctypes
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
     dev = torch.device(device)
@@ -372,7 +372,6 @@ def combine_records_signalled(record_ptrs, flag_ptrs, rank, epoch, rows, device,
     word ``rank`` of every array, waits at most ``wait_us`` microseconds for the other GPUs' announcements and merges.
     ``status``: int32 CUDA tensor of one element that receives 4 when the wait ran out (the output is then not to be
     used). Returns ``[rows, 512]`` in ``out_dtype`` on ``device``."""
-    import ctypes
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
     if len(flag_ptrs) != len(record_ptrs):
@@ -622,13 +621,13 @@ def workspace_status(device=None, clear=False):
                 ws[:4].zero_()
                 torch.cuda.synchronize(idx)
             worst = max(worst, st)
-    for idx, word in _statuses.items():
+    for idx in list(_statuses):
         if device is not None and torch.device(device).index not in (None, idx):
             continue
         with torch.cuda.device(idx):
             torch.cuda.synchronize(idx)
-            worst = max(worst, int(word.item()))
-            if clear:
-                word.zero_()
-                torch.cuda.synchronize(idx)
+            st = lib.nvfp4_mla_status_word_read(int(clear), None)
+            if st < 0:
+                raise RuntimeError(lib.nvfp4_mla_last_error().decode())
+            worst = max(worst, st)
     return worst

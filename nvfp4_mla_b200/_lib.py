@@ -35,6 +35,8 @@ SIGNATURES = {
     "nvfp4_mla_decode_static_capacity": (_i64, []),
     "nvfp4_mla_decode_static_status": (_i32, [_vp]),
     "nvfp4_mla_workspace_status": (_i32, [_vp, _vp]),
+    "nvfp4_mla_status_word": (_i32, [_vp]),
+    "nvfp4_mla_status_word_read": (_i32, [_i32, _vp]),
     "nvfp4_mla_profile_begin": (_i32, [_i32]),
     "nvfp4_mla_profile_end": (_i32, [_vp, _i32]),
     "nvfp4_mla_dequantize": (_i32, [_vp, _vp, _vp, _i64, _f32, _f32, _i32, _vp, _vp, _vp]),

@@ -503,7 +503,7 @@ namespace {
 constexpr int kExtendSlice = 512;  // query tokens at a time in the first form (the partial results of a slice take 2 KB per head and token)
 
 struct ExtendLayout {
-  size_t items, pair, q_scale, lse_part, o_part, q16, kv16, total;
+  size_t status, items, pair, q_scale, lse_part, o_part, q16, kv16, total;
   int group;  // requests at a time
   int pairs, max_items, max_blocks;
 };
@@ -535,6 +535,7 @@ int extend_layout(int batch, int total_q, int heads, int max_kv_len, int window,
     off = mla::align_up(off + bytes, 256);
     return at;
   };
+  l->status = take(sizeof(int));  // (the workspace's first word, as in the decode calls' workspace)
   l->items = take(size_t(items) * sizeof(mla::ExtItem)), l->pair = take(size_t(l->pairs) * sizeof(mla::ExtPair));
   l->q_scale = take(size_t(items) * mla::kExtRows * 4);
   l->lse_part = take(size_t(l->pairs) * 2 * mla::kExtRows * 4), l->o_part = take(size_t(l->pairs) * 2 * mla::kExtRows * mla::CKV * 4);
@@ -589,6 +590,7 @@ int extend_shared(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache
                   const int32_t* kv_lens, const int32_t* qo_indptr, int batch, int total_q, int heads, float sm_scale, float ckv_scale,
                   float kpe_scale, int max_kv_len, int window, int sink_tokens, void* out, uint8_t* ws, const ExtendLayout& l, const DeviceInfo& d,
                   int32_t* status, cudaStream_t st) {
+  if (!status) status = reinterpret_cast<int32_t*>(ws + l.status);
   CUtensorMap kv_map, q_map;
   if (make_half_map(ws + l.kv16, int64_t(l.max_blocks) * mla::kExtBlock, &kv_map)) return 1;
   if (make_half_map(ws + l.q16, int64_t(l.max_items) * mla::kExtRows, &q_map)) return 1;
@@ -814,6 +816,46 @@ int nvfp4_mla_decode_static_status(void* stream) {
   const int status = nvfp4_mla_workspace_status(scratch, stream);
   if (status > 0) {  // reported once: start the next run of calls from a clean word
     cudaError_t e = cudaMemsetAsync(scratch, 0, sizeof(int), static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return -fail("clearing the status word failed: %s", cudaGetErrorString(e));
+  }
+  return status;
+}
+
+// ---- a status word for callers that have none of their own ---------------------------------------------------------
+static __device__ int g_status_word;
+
+namespace {
+int* g_status_word_ptr[kMaxDevices] = {};  // its device address, per device
+int status_word(int** out) {
+  int dev = 0;
+  MLA_CUDA(cudaGetDevice(&dev));
+  MLA_CHECK(dev >= 0 && dev < kMaxDevices, "device index %d out of range", dev);
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (!g_status_word_ptr[dev]) {
+    void* p = nullptr;
+    MLA_CUDA(cudaGetSymbolAddress(&p, g_status_word));
+    MLA_CHECK(p != nullptr, "cudaGetSymbolAddress returned a null address for the status word");
+    g_status_word_ptr[dev] = static_cast<int*>(p);
+  }
+  *out = g_status_word_ptr[dev];
+  return 0;
+}
+}  // namespace
+
+int nvfp4_mla_status_word(int32_t** word) {
+  g_error[0] = 0;
+  MLA_CHECK(word, "null pointer argument");
+  return status_word(word);
+}
+
+int nvfp4_mla_status_word_read(int clear, void* stream) {
+  g_error[0] = 0;
+  int* word = nullptr;
+  if (status_word(&word)) return -1;
+  const int status = nvfp4_mla_workspace_status(word, stream);
+  if (status > 0 && clear) {
+    cudaError_t e = cudaMemsetAsync(word, 0, sizeof(int), static_cast<cudaStream_t>(stream));
     if (e == cudaSuccess) e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return -fail("clearing the status word failed: %s", cudaGetErrorString(e));
   }
