@@ -1001,7 +1001,7 @@ int nvfp4_mla_gather(const uint8_t* ckv_cache, const uint8_t* ckv_sf_cache, cons
   MLA_CHECK(num_pages > 0 && num_pages * page_size < (int64_t(1) << 31), "num_pages * page_size must be in [1, 2^31)");
   MLA_CHECK(page_table_stride >= 0 && page_table_width >= 0, "page_table_stride and page_table_width must be non-negative");
   if (total == 0 || batch == 0) return 0;
-  MLA_CHECK(ckv_cache && ckv_sf_cache && kpe_cache && page_table && indptr && ckv_out && kpe_out, "null pointer argument");
+  MLA_CHECK(ckv_cache && ckv_sf_cache && kpe_cache && (page_table || page_table_width == 0) && indptr && ckv_out && kpe_out, "null pointer argument");
   MLA_CHECK(aligned(ckv_cache, 4) && aligned(kpe_cache, 2) && aligned(ckv_out, 16) && aligned(kpe_out, 8),
             "ckv_cache must be 4-byte and kpe_cache 2-byte aligned, ckv_out 16-byte and kpe_out 8-byte aligned");
   DeviceInfo* d;
