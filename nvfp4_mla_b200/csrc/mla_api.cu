@@ -121,6 +121,17 @@ auto hm16_kernel(int map) {
          : map == mla::kMapWindow ? mla::mla_decode_hm16_kernel<mla::kMapWindow>
                                   : mla::mla_decode_hm16_kernel<mla::kMapNone>;
 }
+auto schedule_kernel(int map) {
+  return map == mla::kMapChunk    ? mla::mla_schedule_kernel<mla::kMapChunk>
+         : map == mla::kMapWindow ? mla::mla_schedule_kernel<mla::kMapWindow>
+                                  : mla::mla_schedule_kernel<mla::kMapNone>;
+}
+template <int GROUPS>
+auto combine_kernel(int map) {
+  return map == mla::kMapChunk    ? mla::mla_combine_sched_kernel<GROUPS, mla::kMapChunk>
+         : map == mla::kMapWindow ? mla::mla_combine_sched_kernel<GROUPS, mla::kMapWindow>
+                                  : mla::mla_combine_sched_kernel<GROUPS, mla::kMapNone>;
+}
 unsigned decode_threads(int precision, int hpc) {
   if (precision == NVFP4_MLA_PRECISION_FP8) return hpc == 128 ? mla::kHmThreads : mla::kDecodeThreads;
   return hpc > 16 ? mla::kH16Threads : mla::kVtThreads;
@@ -271,7 +282,7 @@ int problem_of(int batch, int heads, int max_kv_len, int num_splits, int n_cta, 
   const long long chunk = ((len + splits - 1) / splits + mla::TILE - 1) / mla::TILE * mla::TILE;
   pb->batch = batch, pb->heads = heads, pb->heads_per_cta = hpc, pb->head_groups = (heads + hpc - 1) / hpc;
   pb->splits = splits, pb->chunk = int(chunk), pb->n_cta = n_cta;
-  pb->map = mla::kMapNone, pb->window = 0, pb->sinks = 0, pb->page_shift = 0, pb->pt_width = 0, pb->requests = 0, pb->q_first = 0, pb->q_indptr = nullptr;
+  pb->window = 0, pb->sinks = 0, pb->page_shift = 0, pb->pt_width = 0, pb->requests = 0, pb->q_first = 0, pb->q_indptr = nullptr;
   MLA_CHECK((long long)batch * splits <= mla::kSchedMaxBZ, "batch * num_splits = %lld exceeds %d", (long long)batch * splits,
             mla::kSchedMaxBZ);
   MLA_CHECK(splits + n_cta <= 512, "num_splits %d too large (at most %d)", splits, 512 - n_cta);
@@ -364,7 +375,7 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   if (problem_of(batch, heads, max_kv_len, num_splits, schedule_units(*d, precision, hpc), hpc, &pb)) return 1;
   if (batch == 0) return 0;
   if (map != mla::kMapNone) {
-    pb.map = map, pb.window = window, pb.sinks = sinks, pb.page_shift = __builtin_ctz(unsigned(page_size)), pb.pt_width = pt_width;
+    pb.window = window, pb.sinks = sinks, pb.page_shift = __builtin_ctz(unsigned(page_size)), pb.pt_width = pt_width;
     pb.requests = requests, pb.q_first = q_first, pb.q_indptr = q_indptr;
   }
   const mla::WsLayout L = mla::ws_layout(pb.n_cta, pb.items(), pb.heads_per_cta);
@@ -393,7 +404,7 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   // batches read the output of the schedule kernel.
   const bool inline_sched = schedules_itself(pb, precision, hpc);
   if (!inline_sched) {
-    mla::mla_schedule_kernel<<<1, mla::kSchedThreads, 0, st>>>(kv_lens, pb, header, cta_range, item_range, segs);
+    schedule_kernel(map)<<<1, mla::kSchedThreads, 0, st>>>(kv_lens, pb, header, cta_range, item_range, segs);
     MLA_CUDA(cudaGetLastError());
   }
 
@@ -420,12 +431,12 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   // few rows: four thread groups share a row's partials; many rows: one group per row keeps the CTAs small
   const unsigned rows = unsigned(batch) * unsigned(heads);
   if (rows <= 2u * unsigned(d->sm_count))
-    MLA_CUDA(launch_dependent(mla::mla_combine_sched_kernel<4>, dim3(rows), dim3(512), 0, st, pb,
+    MLA_CUDA(launch_dependent(combine_kernel<4>(map), dim3(rows), dim3(512), 0, st, pb,
                               static_cast<const int2*>(item_range), static_cast<const int*>(inline_sched ? kv_lens : nullptr),
                               static_cast<const float*>(lse_part),
                               static_cast<const float*>(o_part), out, out_f32, lse));
   else
-    MLA_CUDA(launch_dependent(mla::mla_combine_sched_kernel<1>, dim3(rows), dim3(128), 0, st, pb,
+    MLA_CUDA(launch_dependent(combine_kernel<1>(map), dim3(rows), dim3(128), 0, st, pb,
                               static_cast<const int2*>(item_range), static_cast<const int*>(inline_sched ? kv_lens : nullptr),
                               static_cast<const float*>(lse_part),
                               static_cast<const float*>(o_part), out, out_f32, lse));

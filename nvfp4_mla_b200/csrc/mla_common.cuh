@@ -50,7 +50,7 @@ struct Problem {
   int batch, heads, heads_per_cta, head_groups, splits, chunk, n_cta;
   // Windowed decode and query tokens of chunks (splits 1), see WindowMap. window 0: none. pt_width: columns of the page table.
   // kMapChunk: batch entry b is query token q_first + b of the `requests` requests whose tokens q_indptr delimits
-  int map, window, sinks, page_shift, pt_width, requests, q_first;
+  int window, sinks, page_shift, pt_width, requests, q_first;
   const int* q_indptr;
   __host__ __device__ long long items() const { return (long long)batch * splits * head_groups; }
 };
@@ -108,9 +108,6 @@ template <int MAP>
 __device__ __forceinline__ int sched_len(const int* kv_lens, const Problem& pb, int b) {
   if constexpr (MAP != kMapNone) return window_map<MAP>(kv_lens, pb, b).len;
   else return kv_lens[b];
-}
-__device__ __forceinline__ int sched_len(const int* kv_lens, const Problem& pb, int b) {
-  return pb.map == kMapChunk ? sched_len<kMapChunk>(kv_lens, pb, b) : pb.map == kMapWindow ? sched_len<kMapWindow>(kv_lens, pb, b) : kv_lens[b];
 }
 
 // 128-token tiles of (request, split) pair bz = b * splits + z: the split covers tokens [z * chunk, (z + 1) * chunk) of the request.
