@@ -132,8 +132,9 @@ NVFP4_MLA_API int nvfp4_mla_decode_window(const void* q_nope, const void* q_pe, 
  *
  * Where it is estimated to be faster (nvfp4_mla_extend_shares: 1, 0: not, -1: error; in the main chunks of more than a few tokens),
  * all rows of a request share one pass over its cache, which is dequantised once into the workspace: 1152 bytes per visible token,
- * of which there are at most batch * max_kv_len (and with a window at most batch * (window + sink_tokens + 256) + total_q), and as
- * many requests at a time as keep this below 8 GB.
+ * of which there are at most batch * max_kv_len (and with a window at most batch * (window + sink_tokens + 256) + total_q), for as
+ * many requests at a time as keep this below 8 GB (one at least). Beside that the workspace holds all query rows, 1156 bytes per
+ * query token and head (a request's rows rounded up to 128), and 40 MB of partial results.
  * (No counterpart in the reference, which decodes one query token per request.) */
 NVFP4_MLA_API int nvfp4_mla_extend_shares(int batch, int total_q, int heads, int max_kv_len, int window, int sink_tokens);
 NVFP4_MLA_API int64_t nvfp4_mla_extend_workspace_bytes(int batch, int total_q, int heads, int page_size, int page_table_width, int max_kv_len,

@@ -279,7 +279,8 @@ def extend(q_nope, q_pe, ckv_cache, ckv_sf_cache, kpe_cache, page_table, kv_lens
         qo_indptr: ``[batch + 1]`` int32, non-decreasing: request ``b`` has the query tokens ``qo_indptr[b] .. qo_indptr[b + 1]``.
         max_kv_len: an upper bound of ``kv_lens``, which with the shapes fixes the launch shape and the workspace. Without it the page
             table's width is the bound; nothing synchronises either way, and the call can be captured in a CUDA graph. (The workspace
-            holds up to 1152 bytes per token of the bound and request, at most 8 GB: a bound near the lengths saves memory.)
+            holds up to 1152 bytes per token of the bound and request, for as many requests at a time as stay below 8 GB, one at least;
+            1156 bytes per query token and head; and 40 MB. A bound near the lengths saves memory.)
         window, sink_tokens: with ``window > 0`` a token attends to the last ``window`` tokens up to its own position and to the first
             ``sink_tokens``; pages that no query of the call sees are not looked up.
 

@@ -574,10 +574,11 @@ int make_half_map(const void* base, int64_t rows, CUtensorMap* map) {
 // to 16000 tokens).
 //   by token: those of the decode kernels (wants_hm16), every query token a request
 //   shared  : 21 + 0.3 per thousand dequantised tokens + 4.2 per 256-token tile of the fullest pair + 0.2 per thousand rows
-// Measured (by token / shared), heads, requests, query tokens, tokens: 16,1,1,1000: 18 / 22; 16,64,1,4000: 61 / 173; 16,4,8,16000: 78 / 57;
-// 16,64,8,1000: 127 / 64; 32,16,4,4000: 88 / 56; 64,16,8,4000: 251 / 103; 128,16,1,4000: 65 / 57; 128,16,1,16000: 135 / 170;
-// 128,64,1,200: 54 / 27; 128,64,4,4000: 545 / 327. Over the 158 sizes the form that is taken costs 0.9 % more than the better one; the
-// constants are those of calls among others on the host, where a launch is 2 us and the second form has two more.
+// Measured (by token / shared), heads, requests, query tokens, tokens: 16,4,4,4000: 26 / 31; 16,64,1,4000: 63 / 180; 16,4,8,16000: 85 / 61;
+// 16,64,8,1000: 144 / 71; 32,16,4,4000: 92 / 61; 64,16,8,4000: 258 / 105; 128,16,1,4000: 73 / 64; 128,16,1,16000: 141 / 177;
+// 128,64,1,200: 53 / 30; 128,64,4,4000: 537 / 339. The constants are those of calls among others on the host, from when each form had
+// one launch more (two and three now). Over 248 sizes of these ranges the form that is taken costs 1.1 % more than the better one now;
+// it is wrong where the two are close, by 17 % at worst: the first of the sizes above takes the shared form.
 bool extend_shares(int batch, int total_q, int heads, int max_kv_len, int window, int sinks, const DeviceInfo& d) {
   if (d.ext_pairs < 2 || batch <= 0 || total_q <= 0) return false;
   if (heads % 16 != 0) return true;
@@ -620,14 +621,14 @@ int extend_shared(const void* q_nope, const void* q_pe, const uint8_t* ckv_cache
   P.q_scale = O.q_scale, P.ckv_scale = ckv_scale, P.lse_part = reinterpret_cast<float*>(ws + l.lse_part);
   P.o_part = reinterpret_cast<float*>(ws + l.o_part), P.out = static_cast<uint16_t*>(out), P.status = status;
   const int64_t units = int64_t(l.max_blocks) + int64_t(l.max_items) * (mla::kExtRows / mla::kExtQRows);
-  const int64_t resident = int64_t(d.sm_count) * (2048 / mla::kExtPrepThreads);
+  const int64_t most = int64_t(d.sm_count) * (2048 / mla::kExtPrepThreads);  // (eight CTAs per SM; their registers let five run at a time)
   for (int b = 0; b < batch; b += l.group) {
     E.batch = batch - b < l.group ? batch - b : l.group;
     E.kv_lens = kv_lens + b, E.indptr = qo_indptr ? qo_indptr + b : nullptr, E.first_q = qo_indptr ? 0 : b;
     E.edges = (b == 0 ? 1 : 0) | (b + l.group >= batch ? 2 : 0);
     O.page_table = page_table + b * page_table_stride;
     P.E = E;
-    mla::mla_extend_prep_kernel<<<unsigned(units < resident ? units : resident) + 1, mla::kExtPrepThreads, 0, st>>>(E, O);
+    mla::mla_extend_prep_kernel<<<unsigned(units < most ? units : most) + 1, mla::kExtPrepThreads, 0, st>>>(E, O);
     MLA_CUDA(cudaGetLastError());
     MLA_CUDA(launch_dependent_cluster(mla::mla_extend_kernel, dim3(unsigned(2 * l.pairs)), dim3(mla::kExtThreads), mla::ext_smem_bytes(), st, 2u,
                                       kv_map, q_map, P));

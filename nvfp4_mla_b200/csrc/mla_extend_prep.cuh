@@ -15,7 +15,7 @@
 //
 // Operands: the attention kernel multiplies FP16. Every visible token is dequantised once per call into a workspace row of 576 (latent
 // 512, rope 64, exact: e2m1 x e4m3 has six significant bits), every query row once into a row of the same shape, held times a power
-// of two that puts its maximum into [2^14, 2^15) (the latent part stays exact down to 2^-39 of the maximum) with the rope part times
+// of two that puts its maximum into [2^14, 2^15) (latent elements are exact from 2^-31 of the maximum up and off by 2^-25 at most below) with the rope part times
 // kpe_scale / ckv_scale, rounded to FP16. 1.5 KB per token, against 256 KB of operands that the attention loads per token and
 // 128-row tile, if it is read by many tiles.
 #pragma once

@@ -13,7 +13,7 @@
 //
 // What bounds it: the tensor pipe needs 36 * 64 + 32 * 64 = 4352 cycles per tile, shared memory 5690 (728 KB at 128 bytes per cycle: A and
 // B of the products 408, the loads 278, P 32; measured 5900 to 6200), and in calls of more than a few hundred us the 1 kW power
-// limit holds the clock at 1.57 to 1.65 GHz. 1024 query tokens of 128 heads behind 15360 others: 3.56 ms, 1.27 PFLOP/s, 0.93 of what the
+// limit holds the clock at 1.55 to 1.62 GHz. 1024 query tokens of 128 heads behind 15360 others: 3.56 ms, 1.27 PFLOP/s, 0.93 of what the
 // library's BF16 product sustains; 4 chunks of 512 of 16 heads behind 7680: 418 us of the call's 484, tensor pipe 73 % busy (ncu),
 // 76 MB from HBM, 10.7 TB/s from L2. The end of an item costs a pair 10000 to 12500 cycles (output, next query, pipeline filling).
 // Stalls that were taken out without the time changing, which is how the power limit shows: a thread of its own for the query's

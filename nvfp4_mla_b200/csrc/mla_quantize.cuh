@@ -13,10 +13,10 @@
 // one fused multiply-add, anything else by the real division. The block scale and the rope pair are treated alike; a
 // power-of-two rope scale needs no enclosure, its products are exact.
 //
-// 1152 bytes in, 352 bytes out per token, bound by instruction issue and the latency of the walk through the page tables (194 warp
-// instructions per token, 56 % of the issue slots): 274880 tokens in 82 us (63 at the measured copy bandwidth; 110 with a power of two as
-// ckv_scale, where more values tie); 100 with one instruction per product instead
-// of two products per instruction and 64-bit rows. Thirty-two tokens per warp with one walk through the page tables for all of them was slower (246.7 us).
+// 1152 bytes in, 352 bytes out per token, bound by instruction issue (1 048 576 tokens with a power of two as ckv_scale: 327 warp instructions
+// per token, 77 % of the issue slots): 596 415 tokens in 195 us (137 at the measured copy bandwidth), 220 with one instruction per product
+// instead of two products per instruction and 64-bit rows; 275 015 tokens 96 us, 114 with a power of two, where more values tie. Thirty-two
+// tokens per warp with one walk through the page tables for all of them was slower (246.7 us for the 596 415).
 // One warp per token per trip; lane l owns scale block l
 // (channels 16l .. 16l+15: two 16-byte loads, one 8-byte store, the warp writes the token's 256 packed bytes as one
 // contiguous run) and rope channels 2l, 2l+1.
@@ -266,9 +266,9 @@ mla_quantize_append_kernel(const __nv_bfloat16* __restrict__ ckv, const __nv_bfl
 // One warp per token per trip, lane l = scale block l, as above; a lane's normalised BF16 values sit in shared memory for the few that
 // have to be settled, the weights and the factors of the 128 block scales there too. A lane looks up the place of one of the warp's next
 // 32 tokens, so that the walk through the page tables is paid for once in 32 trips. 1512 bytes per token, bound by instruction issue and
-// the latency of a warp's chain of steps (348 warp instructions per token, 67 % of the issue slots): 274880 tokens in 128 us with
-// ckv_scale = 6.5 / (6 * 448) (63 at the measured copy bandwidth), 137 with a power of two, where a third of the block scales needs a
-// second term (172 with the enclosing products for these). Before: 166 and 188 with the enclosing products of the writer above and a walk per token; 345 with the norm in 64 bits
+// the latency of a warp's chain of steps (347 warp instructions per token, 67 % of the issue slots): 275 015 tokens in 134 us with
+// ckv_scale = 6.5 / (6 * 448) (63 at the measured copy bandwidth), 143 with a power of two, where a third of the block scales needs a
+// second term (172 with the enclosing products for these, the two here at 128 and 137 on that box). Before: 166 and 188 with the enclosing products of the writer above and a walk per token; 345 with the norm in 64 bits
 // throughout. Rows fetched ahead into shared memory (134), 40 warps per SM (171) and two CTAs per resident one (129.5) gained nothing.
 // ---------------------------------------------------------------------------------------------------------------
 template <bool INTERLEAVED>
