@@ -105,7 +105,7 @@ struct ExtRequest {
 };
 // index of request b's first query token; without an indptr every request has one
 __device__ __forceinline__ int ext_first(const ExtProblem& E, int b) { return E.indptr ? E.indptr[b] : E.first_q + b; }
-__device__ __forceinline__ int ext_blocks(int tokens) { return tokens > 0 ? (tokens - 1) / kExtBlock + 1 : 0; }
+__device__ __forceinline__ int ext_blocks(int tokens) { return int((uint32_t(tokens) + kExtBlock - 1) / kExtBlock); }  // (not negative)
 __device__ __forceinline__ ExtRequest ext_request(const ExtProblem& E, int b) {
   ExtRequest r;
   const int a = ext_first(E, b), z = ext_first(E, b + 1);
@@ -142,19 +142,27 @@ __device__ __forceinline__ void ext_tables(const ExtProblem& E, ExtTables& s) {
   constexpr int THREADS = kExtPrepThreads;
   const int tid = threadIdx.x;
   // A query index that runs backwards or past total_q could ask for more than there is room for. A request has less than 2^26 of
-  // either, so that a round's 256 requests may add up to 2^34: sums of 64 bits, and no further round after one without room.
+  // either, so that a round's 256 requests may add up to 2^34: sums of 64 bits, and no further round after one without room. Ordinary
+  // counts share one sum (two of 64 bits each time: 32 windowed single tokens of 128 heads 62.3 us instead of 62.0).
   int items = 0, blocks = 0;
   bool failed = false;
   for (int b0 = 0; b0 < E.batch; b0 += THREADS) {
     const int b = b0 + tid;
-    long long mine = 0, all_items, all_blocks;
+    long long mine = 0, ii, ib, all_items, all_blocks;
     ExtRequest r = {};
     if (b < E.batch) {
       r = ext_request(E, b);
       mine = ((long long)r.q * E.heads + kExtRows - 1) / kExtRows;
     }
-    const long long ii = items + block_scan<THREADS / 32>(mine, s.sums, all_items) - mine;
-    const long long ib = blocks + block_scan<THREADS / 32>((long long)r.blocks, s.sums, all_blocks) - r.blocks;
+    if (!__syncthreads_or(mine >= 1 << 22 || r.blocks >= 1 << 22)) {  // the sums are below 2^30
+      long long all;
+      const long long both = mine << 32 | r.blocks, at = block_scan<THREADS / 32>(both, s.sums, all) - both;
+      ii = at >> 32, ib = uint32_t(at), all_items = all >> 32, all_blocks = uint32_t(all);
+    } else {
+      ii = block_scan<THREADS / 32>(mine, s.sums, all_items) - mine;
+      ib = block_scan<THREADS / 32>((long long)r.blocks, s.sums, all_blocks) - r.blocks;
+    }
+    ii += items, ib += blocks;
     failed = items + all_items > E.max_items || blocks + all_blocks > E.max_blocks;
     if (failed) break;
     items += int(all_items), blocks += int(all_blocks);
@@ -194,7 +202,7 @@ __device__ __forceinline__ void ext_schedule(const ExtProblem& E, ExtTables& tab
       m.row0 = r.q0 * E.heads + m.r0, m.pos0 = r.pos0, m.shift = r.shift, m.block0 = tab.block0[lo];
       const int first = r.pos0 + m.r0 / E.heads, last = r.pos0 + (m.r0 + m.rows - 1) / E.heads;  // positions of its query tokens
       const int end = last + 1 < r.n ? last + 1 : r.n;                                           // tokens before it are seen
-      int e = ext_blocks(end - r.shift);                                                         // blocks up to there
+      int e = end > r.shift ? ext_blocks(end - r.shift) : 0;                                     // blocks up to there
       if (E.window > 0) {
         const long long begin = (long long)first - E.window + 1 - r.shift;
         const int t = begin > 0 ? int(begin / kExtBlock) : 0;
