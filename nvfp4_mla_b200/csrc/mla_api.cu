@@ -433,13 +433,13 @@ static int decode_impl(const void* q_nope, const void* q_pe, const uint8_t* ckv_
   if (rows <= 2u * unsigned(d->sm_count))
     MLA_CUDA(launch_dependent(combine_kernel<4>(map), dim3(rows), dim3(512), 0, st, pb,
                               static_cast<const int2*>(item_range), static_cast<const int*>(inline_sched ? kv_lens : nullptr),
-                              static_cast<const float*>(lse_part),
-                              static_cast<const float*>(o_part), out, out_f32, lse));
+                              static_cast<const float*>(lse_part), static_cast<const float*>(o_part), static_cast<const uint2*>(q_nope),
+                              static_cast<const uint32_t*>(q_pe), out, out_f32, lse));
   else
     MLA_CUDA(launch_dependent(combine_kernel<1>(map), dim3(rows), dim3(128), 0, st, pb,
                               static_cast<const int2*>(item_range), static_cast<const int*>(inline_sched ? kv_lens : nullptr),
-                              static_cast<const float*>(lse_part),
-                              static_cast<const float*>(o_part), out, out_f32, lse));
+                              static_cast<const float*>(lse_part), static_cast<const float*>(o_part), static_cast<const uint2*>(q_nope),
+                              static_cast<const uint32_t*>(q_pe), out, out_f32, lse));
   return 0;
 }
 

@@ -405,9 +405,8 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
     for (int l = 0; l < 4; ++l) ptx::prefetch_l2(reinterpret_cast<const char*>(qn) + 128 * l);
     if (half) ptx::prefetch_l2(qp);
     // Q as FP16 times `up`, into tensor memory / shared memory; returns the largest magnitude of the finite elements (the rope part
-    // times `ratio`). Non-finite elements become 0 and the rest of the row stays intact; with a MAP such a row is NaN (its largest magnitude
-    // is returned as infinite), as the definition has it and the form of the chunk attention that shares a pass does.
-    auto load_query = [&](float up) -> float {
+    // times `ratio`). Non-finite elements become 0: they have no meaningful result anyway, the rest of the row stays intact.
+    auto load_query = [&](float up) {
       uint32_t m2 = 0, m2p = 0;  // BF16 magnitudes, two at a time, ordered like integers
       auto clean = [](uint32_t x) {
         if ((x & 0x7F80u) == 0x7F80u) x &= 0xFFFF0000u;
@@ -415,9 +414,8 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
         return x;
       };
       auto two = [&](uint32_t x, float sc, uint32_t& mm) {
-        if constexpr (MAP != kMapNone) mm = ptx::max_s16x2(mm, x & 0x7FFF7FFFu);
         x = clean(x);
-        if constexpr (MAP == kMapNone) mm = ptx::max_s16x2(mm, x & 0x7FFF7FFFu);
+        mm = ptx::max_s16x2(mm, x & 0x7FFF7FFFu);
         return ptx::f32x2_to_f16x2(__uint_as_float(x << 16) * sc, __uint_as_float(x & 0xFFFF0000u) * sc);
       };
 #pragma unroll 1
@@ -446,9 +444,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
         }
         ptx::tmem_st32(tm_lane + H16Cols::QR, col);
       }
-      const uint32_t top = max(m2 << 16, m2 & 0xFFFF0000u), top_p = max(m2p << 16, m2p & 0xFFFF0000u);
-      if (MAP != kMapNone && max(top, top_p) >= 0x7F800000u) return INFINITY;
-      return fmaxf(__uint_as_float(top), __uint_as_float(top_p) * ratio);
+      return fmaxf(__uint_as_float(max(m2 << 16, m2 & 0xFFFF0000u)), __uint_as_float(max(m2p << 16, m2p & 0xFFFF0000u)) * ratio);
     };
     // The sign of the softmax scale goes into Q, so that a larger accumulator is always a larger score. The row is held times a power
     // of two, which the score's scale takes out again. Ordinary rows (maximum in [2^-8, 2^7]) are loaded in one pass, times 2^8:
@@ -470,8 +466,7 @@ __device__ __forceinline__ void h16_softmax_role(H16Smem& s, const DecodeParams&
       load_query(sign * __uint_as_float(uint32_t(127 - e) << 23));
     }
     // (never 0: a masked score is -inf and must stay so)
-    const float qa = MAP != kMapNone && !(amax < INFINITY) ? __uint_as_float(0x7FC00000u)
-                                                           : fmaxf(fabsf(P.sm_scale_log2) * P.ckv_scale * __uint_as_float(uint32_t(127 + e) << 23), 0x1p-149f);
+    const float qa = fmaxf(fabsf(P.sm_scale_log2) * P.ckv_scale * __uint_as_float(uint32_t(127 + e) << 23), 0x1p-149f);
     if (half) ptx::fence_proxy_async_smem();
     ptx::tmem_wait_st();
     ptx::tc_fence_before_sync();

@@ -232,9 +232,6 @@ __device__ __forceinline__ void vt_producer_role(VtSmem& s, const DecodeParams& 
 // `must_wait`: QK^T of the previous tile (barrier `prev_done`, `prev_parity`) still reads the old query; the rows are
 // fetched and scaled first, and the wait sits before the first store. Returns false if the wait gave up (`dead`: an
 // earlier one already has).
-// An element that is not finite counts as 0; with a MAP it makes the row NaN (by way of its score scale), as the definition has it and the
-// form of the chunk attention that shares a pass does.
-template <int MAP>
 __device__ __forceinline__ bool vt_load_query(VtSmem& s, const DecodeParams& P, const Seg& seg, int kt, int par, int lane, int quad,
                                               bool dead, bool must_wait, uint64_t* prev_done, uint32_t prev_parity) {
   const int n = kt >> 3, sub = kt & 7;
@@ -279,16 +276,10 @@ __device__ __forceinline__ bool vt_load_query(VtSmem& s, const DecodeParams& P, 
   e = e > e_pe - 5 ? e : e_pe - 5;
   e = e < -100 ? -100 : e;
   const float up = __uint_as_float(uint32_t(9 - e + 127) << 23);  // 2^(9 - e), exact: the row maximum lands in [512, 1024)
-  bool odd = false;  // whether this thread's part of the row has an element that is not finite
 #pragma unroll
   for (int i = 0; i < 64; ++i) {
     r[i] *= up;
-    if (!(fabsf(r[i]) < INFINITY)) r[i] = 0.f, odd = true;
-  }
-  if constexpr (MAP != kMapNone) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) odd |= !(fabsf(pe[j]) < INFINITY);
-    odd = (__ballot_sync(~0u, odd) >> (lane & 24) & 255u) != 0u;  // the row's eight threads
+    if (!(fabsf(r[i]) < INFINITY)) r[i] = 0.f;  // a non-finite query element has no meaningful result anyway; keep the rest of the row intact
   }
   {
     const bool ok = !dead && (!must_wait || ptx::mbar_wait(prev_done, prev_parity, &s.abort_flag));
@@ -336,8 +327,7 @@ __device__ __forceinline__ bool vt_load_query(VtSmem& s, const DecodeParams& P, 
     for (int j = 0; j < 4; ++j) h[j] = ptx::f32x2_to_f16x2(pe[2 * j] * up, pe[2 * j + 1] * up);
     *reinterpret_cast<uint4*>(s.qrope + n * 128 + (uint32_t(sub ^ (n & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
   }
-  if (sub == 0)
-    s.qa[par][n] = MAP != kMapNone && odd ? __uint_as_float(0x7FC00000u) : P.sm_scale_log2 * P.ckv_scale * __uint_as_float(uint32_t(e - 9 + 127) << 23);
+  if (sub == 0) s.qa[par][n] = P.sm_scale_log2 * P.ckv_scale * __uint_as_float(uint32_t(e - 9 + 127) << 23);
   ptx::fence_proxy_async_smem();
   ptx::bar_sync(2, 128);
   // scale factors of B: pass p multiplies K with B rows [terms 2p | 2p + 1] x 16 heads; the scale word of row i for the
@@ -452,7 +442,7 @@ __device__ __forceinline__ void vt_k_role(VtSmem& s, const DecodeParams& P, int 
     if (seg.ntiles <= 0) continue;
     // the previous tile's QK^T must be done reading the query before the new one overwrites it (waited for inside,
     // after the rows have been fetched)
-    if (!vt_load_query<MAP>(s, P, seg, quad * 32 + lane, seg_count & 3, lane, quad, dead, it != 0, &s.k_free[(it - 1) & 1], ((it - 1) >> 1) & 1))
+    if (!vt_load_query(s, P, seg, quad * 32 + lane, seg_count & 3, lane, quad, dead, it != 0, &s.k_free[(it - 1) & 1], ((it - 1) >> 1) & 1))
       return;
     ++seg_count;
     const int2 gap = MAP ? seg_window<MAP>(P, seg.b).dead : make_int2(0, 0);

@@ -160,11 +160,11 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 }
 
 // Shared tail: `n_parts` partials whose (lse, o-row) addresses are produced by `lse_of(i)` / `o_of(i)`.
-// `weights` and `partial` are shared-memory scratch of at least n_parts (up to kCombineMaxParts) and 3 x 128 x 4 floats.
+// `weights` and `partial` are shared-memory scratch of at least n_parts (up to kCombineMaxParts) and 3 x 128 x 4 floats. With `nan` the row is NaN.
 constexpr int kCombineMaxParts = 512;
 template <int GROUPS, class LseOf, class OOf>
 __device__ __forceinline__ void merge_row(int n_parts, LseOf lse_of, OOf o_of, long long row, void* out_bf16,
-                                          float* out_f32, float* lse_out, float* weights, float4* partial) {
+                                          float* out_f32, float* lse_out, float* weights, float4* partial, bool nan = false) {
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 7, t = threadIdx.x & 127;
   // The first batch of rows is requested before the weights are known (they need the lse values, another round trip to
   // memory): a row with a handful of partials, the common case, then costs one memory latency instead of two. A partial
@@ -185,6 +185,7 @@ __device__ __forceinline__ void merge_row(int n_parts, LseOf lse_of, OOf o_of, l
     if (threadIdx.x < 32 && i < kCombineMaxParts) weights[i] = wl;
   }
   den = warp_sum(den);
+  if (nan) den = __uint_as_float(0x7FC00000u);
   __syncthreads();
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float w, const float4& v) {
@@ -217,7 +218,7 @@ __device__ __forceinline__ void merge_row(int n_parts, LseOf lse_of, OOf o_of, l
       acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
     }
   }
-  const float s = den > 0.f ? 1.f / den : 0.f;
+  const float s = den == 0.f ? 0.f : 1.f / den;  // (NaN stays NaN)
   acc.x *= s, acc.y *= s, acc.z *= s, acc.w *= s;
   if (out_bf16)
     reinterpret_cast<uint2*>(out_bf16)[row * (CKV / 4) + t] = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
@@ -225,12 +226,15 @@ __device__ __forceinline__ void merge_row(int n_parts, LseOf lse_of, OOf o_of, l
   if (lse_out && t == 0) lse_out[row] = den == 0.f ? -INFINITY : M + log2f(den);  // (NaN stays NaN: no later merge takes the row for an empty one)
 }
 
-// Partials addressed through the schedule (what the decode kernel wrote).
+// Partials addressed through the schedule (what the decode kernel wrote). The decode kernels take a query element that is not finite as 0. With a
+// MAP such a row is NaN where it sees a token, as the definition has it and the form of the chunk attention that shares a pass does: the row
+// is looked at here, beside the chain of loads that finds the partials. (In the decode kernels' query loads the same cost 64 requests of 16
+// heads over 4096 tokens 1.4 us of 58.4.)
 template <int GROUPS, int MAP>
 __global__ void __launch_bounds__(128 * GROUPS)
 mla_combine_sched_kernel(Problem pb, const int2* __restrict__ item_range, const int* __restrict__ kv_lens,
-                         const float* __restrict__ lse_part, const float* __restrict__ o_part, void* out_bf16, float* out_f32,
-                         float* lse_out) {
+                         const float* __restrict__ lse_part, const float* __restrict__ o_part, const uint2* __restrict__ q_nope,
+                         const uint32_t* __restrict__ q_pe, void* out_bf16, float* out_f32, float* lse_out) {
   __shared__ int slots[kCombineMaxParts];
   __shared__ int n_parts_s;
   __shared__ float weights[kCombineMaxParts];
@@ -241,6 +245,12 @@ mla_combine_sched_kernel(Problem pb, const int2* __restrict__ item_range, const 
   const long long row = blockIdx.x;
   const int b = int(row / pb.heads), h = int(row % pb.heads);
   const int N = pb.heads_per_cta, hg = h / N, n = h % N;
+  uint2 qn = make_uint2(0u, 0u);
+  uint32_t qp = 0u;
+  if constexpr (MAP != kMapNone) {
+    if (threadIdx.x < CKV / 4) qn = __ldg(q_nope + row * (CKV / 4) + threadIdx.x);
+    if (threadIdx.x < KPE / 2) qp = __ldg(q_pe + row * (KPE / 2) + threadIdx.x);
+  }
   if (threadIdx.x < 32) {  // enumerate the row's partial slots: splits z, CTAs c0..c1 of item (b, z, hg)
     // Without a schedule kernel (kv_lens given: the decode kernel derived its schedule by itself) the CTA that holds
     // the first tile of an item has written the item's CTA range; an item without tiles has none, which the lengths tell.
@@ -274,12 +284,18 @@ mla_combine_sched_kernel(Problem pb, const int2* __restrict__ item_range, const 
     }
     if (threadIdx.x == 0) n_parts_s = count < kCombineMaxParts ? count : kCombineMaxParts;
   }
-  __syncthreads();
+  bool nan = false;
+  if constexpr (MAP != kMapNone) {
+    auto odd = [](uint32_t x) { return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u; };  // either of two BF16 numbers
+    nan = __syncthreads_or(odd(qn.x) || odd(qn.y) || odd(qp));
+  } else {
+    __syncthreads();
+  }
   const int n_parts = n_parts_s;
   ptx::grid_dependency_wait();
   merge_row<GROUPS>(
       n_parts, [&](int i) { return lse_part[(long long)slots[i] * N + n]; },
-      [&](int i) { return o_part + ((long long)slots[i] * N + n) * CKV; }, row, out_bf16, out_f32, lse_out, weights, partial);
+      [&](int i) { return o_part + ((long long)slots[i] * N + n) * CKV; }, row, out_bf16, out_f32, lse_out, weights, partial, nan && n_parts > 0);
 }
 
 // Dense partials: part i holds o rows at o_part + i * o_stride (floats) and lse values at lse_part + i * lse_stride. The
